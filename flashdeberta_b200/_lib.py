@@ -11,10 +11,10 @@ _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libfdb_b200.so")
 
 FDB_OK, FDB_ERR_ALIGNMENT = 0, -3
-FDB_BF16, FDB_FP32, FDB_E4M3 = 0, 1, 2
+FDB_BF16, FDB_FP32, FDB_E4M3, FDB_FP16, FDB_INT8 = 0, 1, 2, 3, 4
 FDB_DEV_TIMEOUT, FDB_DEV_BAD_SEQLEN, FDB_DEV_BAD_INDEX, FDB_DEV_BAD_MASK = 1, 2, 4, 8
 STATIC_SCRATCH_BYTES = 8 << 20
-ABI_VERSION = 5
+ABI_VERSION = 6
 PREPARED_SCHEDULE, PREPARED_TABLES = 1, 2  # fdb_attn_params.prepared
 TUNE_ONE_LAUNCH, TUNE_TWO_LAUNCHES = 1, 2  # fdb_attn_params.tune
 
@@ -53,6 +53,46 @@ class QuantizeAttnParams(C.Structure):
         ("amax_bytes", C.c_uint64)]
 
 
+class ResidualNormParams(C.Structure):
+    """Mirror of ``fdb_residual_norm_params``."""
+
+    _fields_ = [("struct_bytes", C.c_uint32), ("dtype", C.c_int32)] + [(n, C.c_void_p) for n in (
+        "x", "residual", "weight", "bias", "post_weight", "post_bias", "gate", "normed", "stream", "stats")] + [
+        ("rows", C.c_int64), ("gate_rows", C.c_int64), ("hidden", C.c_int32), ("param_dtype", C.c_int32), ("gate_dtype", C.c_int32),
+        ("rms", C.c_int32), ("residual_scale", C.c_float), ("eps", C.c_float)]
+
+
+class ResidualNormBwdParams(C.Structure):
+    """Mirror of ``fdb_residual_norm_bwd_params``."""
+
+    _fields_ = [("struct_bytes", C.c_uint32), ("reserved", C.c_int32), ("fwd", C.POINTER(ResidualNormParams))] + [(n, C.c_void_p) for n in (
+        "dnormed", "dstream", "dx", "dresidual", "dweight", "dbias", "dpost_weight", "dpost_bias", "dgate", "workspace")] + [
+        ("workspace_bytes", C.c_uint64)]
+
+
+class LinearInt8Params(C.Structure):
+    """Mirror of ``fdb_linear_int8_params``."""
+
+    _fields_ = [("struct_bytes", C.c_uint32), ("x_dtype", C.c_int32), ("x", C.c_void_p), ("x_pitch", C.c_int64), ("x_scale", C.c_void_p),
+                ("weight", C.c_void_p), ("weight_pitch", C.c_int64), ("weight_scale", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p),
+                ("rows", C.c_int64), ("in_features", C.c_int32), ("out_features", C.c_int32), ("bias_dtype", C.c_int32),
+                ("out_dtype", C.c_int32), ("gelu", C.c_int32), ("reserved", C.c_int32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("status", C.c_void_p)]
+
+
+class GradTensor(C.Structure):
+    """Mirror of ``fdb_grad_tensor``."""
+
+    _fields_ = [("data", C.c_void_p), ("out", C.c_void_p), ("count", C.c_int64), ("dtype", C.c_int32), ("out_dtype", C.c_int32)]
+
+
+class ClipGradsParams(C.Structure):
+    """Mirror of ``fdb_clip_grads_params``."""
+
+    _fields_ = [("struct_bytes", C.c_uint32), ("n_tensors", C.c_int32), ("tensors", C.c_void_p), ("norm_type", C.c_int32), ("scale", C.c_int32),
+                ("max_norm", C.c_double), ("norm", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 EXPORTS = (
     "fdb_abi_version", "fdb_last_error", "fdb_status_string", "fdb_build_bucket_lut", "fdb_relative_index",
     "fdb_attn_workspace_bytes", "fdb_attn_fwd", "fdb_attn_fwd_static", "fdb_attn_fwd_check", "fdb_relative_index_matrix",
@@ -60,7 +100,8 @@ EXPORTS = (
     "fdb_attn_bwd_probs", "fdb_attn_bwd_bucket_sums", "fdb_expanded_rows", "fdb_expand_tables", "fdb_encoder_create",
     "fdb_encoder_destroy", "fdb_encoder_workspace_bytes", "fdb_encoder_forward", "fdb_attn_bwd_workspace_bytes", "fdb_attn_bwd",
     "fdb_lengths_from_mask", "fdb_column_sums_workspace_bytes", "fdb_column_sums", "fdb_quantize_attn",
-    "fdb_projected_forward",
+    "fdb_projected_forward", "fdb_residual_norm", "fdb_residual_norm_bwd_workspace_bytes", "fdb_residual_norm_bwd", "fdb_quantize_int8",
+    "fdb_linear_int8_workspace_bytes", "fdb_linear_int8", "fdb_clip_grads_workspace_bytes", "fdb_clip_grads",
 )
 
 _lib = None
@@ -137,6 +178,14 @@ def load() -> C.CDLL:
     lib.fdb_expand_tables.restype = C.c_int
     lib.fdb_expand_tables.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32,
                                       C.c_int32, C.c_void_p]
+    for name in ("fdb_residual_norm", "fdb_residual_norm_bwd", "fdb_linear_int8", "fdb_clip_grads"):  # (const struct *, stream)
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.c_void_p, C.c_void_p]
+    for name in ("fdb_residual_norm_bwd_workspace_bytes", "fdb_linear_int8_workspace_bytes", "fdb_clip_grads_workspace_bytes"):
+        getattr(lib, name).restype = C.c_uint64
+        getattr(lib, name).argtypes = [C.c_void_p]
+    lib.fdb_quantize_int8.restype = C.c_int
+    lib.fdb_quantize_int8.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
     # the encoder's structs are in engine.py
     lib.fdb_encoder_create.restype = C.c_int
     lib.fdb_encoder_create.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]

@@ -111,5 +111,6 @@ int launch_relative_index_matrix(const int16_t* lut, int32_t d_min, int32_t len,
                                  void* stream);
 int launch_quantize_e4m3(const void* x, int64_t rows, int64_t row_stride, int64_t head_stride, const int32_t* slab_start,
                          int32_t n_slabs, int32_t heads, int32_t head_dim, void* y, float* scale, void* stream);
+int launch_quantize_int8(const void* x, int dtype, int64_t rows, int cols, void* y, int64_t pitch, float* scale, void* stream);
 
 }  // namespace fdb

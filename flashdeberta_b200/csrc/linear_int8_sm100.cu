@@ -1,0 +1,405 @@
+// out = act(x_scale[m] * weight_scale[n] * sum_k x[m][k] weight[n][k] + bias[n]) in 8-bit integers for sm_100a: the linear layers of an
+// encoder whose weights are held in 8 bits (fdb_linear_int8).
+//
+// tcgen05.mma kind::i8, exact 32-bit sums in tensor memory.  The structure is linear_sm100.cu's: persistent grid; a tile is 128 rows
+// (CG = 1) or 256 rows (CG = 2, a pair of CTAs on two SMs) x BN output features, K in steps of 128 bytes through a ring of stages:
+//   warp 0  TMA, the CTA's 128 x 128 bytes of x and its BN / CG rows of the weight; what lies behind the ends arrives as zeros
+//   warp 1  (of the pair's even CTA) tcgen05.mma, four per stage; two accumulators in tensor memory
+//   warps 2-9: epilogue, two warps per 32-lane quarter of tensor memory: both scales, bias, activation in fp32, one rounding
+// A stage holds as many bytes as in the bf16 kernel and takes as many clocks (measured), for twice the products.
+// Every wait is bounded; on a timeout the CTA raises FDB_DEV_TIMEOUT in the status word, frees its tensor memory and returns.
+// No TMA multicast.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "gelu.cuh"
+#include "internal.h"
+#include "launch.h"
+#include "row_team.cuh"
+#include "sm100_ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace fdb {
+namespace {
+
+using namespace ptx;
+
+constexpr int kBM = 128, kBK = 128;
+constexpr int kThreads = 320;
+constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 8;
+
+struct Int8Args {
+  CUtensorMap tm_x, tm_w;
+  const float *x_scale, *w_scale;
+  const void* bias;
+  void* out;
+  int32_t* status;
+  int64_t rows;
+  int k, n, tiles_n;
+  bool bias_fp32;  // else of the output's type
+  bool wide;       // rows of the output start on 16 bytes, scales and bias too, and n is a multiple of 8
+};
+
+template <int CG, int BN> struct Tile {
+  static constexpr uint32_t kBytesA = kBM * kBK, kBytesW = BN / CG * kBK, kStageBytes = kBytesA + kBytesW;
+  static constexpr int kStages = BN == 64 ? 6 : (BN == 256 ? 6 : (CG == 2 ? 8 : 6));
+  static constexpr uint32_t kPitch = 33;  // words of a row of the epilogue's transposition
+  static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemBars = kSmemTurn + kEpiWarps * 32 * kPitch * 4;
+  enum : uint32_t { kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2, kNumBars = 2 * kStages + 4 };
+  static constexpr uint32_t kSmemBytes = kSmemBars + 8 * kNumBars + 16 + 1024;  // + tensor-memory slot, abort flag, alignment slack
+  static constexpr uint32_t kTmemCols = 2 * BN;
+};
+
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A pair of columns: the sums scaled, bias added, activation.
+template <bool GELU> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
+  const uint64_t acc = pack_f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1));
+  const uint64_t v = fma_f32x2(mul_f32x2(acc, w_scale), x_scale, bias);
+  return GELU ? gelu_tail2(v) : v;
+}
+
+template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a, int n) {
+  if (a.bias == nullptr) return 0.f;
+  return a.bias_fp32 ? __ldg(static_cast<const float*>(a.bias) + n) : to_float<T>(static_cast<const T*>(a.bias)[n]);
+}
+
+// 32 columns of a row per thread, the thread's own row; every column exists and rows may be written in 16-byte pieces.
+template <typename T, bool GELU>
+__device__ __forceinline__ void store_direct(const Int8Args& a, const uint32_t (&acc)[32], int64_t row, int n0, float x_scale, bool live) {
+  const uint64_t sx = pack_f32x2(x_scale, x_scale);
+  T* out = static_cast<T*>(a.out) + row * a.n + n0;
+#pragma unroll
+  for (int c = 0; c < 32; c += 8) {
+    float ws[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    *reinterpret_cast<float4*>(ws) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c));
+    *reinterpret_cast<float4*>(ws + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c + 4));
+    if (a.bias != nullptr) {
+      if (a.bias_fp32) {
+        *reinterpret_cast<float4*>(b) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c));
+        *reinterpret_cast<float4*>(b + 4) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c + 4));
+      } else if constexpr (sizeof(T) == 2) {
+        RowWords<T> r;
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + n0 + c));
+        r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+        unpack(r, b);
+      }
+    }
+    uint32_t o[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float v0, v1;
+      unpack_f32x2(finish_pair<GELU>(acc[c + e], acc[c + e + 1], pack_f32x2(ws[e], ws[e + 1]), sx, pack_f32x2(b[e], b[e + 1])), v0, v1);
+      if constexpr (sizeof(T) == 4) {
+        o[e] = __float_as_uint(v0);
+        o[e + 1] = __float_as_uint(v1);
+      } else {
+        o[e >> 1] = pack_pair<T>(v0, v1);
+      }
+    }
+    if (live) {
+      *reinterpret_cast<uint4*>(out + c) = make_uint4(o[0], o[1], o[2], o[3]);
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out + c + 4) = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  }
+}
+
+// The same where a row starts anywhere or columns are missing: through shared memory, a row of 32 columns at a time across the lanes.
+// (A thread writing its own row element by element would touch 32 sectors with every store.)
+template <typename T, bool GELU>
+__device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, uint32_t* turn, int lane) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) turn[lane * 33 + c] = acc[c];
+  __syncwarp();
+  const int n = n0 + lane;
+  const bool has = n < a.n;
+  const float ws = has ? __ldg(a.w_scale + n) : 0.f, b = has ? bias_at<T>(a, n) : 0.f;
+  const uint64_t ws2 = pack_f32x2(ws, ws), b2 = pack_f32x2(b, b);
+  T* out = static_cast<T*>(a.out) + row0 * a.n + n;
+#pragma unroll 4
+  for (int r = 0; r < 32; r += 2) {
+    const float s0 = __shfl_sync(0xffffffffu, x_scale, r), s1 = __shfl_sync(0xffffffffu, x_scale, r + 1);
+    float v0, v1;
+    unpack_f32x2(finish_pair<GELU>(turn[r * 33 + lane], turn[(r + 1) * 33 + lane], ws2, pack_f32x2(s0, s1), b2), v0, v1);
+    if (has && row0 + r < a.rows) out[(int64_t)r * a.n] = from_float<T>(v0);
+    if (has && row0 + r + 1 < a.rows) out[(int64_t)(r + 1) * a.n] = from_float<T>(v1);
+  }
+  __syncwarp();
+}
+
+template <int CG, int BN, typename OUT, bool GELU>
+__global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_constant__ Int8Args args) {
+  using T = Tile<CG, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem - smem_u32(smem_raw));
+  const int tid = threadIdx.x, warp = (int)uniform(uint32_t(tid) >> 5), lane = tid & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+
+  auto bar = [&](uint32_t i) -> uint32_t { return smem + T::kSmemBars + 8u * i; };
+  const uint32_t tmem_slot = smem + T::kSmemBars + 8u * T::kNumBars;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_gen + T::kSmemBars + 8u * T::kNumBars + 8u);
+
+  if (tid == 0) {
+    *abort_flag = 0u;
+    for (uint32_t i = 0; i < T::kNumBars; ++i) mbar_init(bar(i), (i >= T::kBarAccEmpty) ? uint32_t(kEpiWarps * CG) : 1u);
+    fence_barrier_init();
+    tma_prefetch_desc(&args.tm_x);
+    tma_prefetch_desc(&args.tm_w);
+  }
+  if (warp == kMmaWarp) {
+    if constexpr (CG == 2) { tmem_alloc_pair(tmem_slot, T::kTmemCols); tmem_relinquish_pair(); }
+    else { tmem_alloc(tmem_slot, T::kTmemCols); tmem_relinquish(); }
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync(); else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = uniform(*reinterpret_cast<volatile uint32_t*>(smem_gen + T::kSmemBars + 8u * T::kNumBars));
+
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int kblocks = (args.k + kBK - 1) / kBK;
+  const int num_tiles = (int)((args.rows + kBM * CG - 1) / (kBM * CG)) * args.tiles_n;
+  auto load_w = [&](uint32_t st, int kb, int n0) {
+    const uint32_t w = smem + st * T::kStageBytes + T::kBytesA;
+    if constexpr (CG == 2) {
+      if (rank == 0) mbar_expect_tx(bar(T::kBarFull + st), 2 * T::kStageBytes);
+      tma_load_2d_pair(w, &args.tm_w, bar(T::kBarFull + st), kb * kBK, n0);
+    } else {
+      mbar_expect_tx(bar(T::kBarFull + st), T::kStageBytes);
+      tma_load_2d(w, &args.tm_w, bar(T::kBarFull + st), kb * kBK, n0);
+    }
+  };
+  // The weight is nobody's output: its first stages are on their way before the kernel in front, which rounds x, has finished.
+  const int early = kblocks < T::kStages ? kblocks : T::kStages;
+  if (warp == kTmaWarp) {
+    const int n0 = (first % args.tiles_n) * BN + int(rank) * (BN / CG);
+#pragma unroll 1
+    for (int kb = 0; kb < early; ++kb)
+      if (elect_one()) load_w(uint32_t(kb), kb, n0);
+  }
+  grid_wait();
+  bool ok = true;
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (ok) ok = mbar_wait_warp(b, parity, abort_flag);
+  };
+
+  if (warp == kTmaWarp) {
+    uint32_t st = 0, phase = 0;
+    int skip = early;  // stages whose weights are already on their way
+#pragma unroll 1
+    for (int tile = first; tile < num_tiles && ok; tile += step) {
+      const int m0 = (tile / args.tiles_n) * (kBM * CG) + int(rank) * kBM;
+      const int n0 = (tile % args.tiles_n) * BN + int(rank) * (BN / CG);
+#pragma unroll 1
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (skip == 0) wait(bar(T::kBarEmpty + st), phase ^ 1u);  // (the first round passes at once)
+        if (!ok) break;
+        if (elect_one()) {
+          if (skip == 0) load_w(st, kb, n0);
+          if constexpr (CG == 2) tma_load_2d_pair(smem + st * T::kStageBytes, &args.tm_x, bar(T::kBarFull + st), kb * kBK, m0);
+          else tma_load_2d(smem + st * T::kStageBytes, &args.tm_x, bar(T::kBarFull + st), kb * kBK, m0);
+        }
+        skip -= skip > 0 ? 1 : 0;
+        if (++st == T::kStages) { st = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (rank == 0) {
+      const uint32_t idesc = instr_desc_s8(kBM * CG, BN);
+      const uint64_t da0 = smem_desc_sw128(smem, 1024, 16), dw0 = smem_desc_sw128(smem + T::kBytesA, 1024, 16);
+      uint32_t st = 0, phase = 0, local = 0;
+#pragma unroll 1
+      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+        const uint32_t acc = local & 1u, d = tmem_base + acc * BN;
+        wait(bar(T::kBarAccEmpty + acc), ((local >> 1) & 1u) ^ 1u);  // the epilogue has read this accumulator
+        tc_fence_after();
+#pragma unroll 1
+        for (int kb = 0; kb < kblocks; ++kb) {
+          wait(bar(T::kBarFull + st), phase);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = da0 + uint64_t(st * (T::kStageBytes >> 4)), dw = dw0 + uint64_t(st * (T::kStageBytes >> 4));
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              const uint32_t more = (kb > 0 || ks > 0) ? 1u : 0u;
+              if constexpr (CG == 2) mma_s8_pair(d, da + uint64_t((ks * 32) >> 4), dw + uint64_t((ks * 32) >> 4), idesc, more);
+              else mma_s8(d, da + uint64_t((ks * 32) >> 4), dw + uint64_t((ks * 32) >> 4), idesc, more);
+            }
+            if constexpr (CG == 2) mma_commit_pair(bar(T::kBarEmpty + st)); else mma_commit(bar(T::kBarEmpty + st));
+            if (kb == kblocks - 1) { if constexpr (CG == 2) mma_commit_pair(bar(T::kBarAccFull + acc)); else mma_commit(bar(T::kBarAccFull + acc)); }
+          }
+          if (++st == T::kStages) { st = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;                // the 32 tensor-memory lanes this warp may read
+    const int half = (warp - kEpiWarp0) >> 2;    // which half of the tile's columns
+    constexpr int kChunks = BN / 64;             // 32 columns at a time
+    const uint32_t tmem_lane = tmem_base + (uint32_t(quarter * 32) << 16);
+    uint32_t* turn = reinterpret_cast<uint32_t*>(smem_gen + T::kSmemTurn) + (warp - kEpiWarp0) * 32 * T::kPitch;
+    uint32_t acc_empty[2] = {bar(T::kBarAccEmpty), bar(T::kBarAccEmpty + 1)};
+    if constexpr (CG == 2) { acc_empty[0] = map_to_rank(acc_empty[0], 0); acc_empty[1] = map_to_rank(acc_empty[1], 0); }
+    uint32_t local = 0;
+#pragma unroll 1
+    for (int tile = first; tile < num_tiles; tile += step, ++local) {
+      const int64_t row0 = (int64_t)(tile / args.tiles_n) * (kBM * CG) + int(rank) * kBM + quarter * 32;
+      const int n0 = (tile % args.tiles_n) * BN + half * (BN / 2);
+      const uint32_t acc = local & 1u;
+      const bool live = row0 + lane < args.rows;
+      const float x_scale = live ? __ldg(args.x_scale + row0 + lane) : 0.f;
+      wait(bar(T::kBarAccFull + acc), (local >> 1) & 1u);
+      tc_fence_after();
+#pragma unroll 1
+      for (int ch = 0; ch < kChunks; ++ch) {
+        uint32_t a[32];
+        if (ok) {  // whole warps execute the load, whatever their rows
+          tmem_ld32(tmem_lane + acc * BN + uint32_t(half * (BN / 2) + ch * 32), a);
+          tmem_wait_ld();
+        }
+        if (ch == kChunks - 1) {  // the accumulator is in registers: the next tile but one may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) { if constexpr (CG == 2) mbar_arrive_cluster(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
+        }
+        const int n = n0 + ch * 32;
+        if (!ok || n >= args.n || row0 >= args.rows) continue;
+        if (args.wide && n + 32 <= args.n) store_direct<OUT, GELU>(args, a, row0 + lane, n, x_scale, live);
+        else store_turned<OUT, GELU>(args, a, row0, n, x_scale, turn, lane);
+      }
+    }
+  }
+
+  // ---- teardown ----
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    if (tid == 0 && args.status != nullptr) atomicOr(reinterpret_cast<unsigned int*>(args.status), FDB_DEV_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies and MMAs in flight get a bounded time to land
+    __syncthreads();
+  }
+  if constexpr (CG == 2) {
+    cluster_sync();  // the pair's arrivals on this CTA's barriers have landed, and both are done with tensor memory
+    if (warp == kMmaWarp) tmem_dealloc_pair(tmem_base, T::kTmemCols);
+  } else {
+    if (warp == kMmaWarp) tmem_dealloc(tmem_base, T::kTmemCols);
+  }
+}
+
+template <int CG, int BN, typename OUT, bool GELU>
+int launch(const Int8Args& a, int grid, bool chained, cudaStream_t stream) {
+  static std::atomic<uint64_t> smem_done{0};
+  auto kernel = linear_int8_kernel<CG, BN, OUT, GELU>;
+  cudaError_t e = allow_smem(smem_done, reinterpret_cast<const void*>(kernel), (int)Tile<CG, BN>::kSmemBytes);
+  if (e == cudaSuccess) e = launch_kernel<Int8Args>(kernel, a, dim3((unsigned)grid), kThreads, Tile<CG, BN>::kSmemBytes, chained, stream, CG);
+  if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "linear_int8 launch: %s", cudaGetErrorString(e));
+  return FDB_OK;
+}
+
+template <int CG, int BN>
+int launch_type(const Int8Args& a, int grid, int out_dtype, bool gelu, bool chained, cudaStream_t s) {
+#define FDB_INT8_OUT(OUT) (gelu ? launch<CG, BN, OUT, true>(a, grid, chained, s) : launch<CG, BN, OUT, false>(a, grid, chained, s))
+  if (out_dtype == FDB_BF16) return FDB_INT8_OUT(__nv_bfloat16);
+  return out_dtype == FDB_FP16 ? FDB_INT8_OUT(__half) : FDB_INT8_OUT(float);
+#undef FDB_INT8_OUT
+}
+
+// Tile shapes, with clocks per 128 of K and clocks a launch adds on top, as in linear_sm100.cu.
+struct Config { int cg, bn, clocks, extra; };
+constexpr Config kConfigs[] = {{2, 256, 540, 2600}, {2, 128, 300, 1600}, {1, 128, 340, 1500}, {1, 64, 350, 600}};
+
+bool float_type(int t) { return t == FDB_BF16 || t == FDB_FP16 || t == FDB_FP32; }
+unsigned type_bytes(int t) { return t == FDB_FP32 ? 4u : 2u; }
+int64_t pitch_of(const fdb_linear_int8_params& p) { return (int64_t(p.in_features) + 15) / 16 * 16; }
+uint64_t rows_bytes(const fdb_linear_int8_params& p) { return (uint64_t(p.rows) * pitch_of(p) + 255) / 256 * 256; }
+
+int validate_int8(const fdb_linear_int8_params* p) {
+  if (p == nullptr || p->struct_bytes != sizeof(fdb_linear_int8_params))
+    return fail(FDB_ERR_INVALID_ARGUMENT, "fdb_linear_int8_params: NULL or struct_bytes %u != %zu", p ? p->struct_bytes : 0u, sizeof(fdb_linear_int8_params));
+  if ((p->x_dtype != FDB_INT8 && !float_type(p->x_dtype)) || !float_type(p->out_dtype) || (p->bias != nullptr && !float_type(p->bias_dtype)))
+    return fail(FDB_ERR_INVALID_ARGUMENT, "linear_int8: types %d, %d, %d", p->x_dtype, p->out_dtype, p->bias_dtype);
+  if (p->bias != nullptr && p->bias_dtype != FDB_FP32 && p->bias_dtype != p->out_dtype)
+    return fail(FDB_ERR_INVALID_ARGUMENT, "linear_int8: the bias is of the output's type or fp32");
+  if (p->rows < 0 || p->in_features <= 0 || p->out_features <= 0)
+    return fail(FDB_ERR_INVALID_ARGUMENT, "linear_int8: %lld rows, %d -> %d features", (long long)p->rows, p->in_features, p->out_features);
+  if (p->rows > (int64_t(1) << 31) - 512 || p->in_features > 131071 || p->out_features > (1 << 30))
+    return fail(FDB_ERR_LIMIT, "linear_int8: %lld rows, %d -> %d features (an int32 sum holds 131071 products)", (long long)p->rows, p->in_features, p->out_features);
+  return FDB_OK;
+}
+
+}  // namespace
+}  // namespace fdb
+
+using namespace fdb;
+
+extern "C" FDB_API uint64_t fdb_linear_int8_workspace_bytes(const fdb_linear_int8_params* p) {
+  clear_error();
+  if (validate_int8(p) != FDB_OK || p->x_dtype == FDB_INT8 || p->rows == 0) return 0;
+  return rows_bytes(*p) + uint64_t(p->rows) * sizeof(float);
+}
+
+extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* stream) {
+  clear_error();
+  int rc = validate_int8(p);
+  if (rc != FDB_OK) return rc;
+  const bool given = p->x_dtype == FDB_INT8;
+  if (p->x == nullptr || p->weight == nullptr || p->weight_scale == nullptr || p->out == nullptr || (given && p->x_scale == nullptr))
+    return fail(FDB_ERR_INVALID_ARGUMENT, "linear_int8: x, weight, their scales and out must not be NULL");
+  if (p->weight_pitch < p->in_features || (given && p->x_pitch < p->in_features))
+    return fail(FDB_ERR_INVALID_ARGUMENT, "linear_int8: rows shorter than %d features", p->in_features);
+  if (!aligned_to(16, p->weight) || p->weight_pitch % 16 != 0 || (given && (!aligned_to(16, p->x) || p->x_pitch % 16 != 0)))
+    return fail(FDB_ERR_ALIGNMENT, "linear_int8: rows of integers must start on 16 bytes");
+  if (!aligned_to(4, p->x_scale, p->weight_scale, p->status) || !aligned_to(type_bytes(p->out_dtype), p->out) ||
+      (p->bias != nullptr && !aligned_to(type_bytes(p->bias_dtype), p->bias)) || (!given && !aligned_to(type_bytes(p->x_dtype), p->x)))
+    return fail(FDB_ERR_ALIGNMENT, "linear_int8: tensors must be aligned to their elements");
+  if (p->rows == 0) return FDB_OK;
+  const void* x = p->x;
+  const float* x_scale = p->x_scale;
+  int64_t pitch = p->x_pitch;
+  if (!given) {
+    const uint64_t need = rows_bytes(*p) + uint64_t(p->rows) * sizeof(float);
+    if (p->workspace == nullptr || p->workspace_bytes < need || !aligned_to(256, p->workspace))
+      return fail(FDB_ERR_WORKSPACE, "linear_int8: workspace of %llu bytes needed (256-byte aligned), %llu given", (unsigned long long)need,
+                  (unsigned long long)p->workspace_bytes);
+    float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + rows_bytes(*p));
+    pitch = pitch_of(*p);
+    if ((rc = launch_quantize_int8(p->x, p->x_dtype, p->rows, p->in_features, p->workspace, pitch, scale, stream)) != FDB_OK) return rc;
+    x = p->workspace;
+    x_scale = scale;
+  }
+  const int sms = sm_count();
+  if (sms <= 0) return fail(FDB_ERR_CUDA, "linear_int8 set-up: no device");
+  const Config* best = nullptr;
+  int64_t best_cost = 0, best_tiles = 0;
+  for (const Config& f : kConfigs) {
+    const int64_t tiles = (p->rows + kBM * f.cg - 1) / (kBM * f.cg) * ((p->out_features + f.bn - 1) / f.bn);
+    const int64_t units = sms / f.cg, waves = (tiles + units - 1) / units;
+    const int64_t cost = waves * ((int64_t)((p->in_features + kBK - 1) / kBK) * f.clocks) + f.extra;
+    if (best == nullptr || cost < best_cost) { best = &f; best_cost = cost; best_tiles = tiles; }
+  }
+  if (best_tiles * 2 > 2147483647LL) return fail(FDB_ERR_LIMIT, "linear_int8: %lld rows x %d features", (long long)p->rows, p->out_features);
+  Int8Args a;
+  rc = make_map_bytes(&a.tm_x, x, p->rows, p->in_features, pitch, kBM, "x");
+  if (rc == FDB_OK) rc = make_map_bytes(&a.tm_w, p->weight, p->out_features, p->in_features, p->weight_pitch, best->bn / best->cg, "weight");
+  if (rc != FDB_OK) return rc;
+  a.x_scale = x_scale; a.w_scale = p->weight_scale; a.bias = p->bias; a.out = p->out; a.status = p->status;
+  a.rows = p->rows; a.k = p->in_features; a.n = p->out_features;
+  a.tiles_n = (p->out_features + best->bn - 1) / best->bn;
+  a.bias_fp32 = p->bias_dtype == FDB_FP32;
+  a.wide = p->out_features % 8 == 0 && aligned_to(16, p->out, p->weight_scale, p->bias);
+  const int units = sms / best->cg;
+  const int grid = (int)(best_tiles < units ? best_tiles : units) * best->cg;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool gelu = p->gelu != 0, chained = !given;
+  if (best->cg == 2)
+    return best->bn == 256 ? launch_type<2, 256>(a, grid, p->out_dtype, gelu, chained, s) : launch_type<2, 128>(a, grid, p->out_dtype, gelu, chained, s);
+  return best->bn == 128 ? launch_type<1, 128>(a, grid, p->out_dtype, gelu, chained, s) : launch_type<1, 64>(a, grid, p->out_dtype, gelu, chained, s);
+}

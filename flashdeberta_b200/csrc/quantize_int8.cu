@@ -1,0 +1,121 @@
+// Rows as 8-bit integers with a scale each (fdb_quantize_int8): scale = amax / 127, y = rint(x * (127 / amax)).
+//
+// A team of warps per row (row_team.cuh); a row of up to 8192 elements is read once and stays in registers, a longer one is read a
+// second time (it comes from L2 then).  HBM-bound: x read, one byte per element written.  The magnitudes are compared as the bits of
+// their absolute values: a NaN is larger than everything there, so it reaches the scale.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "internal.h"
+#include "launch.h"
+#include "row_team.cuh"
+
+namespace fdb {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct QuantArgs {
+  const void* x;
+  uint8_t* y;
+  float* scale;
+  int64_t rows, pitch;
+  int cols, team_threads, teams;
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(1024) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
+  __shared__ uint32_t s_top[kThreads / 32][2][32];
+  const int team = threadIdx.x / a.team_threads, t = threadIdx.x - team * a.team_threads;
+  const int warps = a.team_threads / 32, span = a.team_threads * kRowElems;
+  ptx::grid_launch();
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * a.teams + team; row < a.rows; row += (int64_t)gridDim.x * a.teams) {
+    const T* x = static_cast<const T*>(a.x) + row * a.cols;
+    uint32_t top = 0;
+    RowWords<T> first;
+    float v[kRowElems];
+    for (int at = 0; at < a.cols; at += span) {
+      const RowColumns<WIDE> cols{t, a.team_threads, a.cols - at};
+      RowWords<T> r;
+      cols.load(x + at, r);
+      unpack(r, v);
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      if (at == 0) first = r;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (warps > 1) {
+      uint32_t* s = s_top[team][turn];
+      turn ^= 1;
+      if ((threadIdx.x & 31) == 0) s[t >> 5] = top;
+      ptx::bar_sync((uint32_t)team + 1, (uint32_t)a.team_threads);
+      for (int w = 0; w < warps; ++w) top = max(top, s[w]);
+    }
+    const float amax = __uint_as_float(top);
+    const bool zero = amax < 7.888609052e-31f;                       // 2^-100: the reciprocal would leave fp32's range
+    const float inv = zero || top >= 0x7f800000u ? 0.f : 127.f / amax;
+    if (t == 0) a.scale[row] = zero ? 0.f : amax / 127.f;
+    for (int at = 0; at < a.cols; at += span) {
+      const RowColumns<WIDE> cols{t, a.team_threads, a.cols - at};
+      RowWords<T> r = first;
+      if (at != 0) cols.load(x + at, r);
+      unpack(r, v);
+      int q[kRowElems];
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) q[j] = inv == 0.f ? 0 : __float2int_rn(v[j] * inv);
+      uint8_t* y = a.y + row * a.pitch + at;
+      if constexpr (WIDE) {
+        uint2 o;
+        o.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
+        o.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
+        if (cols.live(0)) *reinterpret_cast<uint2*>(y + t * kRowElems) = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kRowElems; ++j)
+          if (cols.live(j)) y[cols.col(j)] = (uint8_t)q[j];
+      }
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch(const QuantArgs& a, bool wide, cudaStream_t s) {
+  const int threads = a.teams * a.team_threads;
+  const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (2048 / threads);
+  const unsigned grid = (unsigned)std::min(want, most);
+  if (wide) quantize_int8_kernel<T, true><<<grid, threads, 0, s>>>(a);
+  else quantize_int8_kernel<T, false><<<grid, threads, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int launch_quantize_int8(const void* x, int dtype, int64_t rows, int cols, void* y, int64_t pitch, float* scale, void* stream) {
+  QuantArgs a = {x, static_cast<uint8_t*>(y), scale, rows, pitch, cols, 0, 0};
+  a.team_threads = row_team_threads(std::min(cols, kRowHiddenMax));
+  a.teams = std::max(1, kThreads / a.team_threads);
+  const bool wide = cols % kRowElems == 0 && aligned_to(16, x) && aligned_to(8, y) && pitch % 8 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == FDB_BF16 ? launch<__nv_bfloat16>(a, wide, s) : (dtype == FDB_FP16 ? launch<__half>(a, wide, s) : launch<float>(a, wide, s));
+  if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "quantize_int8 launch: %s", cudaGetErrorString(e));
+  return FDB_OK;
+}
+
+}  // namespace fdb
+
+using namespace fdb;
+
+extern "C" FDB_API int fdb_quantize_int8(const void* x, int32_t dtype, int64_t rows, int32_t cols, void* y, int64_t pitch, float* scale,
+                                         void* stream) {
+  clear_error();
+  if (dtype != FDB_BF16 && dtype != FDB_FP16 && dtype != FDB_FP32) return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: dtype %d", dtype);
+  if (rows < 0 || cols <= 0 || pitch < cols)
+    return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: rows %lld, cols %d, pitch %lld", (long long)rows, cols, (long long)pitch);
+  if (rows == 0) return FDB_OK;
+  if (x == nullptr || y == nullptr || scale == nullptr) return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: x, y and scale must not be NULL");
+  if (!aligned_to(dtype == FDB_FP32 ? 4 : 2, x) || !aligned_to(4, scale))
+    return fail(FDB_ERR_ALIGNMENT, "quantize_int8: x and scale must be aligned to their elements");
+  return launch_quantize_int8(x, dtype, rows, cols, y, pitch, scale, stream);
+}

@@ -1,0 +1,271 @@
+// The row kernel of residual_norm's backward (the mathematics is at the head of residual_norm.cu), for one type of rows per
+// translation unit.
+#pragma once
+
+#include <atomic>
+
+#include "internal.h"
+#include "launch.h"
+#include "residual_norm.h"
+#include "row_team.cuh"
+
+namespace fdb {
+
+constexpr int kNormBwdTeams = kNormBwdThreads / 32;
+constexpr size_t kNormBwdPlainSmem = 40 * 1024;  // with the 8 KB of the teams' sums, what a launch may take without being asked
+
+// Shared memory of a CTA: the teams' sums, one vector of sums per thread for adding teams up and, where the gate has groups, what
+// C = sum gate A and D = sum gate B have come to (touched only when a group ends).
+inline size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode) {
+  const size_t vector = size_t(threads) * kRowElems * sizeof(float);
+  return (teams > 1 ? vector : 0) + (post && mode == kGateGroups ? 2 * vector : 0);
+}
+
+template <typename T, bool RMS, bool POST, int GATE, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormBwdArgs b) {
+  extern __shared__ __align__(16) float s_vectors[];
+  __shared__ float s_sums[kNormBwdTeams][2 * 32 * 2];
+  const ResidualNormArgs& f = b.f;
+  const int team = threadIdx.x / f.team_threads, t = threadIdx.x - team * f.team_threads;
+  const RowColumns<WIDE> cols{t, f.team_threads, f.hidden};
+  TeamSum<2> team_sum{s_sums[team], f.team_threads / 32, t >> 5, team + 1, 0};
+  const float inv_hidden = 1.f / (float)f.hidden;
+  const int64_t worker = (int64_t)blockIdx.x * f.teams + team;
+  const bool has_rows = worker < b.workers;
+  const int64_t first = has_rows ? f.rows * worker / b.workers : 0, end = has_rows ? f.rows * (worker + 1) / b.workers : 0;
+  constexpr int kNorms = RMS ? 1 : 2;  // vectors of sums per norm: weight, bias
+
+  float sum_w[kRowElems], sum_b[kRowElems], sum_A[kRowElems], sum_B[kRowElems];
+#pragma unroll
+  for (int j = 0; j < kRowElems; ++j) sum_w[j] = sum_b[j] = sum_A[j] = sum_B[j] = 0.f;
+  float* s_team = s_vectors;
+  float* s_C = s_vectors + (f.teams > 1 ? blockDim.x * kRowElems : 0) + threadIdx.x * kRowElems;
+  float* s_D = s_C + blockDim.x * kRowElems;
+  if constexpr (GATE == kGateGroups && POST) {
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) s_C[j] = s_D[j] = 0.f;
+  }
+  ptx::grid_launch();
+
+  struct Row { RowWords<T> x, residual, dnormed, dstream, gate; float4 stats; };
+  const bool element_gate = GATE == kGateElement && f.gate != nullptr && !f.gate_fp32;
+  auto fetch = [&](int64_t row, Row& r) {
+    const int64_t at = row * f.hidden;
+    cols.load(static_cast<const T*>(f.x) + at, r.x);
+    if (f.residual != nullptr) cols.load(static_cast<const T*>(f.residual) + at, r.residual);
+    if (b.dnormed != nullptr) cols.load(static_cast<const T*>(b.dnormed) + at, r.dnormed);
+    if (b.dstream != nullptr) cols.load(static_cast<const T*>(b.dstream) + at, r.dstream);
+    if (element_gate) cols.load(static_cast<const T*>(f.gate) + at, r.gate);
+    r.stats = __ldg(f.stats + row);
+  };
+  // A and B of a group leave the registers
+  auto leave_group = [&](int64_t group, const float (&gate)[kRowElems]) {
+    float* slot = b.slots + (worker + group) * 2 * f.hidden;
+    cols.store(slot, sum_A);
+    if constexpr (!RMS) cols.store(slot + f.hidden, sum_B);
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) {
+      if constexpr (POST) {
+        s_C[j] = fmaf(gate[j], sum_A[j], s_C[j]);
+        if constexpr (!RMS) s_D[j] = fmaf(gate[j], sum_B[j], s_D[j]);
+      }
+      sum_A[j] = sum_B[j] = 0.f;
+    }
+  };
+
+  Row now, next;
+  if (first < end) fetch(first, now);
+  int64_t group = -1;
+  float g[kRowElems];
+#pragma unroll
+  for (int j = 0; j < kRowElems; ++j) g[j] = 1.f;
+  for (int64_t row = first; row < end; ++row) {
+    if (row + 1 < end) fetch(row + 1, next);
+    const int64_t at = row * f.hidden;
+    if constexpr (GATE == kGateGroups) {
+      const int64_t mine = (uint32_t)row / f.gate_rows;
+      if (mine != group) {
+        if (group >= 0) leave_group(group, g);
+        group = mine;
+        cols.template load_param<T>(f.gate, f.gate_fp32, group * f.hidden, g);
+      }
+    } else if constexpr (GATE == kGateElement) {
+      if (element_gate) unpack(now.gate, g);
+      else if (f.gate != nullptr) cols.load(static_cast<const float*>(f.gate) + at, g);
+    } else if (f.gate != nullptr) {
+      cols.template load_param<T>(f.gate, f.gate_fp32, 0, g);
+    }
+
+    // the stream again; hat: x normalised (x itself without the norm), z: the stream normalised
+    float hat[kRowElems], u[kRowElems], z[kRowElems], d[kRowElems], p[kRowElems];
+    unpack(now.x, hat);
+    if constexpr (POST) {
+      cols.template load_param<T>(f.post_weight, f.param_fp32, 0, p);
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) {
+        hat[j] = (RMS ? hat[j] : hat[j] - now.stats.x) * now.stats.y;
+        u[j] = hat[j] * p[j];
+      }
+      if (f.post_bias != nullptr) {
+        cols.template load_param<T>(f.post_bias, f.param_fp32, 0, p);
+#pragma unroll
+        for (int j = 0; j < kRowElems; ++j) u[j] += p[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) u[j] = hat[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) z[j] = g[j] * u[j];
+    if (f.residual != nullptr) {
+      unpack(now.residual, p);
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) z[j] = fmaf(f.residual_scale, p[j], z[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) z[j] = (RMS ? z[j] : z[j] - now.stats.z) * now.stats.w;
+
+    // dz, the gradient of the stream in all
+    float sums[2] = {0.f, 0.f};
+    if (b.dnormed != nullptr) {
+      unpack(now.dnormed, d);
+      cols.template load_param<T>(f.weight, f.param_fp32, 0, p);
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) {
+        sum_w[j] = fmaf(d[j], z[j], sum_w[j]);
+        if constexpr (!RMS) sum_b[j] += d[j];
+        d[j] *= p[j];
+        sums[0] = fmaf(d[j], z[j], sums[0]);
+        if constexpr (!RMS) sums[1] += d[j];
+      }
+      team_sum(sums);
+      sums[0] *= inv_hidden;
+      sums[1] *= inv_hidden;
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.w * (d[j] - fmaf(z[j], sums[0], RMS ? 0.f : sums[1]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) d[j] = 0.f;
+    }
+    if (b.dstream != nullptr) {
+      unpack(now.dstream, p);
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) d[j] += p[j];
+    }
+    if (b.dresidual != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) p[j] = f.residual_scale * d[j];
+      cols.store(static_cast<T*>(b.dresidual) + at, p);
+    }
+    if constexpr (GATE == kGateElement) {
+      if (b.dgate != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kRowElems; ++j) p[j] = d[j] * u[j];
+        if (f.gate_fp32) cols.store(static_cast<float*>(b.dgate) + at, p);
+        else cols.store(static_cast<T*>(b.dgate) + at, p);
+      }
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) d[j] *= g[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) {
+      sum_A[j] = fmaf(d[j], hat[j], sum_A[j]);
+      if constexpr (!RMS) sum_B[j] += d[j];
+    }
+    if constexpr (GATE != kGateElement) {
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) d[j] *= g[j];
+    }
+    if constexpr (POST) {
+      cols.template load_param<T>(f.post_weight, f.param_fp32, 0, p);
+      sums[0] = sums[1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) {
+        d[j] *= p[j];
+        sums[0] = fmaf(d[j], hat[j], sums[0]);
+        if constexpr (!RMS) sums[1] += d[j];
+      }
+      team_sum(sums);
+      sums[0] *= inv_hidden;
+      sums[1] *= inv_hidden;
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.y * (d[j] - fmaf(hat[j], sums[0], RMS ? 0.f : sums[1]));
+    }
+    cols.store(static_cast<T*>(b.dx) + at, d);
+    now = next;
+  }
+  if constexpr (GATE == kGateGroups) {
+    if (group >= 0) leave_group(group, g);
+    if constexpr (POST) {
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) {
+        sum_A[j] = s_C[j];
+        sum_B[j] = s_D[j];
+      }
+    }
+  }
+
+  // the CTA's sums
+  float* part = b.parts + (int64_t)blockIdx.x * b.vectors * f.hidden;
+  auto write = [&](float (&v)[kRowElems], int vector) {
+    if (f.teams == 1) {
+      cols.store(part + (int64_t)vector * f.hidden, v);
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) s_team[threadIdx.x * kRowElems + j] = v[j];
+    __syncthreads();
+    const int all = f.team_threads * kRowElems;
+    for (int i = threadIdx.x; i < all; i += blockDim.x) {
+      const int c = WIDE ? i : (i % kRowElems) * f.team_threads + i / kRowElems;
+      float sum = 0.f;
+      for (int k = 0; k < f.teams; ++k) sum += s_team[k * all + i];
+      if (c < f.hidden) part[(int64_t)vector * f.hidden + c] = sum;
+    }
+  };
+  write(sum_w, 0);
+  if constexpr (!RMS) write(sum_b, 1);
+  write(sum_A, kNorms);
+  if constexpr (!RMS) write(sum_B, kNorms + 1);
+}
+
+// WIDE stores of fp32 sums need rows of them to start on 16 bytes: they do, hidden being a multiple of 8 there.
+template <typename T, typename F>
+auto with_norm_bwd_kernel(bool rms, bool post, int mode, bool wide, int threads, F&& use) {
+#define FDB_BWD4(R, P, G, W) (threads <= kNormBwdThreads ? use(residual_norm_bwd_kernel<T, R, P, G, W, kNormBwdThreads>) : use(residual_norm_bwd_kernel<T, R, P, G, W, 1024>))
+#define FDB_BWD3(R, P, G) (wide ? FDB_BWD4(R, P, G, true) : FDB_BWD4(R, P, G, false))
+#define FDB_BWD2(R, P) (mode == kGateChannel ? FDB_BWD3(R, P, kGateChannel) : (mode == kGateGroups ? FDB_BWD3(R, P, kGateGroups) : FDB_BWD3(R, P, kGateElement)))
+  if (rms) return post ? FDB_BWD2(true, true) : FDB_BWD2(true, false);
+  return post ? FDB_BWD2(false, true) : FDB_BWD2(false, false);
+#undef FDB_BWD4
+#undef FDB_BWD3
+#undef FDB_BWD2
+}
+
+template <typename T> int norm_bwd_resident(bool rms, bool post, int mode, bool wide, int threads, int teams) {
+  return with_norm_bwd_kernel<T>(rms, post, mode, wide, threads, [&](auto kernel) {
+    int n = 0;
+    const size_t smem = residual_norm_bwd_smem(threads, teams, post, mode);
+    if (smem > kNormBwdPlainSmem) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) {
+      cudaGetLastError();
+      n = 1;
+    }
+    return n;
+  });
+}
+
+template <typename T> int norm_bwd_launch(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s) {
+  const int threads = b.f.teams * b.f.team_threads;
+  const bool post = b.f.post_weight != nullptr;
+  return with_norm_bwd_kernel<T>(b.f.rms, post, b.mode, wide, threads, [&](auto kernel) {
+    const size_t smem = residual_norm_bwd_smem(threads, b.f.teams, post, b.mode);
+    cudaError_t e = smem > kNormBwdPlainSmem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    if (e == cudaSuccess) e = launch_kernel<ResidualNormBwdArgs>(kernel, b, dim3((unsigned)b.ctas), threads, smem, false, s);
+    if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm backward launch: %s", cudaGetErrorString(e));
+    return (int)FDB_OK;
+  });
+}
+
+}  // namespace fdb

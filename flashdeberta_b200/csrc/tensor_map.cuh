@@ -62,4 +62,19 @@ inline int make_map_table(CUtensorMap* m, const void* base, int xrows, int heads
   return FDB_OK;
 }
 
+// (rows, cols) bytes, rows `pitch` apart -> 2-D map (col, row), box 128 x box_rows, 128-byte swizzle; zeros behind the ends
+inline int make_map_bytes(CUtensorMap* m, const void* base, int64_t rows, int cols, int64_t pitch, int box_rows, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(FDB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FDB_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, (int)r);
+  return FDB_OK;
+}
+
 }  // namespace fdb

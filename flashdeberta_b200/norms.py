@@ -1,0 +1,219 @@
+"""Residual norms: what lies between two blocks of a layer, in one pass, with its backward.
+
+``ops.residual_norm`` covers the tails of transformers' DebertaV2SelfOutput / DebertaV2Output, which the reference's layer classes
+keep (src/flashdeberta/model.py:259-272), and the other residual streams that encoders are built with: a norm after the block as
+well, a gate per channel, per sequence or per element, a weighted residual, LayerNorm or RMSNorm.  Unlike ``ops.add_layernorm`` it
+trains, takes every width up to 8192 and bf16, fp16 and fp32 rows.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib, ops
+
+TYPES = {torch.bfloat16: _lib.FDB_BF16, torch.float16: _lib.FDB_FP16, torch.float32: _lib.FDB_FP32}
+MAX_HIDDEN = 8192
+
+
+def _gate_rows(gate: torch.Tensor, shape) -> Optional[int]:
+    """Rows of ``shape`` that share a row of the gate, or None where the gate's rows do not each cover one run of rows."""
+    given = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
+    if given[-1] != shape[-1]:
+        return None
+    lead, own = tuple(shape[:-1]), given[:-1]
+    i = 0
+    while i < len(lead) and own[i] == lead[i]:
+        i += 1
+    if any(n != 1 for n in own[i:]):
+        return None
+    rows = 1
+    for n in lead[i:]:
+        rows *= n
+    return rows
+
+
+def _checked(x, residual, weight, bias, post_weight, post_bias, gate, rms):
+    """Raises on what the operator does not take; returns the gate as it is passed on (broadcast where it has to be)."""
+    if not x.is_cuda:
+        raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
+    if x.dtype not in TYPES:
+        raise TypeError(f"residual_norm takes bfloat16, float16 or float32 rows, not {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_HIDDEN:
+        raise ValueError(f"residual_norm takes rows of 1 to {MAX_HIDDEN} elements")
+    hidden = x.shape[-1]
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must match x in shape and dtype")
+    if rms and (bias is not None or post_bias is not None):
+        raise ValueError("the RMS norm takes no bias")
+    if post_bias is not None and post_weight is None:
+        raise ValueError("post_bias needs post_weight")
+    for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
+        if t is None:
+            continue
+        if t.shape != (hidden,):
+            raise ValueError(f"{name} must have shape ({hidden},), got {tuple(t.shape)}")
+        if t.dtype != weight.dtype or t.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{name} must be {x.dtype} or float32, the norms' parameters all alike; got {t.dtype}")
+    for name, t in (("residual", residual), ("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias),
+                    ("gate", gate)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    if gate is None:
+        return None
+    if gate.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"gate must be {x.dtype} or float32, got {gate.dtype}")
+    if gate.dim() > x.dim():
+        raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
+    if _gate_rows(gate, x.shape) is None:  # shared in some other way: one per element then
+        try:
+            return gate.expand(x.shape)
+        except RuntimeError:
+            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}") from None
+    return gate
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale):
+    """The C call's parameters over contiguous tensors."""
+    rows = x.numel() // x.shape[-1]
+    return _lib.ResidualNormParams(
+        C.sizeof(_lib.ResidualNormParams), TYPES[x.dtype], x.data_ptr(), _address(residual), weight.data_ptr(), _address(bias),
+        _address(post_weight), _address(post_bias), _address(gate), normed.data_ptr(), _address(stream), _address(stats), rows,
+        0 if gate is None else _gate_rows(gate, x.shape), x.shape[-1], TYPES[weight.dtype], 0 if gate is None else TYPES[gate.dtype],
+        int(rms), residual_scale, eps)
+
+
+def _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, keep):
+    """(normed, stream, stats); the statistics where a backward will want them (``keep``), else None."""
+    x, residual, weight, bias, post_weight, post_bias, gate = map(_dense, (x, residual, weight, bias, post_weight, post_bias, gate))
+    normed, stream = torch.empty_like(x), torch.empty_like(x)
+    stats = torch.empty(x.numel() // x.shape[-1], 4, dtype=torch.float32, device=x.device) if keep else None
+    if x.numel() == 0:
+        return normed, stream, stats
+    p = _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale)
+    with ops.on_device(x.device):
+        _lib.check(_lib.load().fdb_residual_norm(C.byref(p), ops.raw_stream(x.device)))
+    ops._launches += 1
+    return normed, stream, stats
+
+
+def _backward(dnormed, dstream, x, residual, weight, bias, post_weight, post_bias, gate, stats, eps, rms, residual_scale, wanted):
+    """Gradients of x, residual, weight, bias, post_weight, post_bias and gate; None where ``wanted`` is false."""
+    tensors = [_dense(t) for t in (x, residual, weight, bias, post_weight, post_bias, gate)]
+    x = tensors[0]
+    grads = [torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and w else None for t, w in zip(tensors, wanted)]
+    if x.numel() == 0 or (dnormed is None and dstream is None):
+        return [None if g is None else g.zero_() for g in grads]
+    dnormed, dstream = _dense(dnormed), _dense(dstream)
+    dx = grads[0] if grads[0] is not None else torch.empty_like(x)
+    lib = _lib.load()
+    p = _params(*tensors, x, None, stats, eps, rms, residual_scale)
+    b = _lib.ResidualNormBwdParams(C.sizeof(_lib.ResidualNormBwdParams), 0, C.pointer(p), _address(dnormed), _address(dstream), dx.data_ptr(),
+                                   *(_address(g) for g in grads[1:]))
+    with ops.on_device(x.device):
+        need = lib.fdb_residual_norm_bwd_workspace_bytes(C.byref(b))
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        b.workspace, b.workspace_bytes = ws.data_ptr(), need
+        _lib.check(lib.fdb_residual_norm_bwd(C.byref(b), ops.raw_stream(x.device)))
+    ops._launches += 1 + int(any(g is not None for g in grads[2:]))
+    return grads
+
+
+@torch.library.custom_op("flashdeberta_b200::residual_norm", mutates_args=())
+def residual_norm_op(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, bias: Optional[torch.Tensor],
+                     post_weight: Optional[torch.Tensor], post_bias: Optional[torch.Tensor], gate: Optional[torch.Tensor], eps: float,
+                     rms: bool, residual_scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(normed, stream, statistics) as one node for tracing; the statistics carry no gradient."""
+    return _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, True)
+
+
+@residual_norm_op.register_fake
+def _(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale):
+    rows = x.numel() // x.shape[-1]
+    return x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty((rows, 4), dtype=torch.float32)
+
+
+@torch.library.custom_op("flashdeberta_b200::residual_norm_bwd", mutates_args=())
+def residual_norm_bwd_op(dnormed: torch.Tensor, dstream: torch.Tensor, x: torch.Tensor, residual: Optional[torch.Tensor],
+                         weight: torch.Tensor, bias: Optional[torch.Tensor], post_weight: Optional[torch.Tensor],
+                         post_bias: Optional[torch.Tensor], gate: Optional[torch.Tensor], stats: torch.Tensor, eps: float, rms: bool,
+                         residual_scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Every gradient of ``residual_norm_op``; an absent tensor gives an empty one."""
+    grads = _backward(dnormed, dstream, x, residual, weight, bias, post_weight, post_bias, gate, stats, eps, rms, residual_scale, (True,) * 7)
+    return tuple(x.new_empty(0) if g is None else g for g in grads)
+
+
+@residual_norm_bwd_op.register_fake
+def _(dnormed, dstream, x, residual, weight, bias, post_weight, post_bias, gate, stats, eps, rms, residual_scale):
+    return tuple(x.new_empty(0) if t is None else t.new_empty(t.shape) for t in (x, residual, weight, bias, post_weight, post_bias, gate))
+
+
+def _setup(ctx, inputs, output):
+    *tensors, eps, rms, residual_scale = inputs
+    ctx.save_for_backward(*tensors, output[2])
+    ctx.norm_args = (eps, rms, residual_scale)
+
+
+def _op_backward(ctx, dnormed, dstream, _):
+    *tensors, stats = ctx.saved_tensors
+    x = tensors[0]
+    dnormed, dstream = (torch.zeros_like(x) if g is None else g for g in (dnormed, dstream))
+    grads = residual_norm_bwd_op(dnormed, dstream, *tensors, stats, *ctx.norm_args)
+    return (*(None if t is None else g for t, g in zip(tensors, grads)), None, None, None)
+
+
+residual_norm_op.register_autograd(_op_backward, setup_context=_setup)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """The training call outside tracing."""
+
+    @staticmethod
+    def forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale):
+        return _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, True)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _setup(ctx, inputs, output)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(output[2])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dnormed, dstream, _):
+        if any(ops.intercepted(g) or (g is not None and ops.batched(g)) for g in (dnormed, dstream)):
+            return _op_backward(ctx, dnormed, dstream, _)
+        *tensors, stats = ctx.saved_tensors
+        grads = _backward(dnormed, dstream, *tensors, stats, *ctx.norm_args, ctx.needs_input_grad[:7])
+        return (*grads, None, None, None)
+
+
+def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  eps: float = 1e-7, *, rms: bool = False, post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  residual_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``stream = residual_scale * residual + gate * norm(x; post_weight, post_bias)`` and ``normed = norm(stream; weight, bias)``
+    over the last dimension, one kernel forward and two backward.  Returns ``(normed, stream)``, both of x's shape and type.
+
+    The norm is LayerNorm, or RMSNorm (no bias) with ``rms``; without ``post_weight`` the block's output x goes into the stream as it
+    is.  ``gate`` broadcasts to x: (hidden,) a gate per channel, (batch, 1, hidden) one per sequence, x's shape one per element; None is
+    a gate of one.  ``residual`` may be None.  Rows are bfloat16, float16 or float32; the norms' parameters are of that type or all
+    float32, the gate of either.  Statistics and sums are float32, every result is rounded once (``normed`` is made of the stream
+    before it is rounded).  Gradients of every input, in the inputs' types; no second derivative."""
+    gate = _checked(x, residual, weight, bias, post_weight, post_bias, gate, rms)
+    call = (x, residual, weight, bias, post_weight, post_bias, gate, float(eps), bool(rms), float(residual_scale))
+    if ops.intercepted(*call[:7]):
+        return residual_norm_op(*call)[:2]
+    if ops.wants_grad(*call[:7]):
+        return _ResidualNorm.apply(*call)[:2]
+    return _forward(*call, False)[:2]

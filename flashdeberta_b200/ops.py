@@ -22,6 +22,7 @@ from . import _lib, bucket
 
 __all__ = [
     "disentangled_attention", "disentangled_attention_fp8", "disentangled_attention_static", "disentangled_attention_check", "relative_index_matrix", "quantize_e4m3", "add_layernorm", "can_fuse_add_layernorm", "linear_gelu", "can_fuse_linear_gelu", "embed_layernorm",
+    "residual_norm", "quantize_int8", "int8_rows", "linear_int8", "grad_norm", "clip_grads_", "clip_grad_norm_",
     "check_status", "launch_count", "PreparedWorkspace",
 ]
 
@@ -749,3 +750,9 @@ def attn_train(q, k, v, pos_key, pos_query, cu_seqlens, seq_lens, max_seqlen, sm
 def wants_grad(*tensors) -> bool:
     """True when autograd is recording and one of the tensors takes part in it."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# The operators of the layers around the attention live in modules of their own, which use what is above.
+from .norms import residual_norm  # noqa: E402,F401
+from .int8 import int8_rows, linear_int8, quantize_int8  # noqa: E402,F401
+from .clip import clip_grad_norm_, clip_grads_, grad_norm  # noqa: E402,F401

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define FDB_ABI_VERSION 5
+#define FDB_ABI_VERSION 6
 
 #if defined(__GNUC__)
 #define FDB_API __attribute__((visibility("default")))
@@ -41,8 +41,10 @@ typedef enum fdb_status {
 
 typedef enum fdb_dtype {
   FDB_BF16 = 0,
-  FDB_FP32 = 1, /* check kernel only */
-  FDB_E4M3 = 2  /* fused kernel, per-head scales */
+  FDB_FP32 = 1, /* attention: check kernel only */
+  FDB_E4M3 = 2, /* fused attention kernel, per-head scales */
+  FDB_FP16 = 3, /* residual norms, 8-bit linear layer, gradients */
+  FDB_INT8 = 4  /* input of the 8-bit linear layer */
 } fdb_dtype;
 
 /* Bits of the device status word written by kernels (0 = no anomaly). */
@@ -448,6 +450,112 @@ typedef struct fdb_encoder_call {
 
 FDB_API uint64_t fdb_encoder_workspace_bytes(const fdb_encoder_call* c);
 FDB_API int fdb_encoder_forward(fdb_encoder_call* c, void* stream);
+
+/*
+ * What lies between two blocks of a layer, in one pass over the rows:
+ *     stream = residual_scale * residual + gate * Norm_post(x),   normed = Norm(stream)
+ * Norm is LayerNorm, or RMSNorm with `rms`, eps inside the square root, over the last dimension.  post_weight NULL: no norm after the
+ * block; gate NULL: a gate of one; residual NULL: none is added.  DebertaV2SelfOutput / DebertaV2Output behind the reference's layer
+ * classes (src/flashdeberta/model.py:259-272) are the case without post norm and gate and with a residual_scale of one; unlike
+ * fdb_add_layernorm this takes every type and width, keeps what a backward needs and does not round the sum before the norm.
+ * x, residual, normed, stream: (rows, hidden) contiguous, all of `dtype` (bf16, fp16 or fp32), hidden at most 8192; weights and
+ * biases (hidden) of that type or fp32 (`param_dtype`).  Row r takes row r / gate_rows of the gate, (rows / gate_rows, hidden) of
+ * `gate_dtype`: gate_rows = rows is a gate per channel, 1 one per element.  Pointers are aligned to their elements; 16-byte pieces are
+ * used where hidden and every pointer allow it.  Statistics and sums are fp32; each result is rounded once.
+ */
+typedef struct fdb_residual_norm_params {
+  uint32_t struct_bytes;   /* sizeof(fdb_residual_norm_params), checked */
+  int32_t dtype;           /* FDB_BF16, FDB_FP16 or FDB_FP32 */
+  const void *x, *residual;
+  const void *weight, *bias, *post_weight, *post_bias, *gate;
+  void *normed, *stream;   /* out; stream may be NULL */
+  float* stats;            /* out, (rows, 4), 16-byte aligned: what fdb_residual_norm_bwd reads; or NULL */
+  int64_t rows, gate_rows; /* gate_rows divides rows */
+  int32_t hidden, param_dtype, gate_dtype, rms;
+  float residual_scale, eps;
+} fdb_residual_norm_params;
+FDB_API int fdb_residual_norm(const fdb_residual_norm_params* p, void* stream);
+
+/*
+ * Its backward.  `fwd` is the forward call (inputs, stats; normed must not be NULL, it and stream are not looked at).  dnormed and
+ * dstream: gradients of the results, either may be NULL (zero).  Every gradient but dx may be NULL (not wanted); each has the type
+ * and shape of its tensor.  No atomics: the same bits every time.
+ */
+typedef struct fdb_residual_norm_bwd_params {
+  uint32_t struct_bytes;   /* sizeof(fdb_residual_norm_bwd_params), checked */
+  int32_t reserved;
+  const fdb_residual_norm_params* fwd;
+  const void *dnormed, *dstream;
+  void *dx, *dresidual, *dweight, *dbias, *dpost_weight, *dpost_bias, *dgate;
+  void* workspace;         /* device, >= fdb_residual_norm_bwd_workspace_bytes(), 16-byte aligned */
+  uint64_t workspace_bytes;
+} fdb_residual_norm_bwd_params;
+FDB_API uint64_t fdb_residual_norm_bwd_workspace_bytes(const fdb_residual_norm_bwd_params* p);
+FDB_API int fdb_residual_norm_bwd(const fdb_residual_norm_bwd_params* p, void* stream);
+
+/*
+ * Rows as 8-bit integers with a scale each: scale = amax / 127, y = x * (127 / amax) rounded to the nearest whole number, ties to even
+ * (both quotients and the product in fp32).  A row of zeros, or one whose largest magnitude is below 2^-100, has scale and integers
+ * zero; a row with an infinity or a NaN has integers zero and a scale that is infinite or NaN, so whatever is made of it is NaN.
+ * x: (rows, cols) of FDB_BF16, FDB_FP16 or FDB_FP32, contiguous; y: rows of `pitch` bytes, cols written, pitch >= cols; scale: (rows).
+ * The same kernel scales tokens and the output channels of a weight.
+ */
+FDB_API int fdb_quantize_int8(const void* x, int32_t dtype, int64_t rows, int32_t cols, void* y, int64_t pitch, float* scale, void* stream);
+
+/*
+ * out = act(x_scale[m] * weight_scale[n] * sum_k x[m][k] weight[n][k] + bias[n]): a linear layer in 8-bit integers, the sum exact in
+ * 32-bit integers (in_features at most 131071), act = identity or erf GELU, one rounding to out_dtype.  x is FDB_INT8 with its scales,
+ * or FDB_BF16, FDB_FP16 or FDB_FP32, contiguous, and is scaled and rounded as fdb_quantize_int8 does, into the workspace.
+ */
+typedef struct fdb_linear_int8_params {
+  uint32_t struct_bytes;      /* sizeof(fdb_linear_int8_params), checked */
+  int32_t x_dtype;            /* FDB_INT8 or a type that fdb_quantize_int8 takes */
+  const void* x;              /* (rows, in_features); FDB_INT8: rows of x_pitch bytes */
+  int64_t x_pitch;            /* FDB_INT8: a multiple of 16, x 16-byte aligned; else not looked at (contiguous) */
+  const float* x_scale;       /* FDB_INT8: (rows) */
+  const void* weight;         /* int8 (out_features, in_features), rows of weight_pitch bytes: both multiples of 16 */
+  int64_t weight_pitch;
+  const float* weight_scale;  /* (out_features) */
+  const void* bias;           /* (out_features) of bias_dtype, or NULL */
+  void* out;                  /* (rows, out_features) contiguous */
+  int64_t rows;
+  int32_t in_features, out_features;
+  int32_t bias_dtype, out_dtype; /* FDB_BF16, FDB_FP16 or FDB_FP32 */
+  int32_t gelu;
+  int32_t reserved;
+  void* workspace;            /* device, >= fdb_linear_int8_workspace_bytes(), 256-byte aligned (may be NULL where that is 0) */
+  uint64_t workspace_bytes;
+  int32_t* status;            /* device word that receives FDB_DEV_TIMEOUT if a wait inside a kernel gives up (may be NULL) */
+} fdb_linear_int8_params;
+FDB_API uint64_t fdb_linear_int8_workspace_bytes(const fdb_linear_int8_params* p);
+FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* stream);
+
+/*
+ * The norm over several tensors taken as one vector, norm = (sum |g|^p)^(1/p) for p = 1, 2 or infinity, and the tensors scaled to
+ * it: out = g * min(1, max_norm / (norm + 1e-6)) (clipping by the global norm; a NaN norm makes NaN of everything).  The table is read
+ * by the call itself, on the host, and may go afterwards.  Sums are fp64 over fp32 pieces; no atomics: the same bits every time.
+ * scale = 0: the norm alone, `out` is not looked at.  An entry may be its own output (out == data, same type); entries must not
+ * overlap one another otherwise.  Where the factor is one, entries that are their own output are left as they are.
+ */
+typedef struct fdb_grad_tensor {
+  const void* data;        /* `count` elements, contiguous, aligned to their type */
+  void* out;               /* `count` elements */
+  int64_t count;
+  int32_t dtype, out_dtype; /* FDB_BF16, FDB_FP16 or FDB_FP32 */
+} fdb_grad_tensor;
+typedef struct fdb_clip_grads_params {
+  uint32_t struct_bytes;   /* sizeof(fdb_clip_grads_params), checked */
+  int32_t n_tensors;
+  const fdb_grad_tensor* tensors; /* host memory */
+  int32_t norm_type;       /* 1, 2, or 0 for infinity */
+  int32_t scale;           /* whether the tensors are scaled */
+  double max_norm;
+  float* norm;             /* out, device */
+  void* workspace;         /* device, >= fdb_clip_grads_workspace_bytes(), 16-byte aligned */
+  uint64_t workspace_bytes;
+} fdb_clip_grads_params;
+FDB_API uint64_t fdb_clip_grads_workspace_bytes(const fdb_clip_grads_params* p);
+FDB_API int fdb_clip_grads(const fdb_clip_grads_params* p, void* stream);
 
 #ifdef __cplusplus
 }
