@@ -65,7 +65,7 @@ class ResidualNormParams(C.Structure):
 class ResidualNormBwdParams(C.Structure):
     """Mirror of ``fdb_residual_norm_bwd_params``."""
 
-    _fields_ = [("struct_bytes", C.c_uint32), ("reserved", C.c_int32), ("fwd", C.POINTER(ResidualNormParams))] + [(n, C.c_void_p) for n in (
+    _fields_ = [("struct_bytes", C.c_uint32), ("reserved", C.c_int32), ("fwd", ResidualNormParams)] + [(n, C.c_void_p) for n in (
         "dnormed", "dstream", "dx", "dresidual", "dweight", "dbias", "dpost_weight", "dpost_bias", "dgate", "workspace")] + [
         ("workspace_bytes", C.c_uint64)]
 

@@ -32,10 +32,6 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _span(t: torch.Tensor):
-    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-
-
 def _apart(writes, reads=()) -> bool:
     """Whether runs of memory (from, to) that are written keep clear of one another and of those that are read."""
     writes = sorted(writes)
@@ -49,20 +45,35 @@ def _apart(writes, reads=()) -> bool:
     return True
 
 
-def _run(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], max_norm: float, norm_type: float, device) -> torch.Tensor:
-    """One C call: the norm, and, with ``outs``, the scaled tensors."""
-    table = array.array("q")
-    for i, g in enumerate(grads):
-        kind = TYPES[g.dtype]
-        out = g if outs is None else outs[i]
-        table.extend((g.data_ptr(), out.data_ptr(), g.numel(), kind | TYPES[out.dtype] << 32))  # fdb_grad_tensor
+_at, _count, _size, _whole, _card = (
+    torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.element_size, torch.Tensor.is_contiguous, torch.Tensor.get_device)
+
+
+def _run(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], max_norm: float, norm_type: float) -> torch.Tensor:
+    """One C call: the norm, and, with ``outs``, the scaled tensors.  All are runs of memory."""
+    table = array.array("q", bytes(32 * len(grads)))  # rows of fdb_grad_tensor: two addresses, the count, both types
+    at, count, kinds = list(map(_at, grads)), list(map(_count, grads)), [TYPES[g.dtype] for g in grads]
+    to, into = at, kinds
+    if outs is not None and outs is not grads:
+        to, into = list(map(_at, outs)), [TYPES[o.dtype] for o in outs]
+        own = [a == b for a, b in zip(at, to)]
+        if any(i and a != b for i, a, b in zip(own, kinds, into)):
+            raise ValueError("a gradient cannot be scaled in place into another type")
+    if outs is not None:
+        ends = [a + n * s for a, n, s in zip(to, count, map(_size, outs))]
+        more = [] if outs is grads else [(a, a + n * s) for a, n, s, i in zip(at, count, map(_size, grads), own) if not i]
+        # runs of memory are apart where each ends, in order, before the next begins
+        if any(a > b for a, b in zip(sorted(ends + [hi for _, hi in more]), sorted(to + [lo for lo, _ in more])[1:])) and not _apart(zip(to, ends), more):
+            raise ValueError("the tensors that are written overlap one another or a gradient that is read")
+    table[0::4], table[1::4], table[2::4] = array.array("q", at), array.array("q", to), array.array("q", count)
+    table[3::4] = array.array("q", [a | b << 32 for a, b in zip(kinds, into)])
+    device, lib = grads[0].device, _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=device)
     p = _lib.ClipGradsParams(C.sizeof(_lib.ClipGradsParams), len(grads), table.buffer_info()[0], _NORMS[norm_type], int(outs is not None),
                              max_norm, norm.data_ptr(), None, 0)
-    lib = _lib.load()
     with ops.on_device(device):
         need = lib.fdb_clip_grads_workspace_bytes(C.byref(p))
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        ws = norm.new_empty(max(need, 16), dtype=torch.uint8)
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
         _lib.check(lib.fdb_clip_grads(C.byref(p), ops.raw_stream(device)))
     ops._launches += 2
@@ -71,15 +82,16 @@ def _run(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], 
 
 def _listed(grads: Tensors, what: str) -> List[torch.Tensor]:
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    for g in grads:
-        if g.layout != torch.strided:
-            raise TypeError(f"{what} takes dense tensors, not {g.layout}")
-        if not g.is_cuda:
-            raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
-        if g.dtype not in TYPES:
-            raise TypeError(f"{what} takes bfloat16, float16 or float32 tensors, not {g.dtype}")
-        if g.device != grads[0].device:
-            raise ValueError(f"{what} takes tensors of one device, got {grads[0].device} and {g.device}")
+    if any(g.layout is not torch.strided for g in grads):
+        raise TypeError(f"{what} takes dense tensors")
+    cards = set(map(_card, grads))
+    if -1 in cards:
+        raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
+    if len(cards) > 1:
+        raise ValueError(f"{what} takes tensors of one device, got {sorted(cards)}")
+    other = {g.dtype for g in grads} - TYPES.keys()
+    if other:
+        raise TypeError(f"{what} takes bfloat16, float16 or float32 tensors, not {other.pop()}")
     return grads
 
 
@@ -97,7 +109,7 @@ def grad_norm(grads: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     norm_type, grads = _norm_type(norm_type), _listed(grads, "grad_norm")
     if not grads:
         return torch.tensor(0.0)
-    return _run([g if _dense(g) else g.contiguous() for g in grads], None, 0.0, norm_type, grads[0].device)
+    return _run([g if _dense(g) else g.contiguous() for g in grads], None, 0.0, norm_type)
 
 
 @torch.no_grad()
@@ -117,32 +129,28 @@ def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out:
         return torch.tensor(0.0)
     if outs[0].device != grads[0].device:
         raise ValueError(f"out is on {outs[0].device}, the gradients on {grads[0].device}")
+    if out is None and all(map(_whole, grads)):
+        if 0 in map(_count, grads):
+            grads = [g for g in grads if g.numel()] or grads[:1]
+        return _run(grads, grads, max_norm, norm_type)
     # the kernel goes through memory: a tensor that is no run of it, or is ordered unlike its output, is taken through a copy
-    reads, writes, back, read_only = [], [], [], []
+    reads, writes, back = [], [], []
     for g, o in zip(grads, outs):
         if g.numel() == 0:
             continue
-        if g is o or (g.data_ptr() == o.data_ptr() and g.stride() == o.stride()):
-            if g.dtype != o.dtype:
-                raise ValueError("a gradient cannot be scaled in place into another type")
-            if _dense(g):
-                reads.append(g)
-                writes.append(g)
-                continue
-        elif _dense(g) and _dense(o) and g.stride() == o.stride():
+        if (g.is_contiguous() and o.is_contiguous()) or (_dense(g) and _dense(o) and g.stride() == o.stride()):
             reads.append(g)
             writes.append(o)
-            read_only.append(g)
             continue
+        if g.data_ptr() == o.data_ptr() and g.dtype != o.dtype:
+            raise ValueError("a gradient cannot be scaled in place into another type")
         reads.append(g.contiguous())
-        if reads[-1] is g:
-            read_only.append(g)
         writes.append(o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device))
         if writes[-1] is not o:
             back.append((o, writes[-1]))
-    if not _apart(map(_span, writes), map(_span, read_only)):
-        raise ValueError("the tensors that are written overlap one another or a gradient that is read")
-    norm = _run(reads, writes, max_norm, norm_type, grads[0].device)
+    if not reads:
+        return grads[0].new_zeros((), dtype=torch.float32)
+    norm = _run(reads, writes, max_norm, norm_type)
     for o, scaled in back:
         o.copy_(scaled)
     return norm

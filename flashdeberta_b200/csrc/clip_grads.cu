@@ -34,7 +34,7 @@ struct Entry {
   void* out;
   int64_t count;
   uint32_t first_chunk;
-  uint8_t dtype, out_dtype, wide, same;  // wide: both addresses allow 16-byte pieces; same: the tensor is its own output
+  uint8_t dtype, out_dtype, wide, same;  // wide: both addresses allow pieces of eight elements; same: the tensor is its own output
 };
 template <int N> struct Table {
   double* partial;       // one value per CTA of every table
@@ -51,10 +51,11 @@ template <typename T>
 __device__ __forceinline__ void load_chunk(const T* p, int64_t left, bool wide, RowWords<T> (&r)[kVectors]) {
   if (wide && left >= kChunk) {
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-      for (int w = 0; w < int(sizeof(RowWords<T>) / 16); ++w)
-        reinterpret_cast<uint4*>(r[i].w)[w] = reinterpret_cast<const uint4*>(p + (i * kThreads + threadIdx.x) * kRowElems)[w];
+    for (int i = 0; i < kVectors; ++i) {
+      const T* q = p + (i * kThreads + threadIdx.x) * kRowElems;
+      if constexpr (sizeof(T) == 4) ptx::ld_global_32B(q, r[i].w);
+      else *reinterpret_cast<uint4*>(r[i].w) = *reinterpret_cast<const uint4*>(q);
+    }
     return;
   }
 #pragma unroll
@@ -79,9 +80,9 @@ __device__ __forceinline__ void store_vector(T* p, int64_t left, bool wide, int 
   RowWords<T> r;
   pack(v, r);
   if (wide && left >= kChunk) {
-#pragma unroll
-    for (int w = 0; w < int(sizeof(RowWords<T>) / 16); ++w)
-      reinterpret_cast<uint4*>(p + (i * kThreads + threadIdx.x) * kRowElems)[w] = reinterpret_cast<const uint4*>(r.w)[w];
+    T* q = p + (i * kThreads + threadIdx.x) * kRowElems;
+    if constexpr (sizeof(T) == 4) ptx::st_global_32B(q, r.w);
+    else *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(r.w);
     return;
   }
   const int64_t at = (int64_t)i * kThreads * kRowElems;
@@ -263,7 +264,7 @@ template <int N> bool fill(Table<N>* t, const fdb_clip_grads_params& p, int firs
     e.first_chunk = (uint32_t)chunks;
     e.dtype = (uint8_t)g.dtype;
     e.out_dtype = (uint8_t)g.out_dtype;
-    e.wide = p.scale != 0 ? aligned_to(16, g.data, g.out) : aligned_to(16, g.data);
+    e.wide = aligned_to(8 * type_bytes(g.dtype), g.data) && (p.scale == 0 || aligned_to(8 * type_bytes(g.out_dtype), g.out));
     e.same = g.out == g.data;
     chunks += (uint64_t)((g.count + kChunk - 1) / kChunk);
     if (chunks > 0xffffffffull) return false;

@@ -31,26 +31,28 @@ __device__ __forceinline__ uint64_t gelu_erf2(uint64_t v) {
 // The same for results that are kept in more than bf16, or come from values far below zero: 1/2 erfc(z) = t P(t) e^(-z^2) with
 // t = 1 / (1 + 0.375 z) and P of degree 6 fitted here for the smallest relative error (9.2e-7 over 0 <= z <= 12; 3.4e-6 in fp32 with
 // the exponential's argument rounded), and v Phi(v) = max(v, 0) - |v| 1/2 erfc(|v| / sqrt 2), which loses nothing where Phi(v) is
-// small.  Two FMAs a pair more than gelu_erf2.  +inf stays, -inf gives zero, NaN stays.
+// small.  +inf stays, -inf gives zero, NaN stays.
 __device__ __forceinline__ uint64_t gelu_tail2(uint64_t v) {
   auto both = [](float c) { return ptx::pack_f32x2(c, c); };
-  const uint64_t z = ptx::mul_f32x2(v & 0x7fffffff7fffffffull, both(0.70710678118654752f));
-  float d0, d1, e0, e1, t0, t1, v0, v1;
-  ptx::unpack_f32x2(ptx::fma_f32x2(both(0.375f), z, both(1.f)), d0, d1);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(d0));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(d1));
-  ptx::unpack_f32x2(ptx::mul_f32x2(ptx::mul_f32x2(z, z), both(-1.4426950408889634f)), e0, e1);
-  const uint64_t e = ptx::pack_f32x2(ptx::ex2(e0), ptx::ex2(e1)), t = ptx::pack_f32x2(t0, t1);
-  uint64_t p = ptx::fma_f32x2(both(-0.06661498370203611f), t, both(0.19073576888425917f));
-  p = ptx::fma_f32x2(p, t, both(-0.06032194842606266f));
-  p = ptx::fma_f32x2(p, t, both(0.13837509530295133f));
-  p = ptx::fma_f32x2(p, t, both(0.08452121837156336f));
-  p = ptx::fma_f32x2(p, t, both(0.10761853239249744f));
-  p = ptx::fma_f32x2(p, t, both(0.10568661785036586f));
-  const uint64_t q = ptx::mul_f32x2(ptx::mul_f32x2(p, t), e);
+  float v0, v1, d0, d1, e0, e1, t0, t1, r, r0, r1;
   ptx::unpack_f32x2(v, v0, v1);
-  const uint64_t low = ptx::pack_f32x2(fmaxf(-fabsf(v0), -1e4f), fmaxf(-fabsf(v1), -1e4f));  // (an infinity times zero is a NaN)
-  return ptx::fma_f32x2(low, q, ptx::pack_f32x2(fmaxf(v0, 0.f), fmaxf(v1, 0.f)));
+  const uint64_t a = ptx::pack_f32x2(fminf(fabsf(v0), 1e4f), fminf(fabsf(v1), 1e4f));  // (an infinity times zero would be a NaN)
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r0) : "f"(v0));
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r1) : "f"(v1));
+  ptx::unpack_f32x2(ptx::fma_f32x2(a, both(0.375f * 0.70710678118654752f), both(1.f)), d0, d1);
+  // one reciprocal for both (of at most 2653^2): the special-function unit has the exponentials to do as well
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
+  t0 = r * d1;
+  t1 = r * d0;
+  ptx::unpack_f32x2(ptx::mul_f32x2(ptx::mul_f32x2(a, both(-0.5f * 1.4426950408889634f)), a), e0, e1);
+  const uint64_t e = ptx::pack_f32x2(ptx::ex2(e0), ptx::ex2(e1)), t = ptx::pack_f32x2(t0, t1);
+  uint64_t p = ptx::fma_f32x2(both(0.06661498370203611f), t, both(-0.19073576888425917f));  // -P: what is taken off
+  p = ptx::fma_f32x2(p, t, both(0.06032194842606266f));
+  p = ptx::fma_f32x2(p, t, both(-0.13837509530295133f));
+  p = ptx::fma_f32x2(p, t, both(-0.08452121837156336f));
+  p = ptx::fma_f32x2(p, t, both(-0.10761853239249744f));
+  p = ptx::fma_f32x2(p, t, both(-0.10568661785036586f));
+  return ptx::fma_f32x2(ptx::mul_f32x2(a, e), ptx::mul_f32x2(p, t), ptx::pack_f32x2(r0, r1));
 }
 
 }  // namespace fdb

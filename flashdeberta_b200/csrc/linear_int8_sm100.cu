@@ -5,7 +5,7 @@
 // (CG = 1) or 256 rows (CG = 2, a pair of CTAs on two SMs) x BN output features, K in steps of 128 bytes through a ring of stages:
 //   warp 0  TMA, the CTA's 128 x 128 bytes of x and its BN / CG rows of the weight; what lies behind the ends arrives as zeros
 //   warp 1  (of the pair's even CTA) tcgen05.mma, four per stage; two accumulators in tensor memory
-//   warps 2-9: epilogue, two warps per 32-lane quarter of tensor memory: both scales, bias, activation in fp32, one rounding
+//   the other warps: epilogue, two or four per 32-lane quarter of tensor memory: both scales, bias, activation in fp32, one rounding
 // A stage holds as many bytes as in the bf16 kernel and takes as many clocks (measured), for twice the products.
 // Every wait is bounded; on a timeout the CTA raises FDB_DEV_TIMEOUT in the status word, frees its tensor memory and returns.
 // No TMA multicast.
@@ -27,11 +27,10 @@ namespace {
 using namespace ptx;
 
 constexpr int kBM = 128, kBK = 128;
-constexpr int kThreads = 320;
-constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 8;
+constexpr int kTmaWarp = 0, kMmaWarp = 1, kEpiWarp0 = 2;
 
 struct Int8Args {
-  CUtensorMap tm_x, tm_w;
+  CUtensorMap tm_x, tm_w, tm_out;
   const float *x_scale, *w_scale;
   const void* bias;
   void* out;
@@ -39,14 +38,16 @@ struct Int8Args {
   int64_t rows;
   int k, n, tiles_n;
   bool bias_fp32;  // else of the output's type
-  bool wide;       // rows of the output start on 16 bytes, scales and bias too, and n is a multiple of 8
+  bool wide;       // rows of the output start on 16 bytes, scales and bias too
 };
+
+constexpr int kTurnWords = 32 * 16;  // of the epilogue's stage, per warp
 
 template <int CG, int BN> struct Tile {
   static constexpr uint32_t kBytesA = kBM * kBK, kBytesW = BN / CG * kBK, kStageBytes = kBytesA + kBytesW;
   static constexpr int kStages = BN == 64 ? 6 : (BN == 256 ? 6 : (CG == 2 ? 8 : 6));
-  static constexpr uint32_t kPitch = 33;  // words of a row of the epilogue's transposition
-  static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemBars = kSmemTurn + kEpiWarps * 32 * kPitch * 4;
+  static constexpr int kEpiWarps = BN == 64 ? 8 : 16, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+  static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemBars = kSmemTurn + kEpiWarps * kTurnWords * 4;
   enum : uint32_t { kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2, kNumBars = 2 * kStages + 4 };
   static constexpr uint32_t kSmemBytes = kSmemBars + 8 * kNumBars + 16 + 1024;  // + tensor-memory slot, abort flag, alignment slack
   static constexpr uint32_t kTmemCols = 2 * BN;
@@ -59,10 +60,22 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, floa
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// A pair of 32-bit integers as floats, each rounded once.  The conversion instruction goes through the special-function unit (16 a
+// clock and SM), where the GELU's exponentials queue; MAGIC takes the upper and the lower half of the integer (its sign bit
+// flipped) as the mantissas of 2^23 + half and puts them together in one FMA, whose rounding is the only one.
+template <bool MAGIC> __device__ __forceinline__ uint64_t float_pair(uint32_t a0, uint32_t a1) {
+  if constexpr (!MAGIC) return pack_f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1));
+  a0 ^= 0x80000000u;
+  a1 ^= 0x80000000u;
+  const uint64_t hi = pack_f32x2(__uint_as_float(__byte_perm(a0, 0x4B00u, 0x5432)), __uint_as_float(__byte_perm(a1, 0x4B00u, 0x5432)));
+  const uint64_t lo = pack_f32x2(__uint_as_float(__byte_perm(a0, 0x4B00u, 0x5410)), __uint_as_float(__byte_perm(a1, 0x4B00u, 0x5410)));
+  const float off_hi = -(8388608.f + 32768.f), off_lo = -8388608.f;
+  return fma_f32x2(add_f32x2(hi, pack_f32x2(off_hi, off_hi)), pack_f32x2(65536.f, 65536.f), add_f32x2(lo, pack_f32x2(off_lo, off_lo)));
+}
+
 // A pair of columns: the sums scaled, bias added, activation.
-template <bool GELU> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
-  const uint64_t acc = pack_f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1));
-  const uint64_t v = fma_f32x2(mul_f32x2(acc, w_scale), x_scale, bias);
+template <bool GELU, bool MAGIC> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
+  const uint64_t v = fma_f32x2(mul_f32x2(float_pair<MAGIC>(a0, a1), w_scale), x_scale, bias);
   return GELU ? gelu_tail2(v) : v;
 }
 
@@ -71,71 +84,100 @@ template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a
   return a.bias_fp32 ? __ldg(static_cast<const float*>(a.bias) + n) : to_float<T>(static_cast<const T*>(a.bias)[n]);
 }
 
-// 32 columns of a row per thread, the thread's own row; every column exists and rows may be written in 16-byte pieces.
+// 32 columns of 32 rows per warp, each thread its own row: through 64 bytes of shared memory per row and a TMA store per 64 bytes of
+// columns, which leaves out what lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 54 at
+// 16384 x 1024 -> 4096.)  Column piece p (16 bytes) of row r lies at piece p ^ (r / 2 % 4), the map's swizzle: no bank conflicts.
 template <typename T, bool GELU>
-__device__ __forceinline__ void store_direct(const Int8Args& a, const uint32_t (&acc)[32], int64_t row, int n0, float x_scale, bool live) {
+__device__ __forceinline__ void store_tile(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, uint32_t* stage, int lane) {
   const uint64_t sx = pack_f32x2(x_scale, x_scale);
-  T* out = static_cast<T*>(a.out) + row * a.n + n0;
+  constexpr int kCols = 64 / sizeof(T);  // of one store
 #pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    float ws[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    *reinterpret_cast<float4*>(ws) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c));
-    *reinterpret_cast<float4*>(ws + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c + 4));
-    if (a.bias != nullptr) {
-      if (a.bias_fp32) {
-        *reinterpret_cast<float4*>(b) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c));
-        *reinterpret_cast<float4*>(b + 4) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c + 4));
-      } else if constexpr (sizeof(T) == 2) {
-        RowWords<T> r;
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + n0 + c));
-        r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
-        unpack(r, b);
-      }
-    }
-    uint32_t o[8];
+  for (int part = 0; part < 32; part += kCols) {
+    uint32_t o[16];
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      float v0, v1;
-      unpack_f32x2(finish_pair<GELU>(acc[c + e], acc[c + e + 1], pack_f32x2(ws[e], ws[e + 1]), sx, pack_f32x2(b[e], b[e + 1])), v0, v1);
-      if constexpr (sizeof(T) == 4) {
-        o[e] = __float_as_uint(v0);
-        o[e + 1] = __float_as_uint(v1);
+    for (int c = part; c < part + kCols; c += 8) {
+      float ws[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      const bool full = n0 + c + 8 <= a.n;  // (else n is no multiple of 8: single columns)
+      if (full) {
+        *reinterpret_cast<float4*>(ws) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c));
+        *reinterpret_cast<float4*>(ws + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c + 4));
+        if (a.bias != nullptr) {
+          if (a.bias_fp32) {
+            *reinterpret_cast<float4*>(b) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c));
+            *reinterpret_cast<float4*>(b + 4) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c + 4));
+          } else if constexpr (sizeof(T) == 2) {
+            RowWords<T> r;
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + n0 + c));
+            r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+            unpack(r, b);
+          }
+        }
       } else {
-        o[e >> 1] = pack_pair<T>(v0, v1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ws[e] = n0 + c + e < a.n ? __ldg(a.w_scale + n0 + c + e) : 0.f;
+          if (n0 + c + e < a.n) b[e] = bias_at<T>(a, n0 + c + e);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        float v0, v1;
+        // (half of the integers either way: neither the special-function unit nor the issue slots are full then)
+        const uint64_t ws2 = pack_f32x2(ws[e], ws[e + 1]), b2 = pack_f32x2(b[e], b[e + 1]);
+        unpack_f32x2(e % 4 == 0 ? finish_pair<GELU, GELU>(acc[c + e], acc[c + e + 1], ws2, sx, b2) : finish_pair<GELU, false>(acc[c + e], acc[c + e + 1], ws2, sx, b2),
+                     v0, v1);
+        if constexpr (sizeof(T) == 4) {
+          o[c - part + e] = __float_as_uint(v0);
+          o[c - part + e + 1] = __float_as_uint(v1);
+        } else {
+          o[(c - part + e) >> 1] = pack_pair<T>(v0, v1);
+        }
       }
     }
-    if (live) {
-      *reinterpret_cast<uint4*>(out + c) = make_uint4(o[0], o[1], o[2], o[3]);
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out + c + 4) = make_uint4(o[4], o[5], o[6], o[7]);
+    tma_store_wait_read();  // the store before has left the stage (each lane waits for its own, and there is one that issues)
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      *reinterpret_cast<uint4*>(stage + lane * 16 + 4 * (p ^ ((lane >> 1) & 3))) = make_uint4(o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0 && n0 + part < a.n) {
+      tma_store_2d(&a.tm_out, smem_u32(stage), n0 + part, (int)row0);
+      tma_store_commit();
     }
   }
 }
 
-// The same where a row starts anywhere or columns are missing: through shared memory, a row of 32 columns at a time across the lanes.
-// (A thread writing its own row element by element would touch 32 sectors with every store.)
+// The same where a row starts anywhere or columns are missing: through shared memory, two rows of 16 columns at a time across the
+// lanes.  (A thread writing its own row element by element would touch 32 sectors with every store.)  Column c of row r lies in word
+// 16 r + (c ^ (r / 2 % 16)): neither side of the turn has two lanes on one bank.
 template <typename T, bool GELU>
 __device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, uint32_t* turn, int lane) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) turn[lane * 33 + c] = acc[c];
-  __syncwarp();
-  const int n = n0 + lane;
-  const bool has = n < a.n;
-  const float ws = has ? __ldg(a.w_scale + n) : 0.f, b = has ? bias_at<T>(a, n) : 0.f;
-  const uint64_t ws2 = pack_f32x2(ws, ws), b2 = pack_f32x2(b, b);
-  T* out = static_cast<T*>(a.out) + row0 * a.n + n;
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) turn[lane * 16 + (c ^ ((lane >> 1) & 15))] = acc[half * 16 + c];
+    __syncwarp();
+    const int c = lane & 15, up = lane >> 4, n = n0 + half * 16 + c;
+    const bool has = n < a.n;
+    const float ws = has ? __ldg(a.w_scale + n) : 0.f, b = has ? bias_at<T>(a, n) : 0.f;
+    const uint64_t ws2 = pack_f32x2(ws, ws), b2 = pack_f32x2(b, b);
+    T* out = static_cast<T*>(a.out) + row0 * a.n + n;
 #pragma unroll 4
-  for (int r = 0; r < 32; r += 2) {
-    const float s0 = __shfl_sync(0xffffffffu, x_scale, r), s1 = __shfl_sync(0xffffffffu, x_scale, r + 1);
-    float v0, v1;
-    unpack_f32x2(finish_pair<GELU>(turn[r * 33 + lane], turn[(r + 1) * 33 + lane], ws2, pack_f32x2(s0, s1), b2), v0, v1);
-    if (has && row0 + r < a.rows) out[(int64_t)r * a.n] = from_float<T>(v0);
-    if (has && row0 + r + 1 < a.rows) out[(int64_t)(r + 1) * a.n] = from_float<T>(v1);
+    for (int r = 0; r < 32; r += 4) {
+      const int r0 = r + up, r1 = r + 2 + up;
+      const float s0 = __shfl_sync(0xffffffffu, x_scale, r0), s1 = __shfl_sync(0xffffffffu, x_scale, r1);
+      float v0, v1;
+      unpack_f32x2(finish_pair<GELU, false>(turn[r0 * 16 + (c ^ ((r0 >> 1) & 15))], turn[r1 * 16 + (c ^ ((r1 >> 1) & 15))], ws2, pack_f32x2(s0, s1), b2), v0, v1);
+      if (has && row0 + r0 < a.rows) out[(int64_t)r0 * a.n] = from_float<T>(v0);
+      if (has && row0 + r1 < a.rows) out[(int64_t)r1 * a.n] = from_float<T>(v1);
+    }
+    __syncwarp();
   }
-  __syncwarp();
 }
 
 template <int CG, int BN, typename OUT, bool GELU>
-__global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_constant__ Int8Args args) {
+__global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(const __grid_constant__ Int8Args args) {
   using T = Tile<CG, BN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -149,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
 
   if (tid == 0) {
     *abort_flag = 0u;
-    for (uint32_t i = 0; i < T::kNumBars; ++i) mbar_init(bar(i), (i >= T::kBarAccEmpty) ? uint32_t(kEpiWarps * CG) : 1u);
+    for (uint32_t i = 0; i < T::kNumBars; ++i) mbar_init(bar(i), (i >= T::kBarAccEmpty) ? uint32_t(T::kEpiWarps * CG) : 1u);
     fence_barrier_init();
     tma_prefetch_desc(&args.tm_x);
     tma_prefetch_desc(&args.tm_w);
@@ -242,27 +284,26 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
     }
   } else {
     const int quarter = warp & 3;                // the 32 tensor-memory lanes this warp may read
-    const int half = (warp - kEpiWarp0) >> 2;    // which half of the tile's columns
-    constexpr int kChunks = BN / 64;             // 32 columns at a time
+    constexpr int kCols = BN * 4 / T::kEpiWarps, kChunks = kCols / 32;  // this warp's columns of the tile; 32 at a time
+    const int part = (warp - kEpiWarp0) >> 2;
     const uint32_t tmem_lane = tmem_base + (uint32_t(quarter * 32) << 16);
-    uint32_t* turn = reinterpret_cast<uint32_t*>(smem_gen + T::kSmemTurn) + (warp - kEpiWarp0) * 32 * T::kPitch;
+    uint32_t* turn = reinterpret_cast<uint32_t*>(smem_gen + T::kSmemTurn) + (warp - kEpiWarp0) * kTurnWords;
     uint32_t acc_empty[2] = {bar(T::kBarAccEmpty), bar(T::kBarAccEmpty + 1)};
     if constexpr (CG == 2) { acc_empty[0] = map_to_rank(acc_empty[0], 0); acc_empty[1] = map_to_rank(acc_empty[1], 0); }
     uint32_t local = 0;
 #pragma unroll 1
     for (int tile = first; tile < num_tiles; tile += step, ++local) {
       const int64_t row0 = (int64_t)(tile / args.tiles_n) * (kBM * CG) + int(rank) * kBM + quarter * 32;
-      const int n0 = (tile % args.tiles_n) * BN + half * (BN / 2);
+      const int n0 = (tile % args.tiles_n) * BN + part * kCols;
       const uint32_t acc = local & 1u;
-      const bool live = row0 + lane < args.rows;
-      const float x_scale = live ? __ldg(args.x_scale + row0 + lane) : 0.f;
+      const float x_scale = row0 + lane < args.rows ? __ldg(args.x_scale + row0 + lane) : 0.f;
       wait(bar(T::kBarAccFull + acc), (local >> 1) & 1u);
       tc_fence_after();
 #pragma unroll 1
       for (int ch = 0; ch < kChunks; ++ch) {
         uint32_t a[32];
         if (ok) {  // whole warps execute the load, whatever their rows
-          tmem_ld32(tmem_lane + acc * BN + uint32_t(half * (BN / 2) + ch * 32), a);
+          tmem_ld32(tmem_lane + acc * BN + uint32_t(part * kCols + ch * 32), a);
           tmem_wait_ld();
         }
         if (ch == kChunks - 1) {  // the accumulator is in registers: the next tile but one may overwrite it
@@ -272,11 +313,13 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_kernel(const __grid_c
         }
         const int n = n0 + ch * 32;
         if (!ok || n >= args.n || row0 >= args.rows) continue;
-        if (args.wide && n + 32 <= args.n) store_direct<OUT, GELU>(args, a, row0 + lane, n, x_scale, live);
+        if (args.wide) store_tile<OUT, GELU>(args, a, row0, n, x_scale, turn, lane);
         else store_turned<OUT, GELU>(args, a, row0, n, x_scale, turn, lane);
       }
     }
   }
+
+  if (warp >= kEpiWarp0 && lane == 0) tma_store_wait();
 
   // ---- teardown ----
   tc_fence_before();
@@ -299,7 +342,7 @@ int launch(const Int8Args& a, int grid, bool chained, cudaStream_t stream) {
   static std::atomic<uint64_t> smem_done{0};
   auto kernel = linear_int8_kernel<CG, BN, OUT, GELU>;
   cudaError_t e = allow_smem(smem_done, reinterpret_cast<const void*>(kernel), (int)Tile<CG, BN>::kSmemBytes);
-  if (e == cudaSuccess) e = launch_kernel<Int8Args>(kernel, a, dim3((unsigned)grid), kThreads, Tile<CG, BN>::kSmemBytes, chained, stream, CG);
+  if (e == cudaSuccess) e = launch_kernel<Int8Args>(kernel, a, dim3((unsigned)grid), Tile<CG, BN>::kThreads, Tile<CG, BN>::kSmemBytes, chained, stream, CG);
   if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "linear_int8 launch: %s", cudaGetErrorString(e));
   return FDB_OK;
 }
@@ -394,7 +437,13 @@ extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* st
   a.rows = p->rows; a.k = p->in_features; a.n = p->out_features;
   a.tiles_n = (p->out_features + best->bn - 1) / best->bn;
   a.bias_fp32 = p->bias_dtype == FDB_FP32;
-  a.wide = p->out_features % 8 == 0 && aligned_to(16, p->out, p->weight_scale, p->bias);
+  a.wide = p->out_features * (int64_t)type_bytes(p->out_dtype) % 16 == 0 && aligned_to(16, p->out, p->weight_scale, p->bias);
+  if (a.wide) {
+    const CUtensorMapDataType type = p->out_dtype == FDB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                              : (p->out_dtype == FDB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
+    rc = make_map_out(&a.tm_out, p->out, p->rows, p->out_features, type, (int)type_bytes(p->out_dtype), 32, "out");
+    if (rc != FDB_OK) return rc;
+  }
   const int units = sms / best->cg;
   const int grid = (int)(best_tiles < units ? best_tiles : units) * best->cg;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

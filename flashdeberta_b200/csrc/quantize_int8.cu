@@ -1,8 +1,8 @@
 // Rows as 8-bit integers with a scale each (fdb_quantize_int8): scale = amax / 127, y = rint(x * (127 / amax)).
 //
-// A team of warps per row (row_team.cuh); a row of up to 8192 elements is read once and stays in registers, a longer one is read a
-// second time (it comes from L2 then).  HBM-bound: x read, one byte per element written.  The magnitudes are compared as the bits of
-// their absolute values: a NaN is larger than everything there, so it reaches the scale.
+// A warp per row of up to 1024 elements, up to eight warps beyond (row_team.cuh); a row of up to 8192 is read once and stays in
+// registers, a longer one is read a second time (it comes from L2 then).  HBM-bound: x read, one byte per element written.  The
+// magnitudes are compared as the bits of their absolute values: a NaN is larger than everything there, so it reaches the scale.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -14,7 +14,7 @@
 namespace fdb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128, kWarpElems = 1024;
 
 struct QuantArgs {
   const void* x;
@@ -24,25 +24,26 @@ struct QuantArgs {
   int cols, team_threads, teams;
 };
 
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(1024) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
-  __shared__ uint32_t s_top[kThreads / 32][2][32];
+template <typename T, bool WIDE, int V>
+__global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
+  constexpr int kElems = V * kRowElems;
+  __shared__ uint32_t s_top[kThreads / 32][2][8];
   const int team = threadIdx.x / a.team_threads, t = threadIdx.x - team * a.team_threads;
-  const int warps = a.team_threads / 32, span = a.team_threads * kRowElems;
+  const int warps = a.team_threads / 32, span = a.team_threads * kElems;
   ptx::grid_launch();
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * a.teams + team; row < a.rows; row += (int64_t)gridDim.x * a.teams) {
     const T* x = static_cast<const T*>(a.x) + row * a.cols;
     uint32_t top = 0;
-    RowWords<T> first;
-    float v[kRowElems];
+    RowWords<T, V> first;
+    float v[kElems];
     for (int at = 0; at < a.cols; at += span) {
-      const RowColumns<WIDE> cols{t, a.team_threads, a.cols - at};
-      RowWords<T> r;
+      const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
+      RowWords<T, V> r;
       cols.load(x + at, r);
       unpack(r, v);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      for (int j = 0; j < kElems; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
       if (at == 0) first = r;
     }
     top = __reduce_max_sync(0xffffffffu, top);
@@ -58,35 +59,41 @@ __global__ void __launch_bounds__(1024) quantize_int8_kernel(const __grid_consta
     const float inv = zero || top >= 0x7f800000u ? 0.f : 127.f / amax;
     if (t == 0) a.scale[row] = zero ? 0.f : amax / 127.f;
     for (int at = 0; at < a.cols; at += span) {
-      const RowColumns<WIDE> cols{t, a.team_threads, a.cols - at};
-      RowWords<T> r = first;
+      const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
+      RowWords<T, V> r = first;
       if (at != 0) cols.load(x + at, r);
       unpack(r, v);
-      int q[kRowElems];
+      int q[kElems];
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) q[j] = inv == 0.f ? 0 : __float2int_rn(v[j] * inv);
+      for (int j = 0; j < kElems; ++j) q[j] = inv == 0.f ? 0 : __float2int_rn(v[j] * inv);
       uint8_t* y = a.y + row * a.pitch + at;
       if constexpr (WIDE) {
-        uint2 o;
-        o.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
-        o.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
-        if (cols.live(0)) *reinterpret_cast<uint2*>(y + t * kRowElems) = o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int* p = q + i * kRowElems;
+          uint2 o;
+          o.x = (p[0] & 255) | (p[1] & 255) << 8 | (p[2] & 255) << 16 | p[3] << 24;
+          o.y = (p[4] & 255) | (p[5] & 255) << 8 | (p[6] & 255) << 16 | p[7] << 24;
+          if (cols.live(i * kRowElems)) *reinterpret_cast<uint2*>(y + cols.col(i * kRowElems)) = o;
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < kRowElems; ++j)
+        for (int j = 0; j < kElems; ++j)
           if (cols.live(j)) y[cols.col(j)] = (uint8_t)q[j];
       }
     }
   }
 }
 
-template <typename T>
-cudaError_t launch(const QuantArgs& a, bool wide, cudaStream_t s) {
+template <typename T, bool WIDE>
+cudaError_t launch(const QuantArgs& a, int v, cudaStream_t s) {
   const int threads = a.teams * a.team_threads;
   const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (2048 / threads);
   const unsigned grid = (unsigned)std::min(want, most);
-  if (wide) quantize_int8_kernel<T, true><<<grid, threads, 0, s>>>(a);
-  else quantize_int8_kernel<T, false><<<grid, threads, 0, s>>>(a);
+  if (v == 1) quantize_int8_kernel<T, WIDE, 1><<<grid, threads, 0, s>>>(a);
+  else if (v == 2) quantize_int8_kernel<T, WIDE, 2><<<grid, threads, 0, s>>>(a);
+  else if (v == 3) quantize_int8_kernel<T, WIDE, 3><<<grid, threads, 0, s>>>(a);
+  else quantize_int8_kernel<T, WIDE, 4><<<grid, threads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -94,11 +101,14 @@ cudaError_t launch(const QuantArgs& a, bool wide, cudaStream_t s) {
 
 int launch_quantize_int8(const void* x, int dtype, int64_t rows, int cols, void* y, int64_t pitch, float* scale, void* stream) {
   QuantArgs a = {x, static_cast<uint8_t*>(y), scale, rows, pitch, cols, 0, 0};
-  a.team_threads = row_team_threads(std::min(cols, kRowHiddenMax));
+  const int warps = std::min(8, (cols + kWarpElems - 1) / kWarpElems), v = std::min(4, (cols + warps * 256 - 1) / (warps * 256));
+  a.team_threads = warps * 32;
   a.teams = std::max(1, kThreads / a.team_threads);
-  const bool wide = cols % kRowElems == 0 && aligned_to(16, x) && aligned_to(8, y) && pitch % 8 == 0;
+  const bool wide = cols % kRowElems == 0 && aligned_to(dtype == FDB_FP32 ? 32 : 16, x) && aligned_to(8, y) && pitch % 8 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == FDB_BF16 ? launch<__nv_bfloat16>(a, wide, s) : (dtype == FDB_FP16 ? launch<__half>(a, wide, s) : launch<float>(a, wide, s));
+#define FDB_QUANT(T) (wide ? launch<T, true>(a, v, s) : launch<T, false>(a, v, s))
+  const cudaError_t e = dtype == FDB_BF16 ? FDB_QUANT(__nv_bfloat16) : (dtype == FDB_FP16 ? FDB_QUANT(__half) : FDB_QUANT(float));
+#undef FDB_QUANT
   if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "quantize_int8 launch: %s", cudaGetErrorString(e));
   return FDB_OK;
 }

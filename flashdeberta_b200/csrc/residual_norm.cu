@@ -32,99 +32,6 @@
 namespace fdb {
 namespace {
 
-constexpr int kFwdThreads = 256;
-
-template <typename T, bool RMS, bool POST, bool WIDE>
-__global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
-  __shared__ float s_sums[kFwdThreads / 32][2 * 32];
-  const int team = threadIdx.x / a.team_threads, t = threadIdx.x - team * a.team_threads;
-  const RowColumns<WIDE> cols{t, a.team_threads, a.hidden};
-  TeamSum<1> team_sum{s_sums[team], a.team_threads / 32, t >> 5, team + 1, 0};
-  const float inv_hidden = 1.f / (float)a.hidden;
-  const T* x = static_cast<const T*>(a.x);
-  const T* residual = static_cast<const T*>(a.residual);
-
-  // statistics of a row; afterwards v holds its normalised form
-  auto normalise = [&](float (&v)[kRowElems], float& mean, float& inv) {
-    float sum[1] = {0.f};
-    mean = 0.f;
-    if constexpr (!RMS) {
-#pragma unroll
-      for (int j = 0; j < kRowElems; ++j) sum[0] += v[j];
-      team_sum(sum);
-      mean = sum[0] * inv_hidden;
-      sum[0] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < kRowElems; ++j) {
-      v[j] = cols.live(j) ? v[j] - mean : 0.f;
-      sum[0] = fmaf(v[j], v[j], sum[0]);
-    }
-    team_sum(sum);
-    inv = 1.f / sqrtf(fmaf(sum[0], inv_hidden, a.eps));
-#pragma unroll
-    for (int j = 0; j < kRowElems; ++j) v[j] *= inv;
-  };
-  auto affine = [&](float (&v)[kRowElems], const void* weight, const void* bias) {
-    float p[kRowElems];
-    cols.template load_param<T>(weight, a.param_fp32, 0, p);
-#pragma unroll
-    for (int j = 0; j < kRowElems; ++j) v[j] *= p[j];
-    if (bias == nullptr) return;
-    cols.template load_param<T>(bias, a.param_fp32, 0, p);
-#pragma unroll
-    for (int j = 0; j < kRowElems; ++j) v[j] += p[j];
-  };
-
-  for (int64_t row = (int64_t)blockIdx.x * a.teams + team; row < a.rows; row += (int64_t)gridDim.x * a.teams) {
-    const int64_t at = row * a.hidden;
-    RowWords<T> rx, rr;
-    cols.load(x + at, rx);
-    if (residual != nullptr) cols.load(residual + at, rr);
-    float v[kRowElems], p[kRowElems];
-    float4 stats = make_float4(0.f, 1.f, 0.f, 1.f);
-    unpack(rx, v);
-    if constexpr (POST) {
-      normalise(v, stats.x, stats.y);
-      affine(v, a.post_weight, a.post_bias);
-    }
-    if (a.gate != nullptr) {
-      cols.template load_param<T>(a.gate, a.gate_fp32, (int64_t)((uint32_t)row / a.gate_rows) * a.hidden, p);
-#pragma unroll
-      for (int j = 0; j < kRowElems; ++j) v[j] *= p[j];
-    }
-    if (residual != nullptr) {
-      unpack(rr, p);
-#pragma unroll
-      for (int j = 0; j < kRowElems; ++j) v[j] = fmaf(a.residual_scale, p[j], v[j]);
-    }
-    if (a.stream != nullptr) cols.store(static_cast<T*>(a.stream) + at, v);
-    normalise(v, stats.z, stats.w);
-    affine(v, a.weight, a.bias);
-    cols.store(static_cast<T*>(a.normed) + at, v);
-    if (a.stats != nullptr && t == 0) a.stats[row] = stats;
-  }
-}
-
-template <typename T, bool RMS, bool POST, bool WIDE>
-int launch(const ResidualNormArgs& a, cudaStream_t s) {
-  const int64_t want = (a.rows + a.teams - 1) / a.teams;
-  const int64_t most = (int64_t)std::max(1, sm_count()) * (2048 / (a.teams * a.team_threads));
-  residual_norm_kernel<T, RMS, POST, WIDE><<<(unsigned)std::min(want, most), (unsigned)(a.teams * a.team_threads), 0, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm launch: %s", cudaGetErrorString(e));
-  return FDB_OK;
-}
-
-template <typename T>
-int launch_type(const ResidualNormArgs& a, bool wide, cudaStream_t s) {
-#define FDB_NORM(RMS, POST) (wide ? launch<T, RMS, POST, true>(a, s) : launch<T, RMS, POST, false>(a, s))
-  const bool post = a.post_weight != nullptr;
-  if (a.rms) return post ? FDB_NORM(true, true) : FDB_NORM(true, false);
-  return post ? FDB_NORM(false, true) : FDB_NORM(false, false);
-#undef FDB_NORM
-}
-
 unsigned type_bytes(int dtype) { return dtype == FDB_FP32 ? 4u : 2u; }
 
 // Checks of a call and its kernel arguments; `wide`: rows and vectors may be read in 16-byte pieces.
@@ -150,8 +57,8 @@ int prepare(const fdb_residual_norm_params* p, ResidualNormArgs* a, bool* wide) 
   if (!aligned_to(size, p->x, p->residual, p->normed, p->stream) || !aligned_to(param, p->weight, p->bias, p->post_weight, p->post_bias) ||
       (p->gate != nullptr && !aligned_to(gate, p->gate)) || !aligned_to(16, p->stats))
     return fail(FDB_ERR_ALIGNMENT, "residual_norm: tensors must be aligned to their elements, stats to 16 bytes");
-  *wide = p->hidden % kRowElems == 0 &&
-          aligned_to(16, p->x, p->residual, p->normed, p->stream, p->weight, p->bias, p->post_weight, p->post_bias, p->gate);
+  *wide = p->hidden % kRowElems == 0 && aligned_to(8 * size, p->x, p->residual, p->normed, p->stream) &&
+          aligned_to(8 * param, p->weight, p->bias, p->post_weight, p->post_bias) && (p->gate == nullptr || aligned_to(8 * gate, p->gate));
   a->x = p->x; a->residual = p->residual;
   a->weight = p->weight; a->bias = p->bias; a->post_weight = p->post_weight; a->post_bias = p->post_bias; a->gate = p->gate;
   a->normed = p->normed; a->stream = p->stream; a->stats = reinterpret_cast<float4*>(p->stats);
@@ -159,8 +66,7 @@ int prepare(const fdb_residual_norm_params* p, ResidualNormArgs* a, bool* wide) 
   a->hidden = p->hidden;
   a->residual_scale = p->residual_scale; a->eps = p->eps;
   a->rms = p->rms != 0; a->param_fp32 = p->param_dtype == FDB_FP32; a->gate_fp32 = p->gate_dtype == FDB_FP32;
-  a->team_threads = row_team_threads(p->hidden);
-  a->teams = std::max(1, kFwdThreads / a->team_threads);
+  a->team_threads = a->teams = 0;
   return FDB_OK;
 }
 
@@ -171,14 +77,12 @@ int gate_mode(const fdb_residual_norm_params& p) {
 }
 
 // Teams, CTAs and workspace of a backward call.
-void plan(const fdb_residual_norm_params& p, bool wide, ResidualNormBwdArgs* b, uint64_t* bytes) {
+void plan(const fdb_residual_norm_params& p, ResidualNormBwdArgs* b, uint64_t* bytes) {
   const int mode = gate_mode(p);
+  b->f.team_threads = row_team_threads(p.hidden);
   b->f.teams = std::max(1, kNormBwdThreads / b->f.team_threads);
-  const int threads = b->f.teams * b->f.team_threads;
-  auto resident_of = p.dtype == FDB_BF16 ? norm_bwd_resident_bf16 : (p.dtype == FDB_FP16 ? norm_bwd_resident_fp16 : norm_bwd_resident_fp32);
-  const int resident = resident_of(p.rms != 0, p.post_weight != nullptr, mode, wide, threads, b->f.teams);
   const int64_t want = (p.rows + b->f.teams - 1) / b->f.teams;
-  b->ctas = (int)std::max<int64_t>(1, std::min(want, (int64_t)std::max(1, sm_count()) * std::max(1, resident)));
+  b->ctas = (int)std::max<int64_t>(1, std::min<int64_t>(want, std::max(1, sm_count())));
   b->workers = std::min((int64_t)b->ctas * b->f.teams, p.rows);  // each has a row
   b->vectors = (p.rms != 0 ? 1 : 2) * 2;  // of weight and bias, and A and B or what they become
   b->groups = mode == kGateGroups ? (int)(p.rows / p.gate_rows) : 0;
@@ -287,8 +191,8 @@ extern "C" FDB_API int fdb_residual_norm(const fdb_residual_norm_params* p, void
   if (rc != FDB_OK) return rc;
   if (p->rows == 0) return FDB_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->dtype == FDB_BF16) return launch_type<__nv_bfloat16>(a, wide, s);
-  return p->dtype == FDB_FP16 ? launch_type<__half>(a, wide, s) : launch_type<float>(a, wide, s);
+  if (p->dtype == FDB_BF16) return norm_fwd_launch_bf16(a, wide, s);
+  return p->dtype == FDB_FP16 ? norm_fwd_launch_fp16(a, wide, s) : norm_fwd_launch_fp32(a, wide, s);
 }
 
 namespace {
@@ -296,9 +200,9 @@ int prepare_bwd(const fdb_residual_norm_bwd_params* p, ResidualNormBwdArgs* b, b
   if (p == nullptr || p->struct_bytes != sizeof(fdb_residual_norm_bwd_params))
     return fail(FDB_ERR_INVALID_ARGUMENT, "fdb_residual_norm_bwd_params: NULL or struct_bytes %u != %zu", p ? p->struct_bytes : 0u,
                 sizeof(fdb_residual_norm_bwd_params));
-  int rc = prepare(p->fwd, &b->f, wide);
+  int rc = prepare(&p->fwd, &b->f, wide);
   if (rc != FDB_OK) return rc;
-  const fdb_residual_norm_params& f = *p->fwd;
+  const fdb_residual_norm_params& f = p->fwd;
   if (f.stats == nullptr || (p->dnormed == nullptr && p->dstream == nullptr) || p->dx == nullptr)
     return fail(FDB_ERR_INVALID_ARGUMENT, "residual_norm backward: stats, dx and one of dnormed and dstream must not be NULL");
   if ((p->dresidual != nullptr && f.residual == nullptr) || (p->dbias != nullptr && f.bias == nullptr) ||
@@ -309,11 +213,12 @@ int prepare_bwd(const fdb_residual_norm_bwd_params* p, ResidualNormBwdArgs* b, b
   if (!aligned_to(size, p->dnormed, p->dstream, p->dx, p->dresidual) || !aligned_to(param, p->dweight, p->dbias, p->dpost_weight, p->dpost_bias) ||
       (p->dgate != nullptr && !aligned_to(gate, p->dgate)))
     return fail(FDB_ERR_ALIGNMENT, "residual_norm backward: tensors must be aligned to their elements");
-  *wide = *wide && aligned_to(16, p->dnormed, p->dstream, p->dx, p->dresidual, p->dgate);
+  *wide = *wide && aligned_to(8 * size, p->dnormed, p->dstream, p->dx, p->dresidual) && (p->dgate == nullptr || aligned_to(8 * gate, p->dgate)) &&
+          aligned_to(32, p->workspace);
   b->dnormed = p->dnormed; b->dstream = p->dstream; b->dx = p->dx; b->dresidual = p->dresidual;
   b->dweight = p->dweight; b->dbias = p->dbias; b->dpost_weight = p->dpost_weight; b->dpost_bias = p->dpost_bias; b->dgate = p->dgate;
   b->mode = gate_mode(f);
-  plan(f, *wide, b, bytes);
+  plan(f, b, bytes);
   return FDB_OK;
 }
 }  // namespace
@@ -333,21 +238,21 @@ extern "C" FDB_API int fdb_residual_norm_bwd(const fdb_residual_norm_bwd_params*
   uint64_t bytes = 0;
   int rc = prepare_bwd(p, &b, &wide, &bytes);
   if (rc != FDB_OK) return rc;
-  if (p->workspace == nullptr || p->workspace_bytes < bytes || !aligned_to(16, p->workspace))
-    return fail(FDB_ERR_WORKSPACE, "residual_norm backward: workspace of %llu bytes needed (16-byte aligned), %llu given",
+  if (p->workspace == nullptr || p->workspace_bytes < bytes || !aligned_to(32, p->workspace))
+    return fail(FDB_ERR_WORKSPACE, "residual_norm backward: workspace of %llu bytes needed (32-byte aligned), %llu given",
                 (unsigned long long)bytes, (unsigned long long)p->workspace_bytes);
   b.parts = static_cast<float*>(p->workspace);
   b.slots = b.parts + (int64_t)b.ctas * b.vectors * b.f.hidden;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // (without rows the CTA that is launched has none either: it leaves sums of zero)
-  auto launch_rows = p->fwd->dtype == FDB_BF16 ? norm_bwd_launch_bf16 : (p->fwd->dtype == FDB_FP16 ? norm_bwd_launch_fp16 : norm_bwd_launch_fp32);
+  auto launch_rows = p->fwd.dtype == FDB_BF16 ? norm_bwd_launch_bf16 : (p->fwd.dtype == FDB_FP16 ? norm_bwd_launch_fp16 : norm_bwd_launch_fp32);
   if ((rc = launch_rows(b, wide, s)) != FDB_OK) return rc;
   const bool group_gate = b.groups > 0 && b.dgate != nullptr;
   if (b.dweight == nullptr && b.dbias == nullptr && b.dpost_weight == nullptr && b.dpost_bias == nullptr && (b.dgate == nullptr || b.mode == kGateElement))
     return FDB_OK;
   const dim3 grid((unsigned)((b.f.hidden + kFinishCols - 1) / kFinishCols), (unsigned)(1 + (group_gate ? std::min(b.groups, 1024) : 0)));
-  auto kernel = p->fwd->dtype == FDB_BF16 ? residual_norm_sums_kernel<__nv_bfloat16>
-                                          : (p->fwd->dtype == FDB_FP16 ? residual_norm_sums_kernel<__half> : residual_norm_sums_kernel<float>);
+  auto kernel = p->fwd.dtype == FDB_BF16 ? residual_norm_sums_kernel<__nv_bfloat16>
+                                          : (p->fwd.dtype == FDB_FP16 ? residual_norm_sums_kernel<__half> : residual_norm_sums_kernel<float>);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kFinishCols, kFinishRows);

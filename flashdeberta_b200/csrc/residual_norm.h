@@ -31,18 +31,18 @@ struct ResidualNormBwdArgs {
   int ctas, vectors, mode, groups;
 };
 
-constexpr int kNormBwdThreads = 512;  // threads of a CTA whose rows are shorter than it
+constexpr int kNormBwdThreads = 512;  // threads of a backward CTA whose rows take fewer: one CTA per SM, of several rows at a time
 
 // the worker that has a row
 __host__ __device__ inline int64_t residual_norm_worker_of(int64_t row, int64_t rows, int64_t workers) { return ((row + 1) * workers - 1) / rows; }
 
-// The row kernel of the backward, per type of rows: CTAs that an SM holds; its launch.
-#define FDB_NORM_BWD(TYPE)                                                                                      \
-  int norm_bwd_resident_##TYPE(bool rms, bool post, int mode, bool wide, int threads, int teams);               \
+// The row kernels, per type of rows.
+#define FDB_NORM(TYPE)                                                                \
+  int norm_fwd_launch_##TYPE(const ResidualNormArgs& a, bool wide, cudaStream_t s);   \
   int norm_bwd_launch_##TYPE(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s);
-FDB_NORM_BWD(bf16)
-FDB_NORM_BWD(fp16)
-FDB_NORM_BWD(fp32)
-#undef FDB_NORM_BWD
+FDB_NORM(bf16)
+FDB_NORM(fp16)
+FDB_NORM(fp32)
+#undef FDB_NORM
 
 }  // namespace fdb

@@ -2,8 +2,6 @@
 // translation unit.
 #pragma once
 
-#include <atomic>
-
 #include "internal.h"
 #include "launch.h"
 #include "residual_norm.h"
@@ -14,37 +12,27 @@ namespace fdb {
 constexpr int kNormBwdTeams = kNormBwdThreads / 32;
 constexpr size_t kNormBwdPlainSmem = 40 * 1024;  // with the 8 KB of the teams' sums, what a launch may take without being asked
 
-// Shared memory of a CTA: the teams' sums, one vector of sums per thread for adding teams up and, where the gate has groups, what
-// C = sum gate A and D = sum gate B have come to (touched only when a group ends).
+// Shared memory of a CTA: weight, post_weight, post_bias and a channel's gate in fp32 (read for every row, converted once), one vector of
+// sums per thread for adding teams up and, where the gate has groups, what C = sum gate A and D = sum gate B have come to (touched
+// only when a group ends).
 inline size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode) {
-  const size_t vector = size_t(threads) * kRowElems * sizeof(float);
-  return (teams > 1 ? vector : 0) + (post && mode == kGateGroups ? 2 * vector : 0);
+  const size_t vector = size_t(threads) * kRowElems * sizeof(float), params = size_t(threads / teams) * kRowElems * sizeof(float);
+  return 4 * params + (teams > 1 ? vector : 0) + (post && mode == kGateGroups ? 2 * vector : 0);
 }
 
 template <typename T, bool RMS, bool POST, int GATE, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormBwdArgs b) {
+  constexpr int kSums = RMS ? 1 : 2;  // per norm and row; and vectors of sums over rows: weight, bias
   extern __shared__ __align__(16) float s_vectors[];
-  __shared__ float s_sums[kNormBwdTeams][2 * 32 * 2];
+  __shared__ __align__(16) float s_sums[kNormBwdTeams][TeamSum<kSums>::kSlots];
   const ResidualNormArgs& f = b.f;
   const int team = threadIdx.x / f.team_threads, t = threadIdx.x - team * f.team_threads;
   const RowColumns<WIDE> cols{t, f.team_threads, f.hidden};
-  TeamSum<2> team_sum{s_sums[team], f.team_threads / 32, t >> 5, team + 1, 0};
+  TeamSum<kSums> team_sum{s_sums[team], f.team_threads / 32, t >> 5, team + 1, 0};
   const float inv_hidden = 1.f / (float)f.hidden;
   const int64_t worker = (int64_t)blockIdx.x * f.teams + team;
   const bool has_rows = worker < b.workers;
   const int64_t first = has_rows ? f.rows * worker / b.workers : 0, end = has_rows ? f.rows * (worker + 1) / b.workers : 0;
-  constexpr int kNorms = RMS ? 1 : 2;  // vectors of sums per norm: weight, bias
-
-  float sum_w[kRowElems], sum_b[kRowElems], sum_A[kRowElems], sum_B[kRowElems];
-#pragma unroll
-  for (int j = 0; j < kRowElems; ++j) sum_w[j] = sum_b[j] = sum_A[j] = sum_B[j] = 0.f;
-  float* s_team = s_vectors;
-  float* s_C = s_vectors + (f.teams > 1 ? blockDim.x * kRowElems : 0) + threadIdx.x * kRowElems;
-  float* s_D = s_C + blockDim.x * kRowElems;
-  if constexpr (GATE == kGateGroups && POST) {
-#pragma unroll
-    for (int j = 0; j < kRowElems; ++j) s_C[j] = s_D[j] = 0.f;
-  }
   ptx::grid_launch();
 
   struct Row { RowWords<T> x, residual, dnormed, dstream, gate; float4 stats; };
@@ -58,6 +46,44 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     if (element_gate) cols.load(static_cast<const T*>(f.gate) + at, r.gate);
     r.stats = __ldg(f.stats + row);
   };
+  Row now, next;
+  if (first < end) fetch(first, now);
+
+  // vectors over the columns: two 16-byte pieces per thread, each piece of the team's threads side by side
+  enum : int { kWeight = 0, kPostWeight = 1, kPostBias = 2, kGateVector = 3 };
+  auto vector_at = [&](int v) { return reinterpret_cast<float4*>(s_vectors) + v * 2 * f.team_threads + t; };
+  auto put_vector = [&](int v, const void* p, bool fp32) {
+    float q[kRowElems];
+    if (p != nullptr) cols.template load_param<T>(p, fp32, 0, q);
+    else
+#pragma unroll
+      for (int j = 0; j < kRowElems; ++j) q[j] = v == kGateVector ? 1.f : 0.f;
+    vector_at(v)[0] = make_float4(q[0], q[1], q[2], q[3]);
+    vector_at(v)[f.team_threads] = make_float4(q[4], q[5], q[6], q[7]);
+  };
+  auto get_vector = [&](int v, float (&q)[kRowElems]) {
+    const float4 lo = vector_at(v)[0], hi = vector_at(v)[f.team_threads];
+    q[0] = lo.x; q[1] = lo.y; q[2] = lo.z; q[3] = lo.w; q[4] = hi.x; q[5] = hi.y; q[6] = hi.z; q[7] = hi.w;
+  };
+  if (team == 0) {
+    put_vector(kWeight, f.weight, f.param_fp32);
+    put_vector(kPostWeight, f.post_weight, f.param_fp32);
+    put_vector(kPostBias, f.post_bias, f.param_fp32);
+    put_vector(kGateVector, GATE == kGateChannel ? f.gate : nullptr, f.gate_fp32);
+  }
+  float* s_team = s_vectors + 4 * f.team_threads * kRowElems;
+  float* s_C = s_team + (f.teams > 1 ? blockDim.x * kRowElems : 0) + threadIdx.x * kRowElems;
+  float* s_D = s_C + blockDim.x * kRowElems;
+  if constexpr (GATE == kGateGroups && POST) {
+#pragma unroll
+    for (int j = 0; j < kRowElems; ++j) s_C[j] = s_D[j] = 0.f;
+  }
+  for (int i = threadIdx.x; i < int(sizeof(s_sums) / sizeof(float)); i += blockDim.x) s_sums[0][i] = 0.f;
+  __syncthreads();
+
+  float sum_w[kRowElems], sum_b[kRowElems], sum_A[kRowElems], sum_B[kRowElems];
+#pragma unroll
+  for (int j = 0; j < kRowElems; ++j) sum_w[j] = sum_b[j] = sum_A[j] = sum_B[j] = 0.f;
   // A and B of a group leave the registers
   auto leave_group = [&](int64_t group, const float (&gate)[kRowElems]) {
     float* slot = b.slots + (worker + group) * 2 * f.hidden;
@@ -73,8 +99,6 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     }
   };
 
-  Row now, next;
-  if (first < end) fetch(first, now);
   int64_t group = -1;
   float g[kRowElems];
 #pragma unroll
@@ -92,22 +116,22 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     } else if constexpr (GATE == kGateElement) {
       if (element_gate) unpack(now.gate, g);
       else if (f.gate != nullptr) cols.load(static_cast<const float*>(f.gate) + at, g);
-    } else if (f.gate != nullptr) {
-      cols.template load_param<T>(f.gate, f.gate_fp32, 0, g);
+    } else {
+      get_vector(kGateVector, g);
     }
 
     // the stream again; hat: x normalised (x itself without the norm), z: the stream normalised
     float hat[kRowElems], u[kRowElems], z[kRowElems], d[kRowElems], p[kRowElems];
     unpack(now.x, hat);
     if constexpr (POST) {
-      cols.template load_param<T>(f.post_weight, f.param_fp32, 0, p);
+      get_vector(kPostWeight, p);
 #pragma unroll
       for (int j = 0; j < kRowElems; ++j) {
         hat[j] = (RMS ? hat[j] : hat[j] - now.stats.x) * now.stats.y;
         u[j] = hat[j] * p[j];
       }
-      if (f.post_bias != nullptr) {
-        cols.template load_param<T>(f.post_bias, f.param_fp32, 0, p);
+      if constexpr (!RMS) {
+        get_vector(kPostBias, p);
 #pragma unroll
         for (int j = 0; j < kRowElems; ++j) u[j] += p[j];
       }
@@ -126,23 +150,23 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     for (int j = 0; j < kRowElems; ++j) z[j] = (RMS ? z[j] : z[j] - now.stats.z) * now.stats.w;
 
     // dz, the gradient of the stream in all
-    float sums[2] = {0.f, 0.f};
+    float sums[kSums];
+    for (float& v : sums) v = 0.f;
     if (b.dnormed != nullptr) {
       unpack(now.dnormed, d);
-      cols.template load_param<T>(f.weight, f.param_fp32, 0, p);
+      get_vector(kWeight, p);
 #pragma unroll
       for (int j = 0; j < kRowElems; ++j) {
         sum_w[j] = fmaf(d[j], z[j], sum_w[j]);
         if constexpr (!RMS) sum_b[j] += d[j];
         d[j] *= p[j];
         sums[0] = fmaf(d[j], z[j], sums[0]);
-        if constexpr (!RMS) sums[1] += d[j];
+        if constexpr (!RMS) sums[kSums - 1] += d[j];
       }
       team_sum(sums);
-      sums[0] *= inv_hidden;
-      sums[1] *= inv_hidden;
+      for (float& v : sums) v *= inv_hidden;
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.w * (d[j] - fmaf(z[j], sums[0], RMS ? 0.f : sums[1]));
+      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.w * (d[j] - fmaf(z[j], sums[0], RMS ? 0.f : sums[kSums - 1]));
     } else {
 #pragma unroll
       for (int j = 0; j < kRowElems; ++j) d[j] = 0.f;
@@ -177,19 +201,18 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
       for (int j = 0; j < kRowElems; ++j) d[j] *= g[j];
     }
     if constexpr (POST) {
-      cols.template load_param<T>(f.post_weight, f.param_fp32, 0, p);
-      sums[0] = sums[1] = 0.f;
+      get_vector(kPostWeight, p);
+      for (float& v : sums) v = 0.f;
 #pragma unroll
       for (int j = 0; j < kRowElems; ++j) {
         d[j] *= p[j];
         sums[0] = fmaf(d[j], hat[j], sums[0]);
-        if constexpr (!RMS) sums[1] += d[j];
+        if constexpr (!RMS) sums[kSums - 1] += d[j];
       }
       team_sum(sums);
-      sums[0] *= inv_hidden;
-      sums[1] *= inv_hidden;
+      for (float& v : sums) v *= inv_hidden;
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.y * (d[j] - fmaf(hat[j], sums[0], RMS ? 0.f : sums[1]));
+      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.y * (d[j] - fmaf(hat[j], sums[0], RMS ? 0.f : sums[kSums - 1]));
     }
     cols.store(static_cast<T*>(b.dx) + at, d);
     now = next;
@@ -226,8 +249,8 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
   };
   write(sum_w, 0);
   if constexpr (!RMS) write(sum_b, 1);
-  write(sum_A, kNorms);
-  if constexpr (!RMS) write(sum_B, kNorms + 1);
+  write(sum_A, kSums);
+  if constexpr (!RMS) write(sum_B, kSums + 1);
 }
 
 // WIDE stores of fp32 sums need rows of them to start on 16 bytes: they do, hidden being a multiple of 8 there.
@@ -241,19 +264,6 @@ auto with_norm_bwd_kernel(bool rms, bool post, int mode, bool wide, int threads,
 #undef FDB_BWD4
 #undef FDB_BWD3
 #undef FDB_BWD2
-}
-
-template <typename T> int norm_bwd_resident(bool rms, bool post, int mode, bool wide, int threads, int teams) {
-  return with_norm_bwd_kernel<T>(rms, post, mode, wide, threads, [&](auto kernel) {
-    int n = 0;
-    const size_t smem = residual_norm_bwd_smem(threads, teams, post, mode);
-    if (smem > kNormBwdPlainSmem) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) {
-      cudaGetLastError();
-      n = 1;
-    }
-    return n;
-  });
 }
 
 template <typename T> int norm_bwd_launch(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s) {

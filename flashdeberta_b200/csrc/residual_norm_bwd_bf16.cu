@@ -2,8 +2,5 @@
 #include "residual_norm_bwd.cuh"
 
 namespace fdb {
-int norm_bwd_resident_bf16(bool rms, bool post, int mode, bool wide, int threads, int teams) {
-  return norm_bwd_resident<__nv_bfloat16>(rms, post, mode, wide, threads, teams);
-}
 int norm_bwd_launch_bf16(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s) { return norm_bwd_launch<__nv_bfloat16>(b, wide, s); }
 }  // namespace fdb

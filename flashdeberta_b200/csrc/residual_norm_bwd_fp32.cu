@@ -2,8 +2,5 @@
 #include "residual_norm_bwd.cuh"
 
 namespace fdb {
-int norm_bwd_resident_fp32(bool rms, bool post, int mode, bool wide, int threads, int teams) {
-  return norm_bwd_resident<float>(rms, post, mode, wide, threads, teams);
-}
 int norm_bwd_launch_fp32(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s) { return norm_bwd_launch<float>(b, wide, s); }
 }  // namespace fdb

@@ -5,7 +5,7 @@ the 8-bit form of what ``ops.linear_gelu`` does in bf16.  Forward only.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -34,23 +34,22 @@ def int8_rows(t: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor):
     """(address, pitch) of a matrix whose rows start on 16 bytes, else None."""
-    cols = t.shape[-1]
-    if cols > 1 and t.stride(-1) != 1 or t.data_ptr() % 16 != 0:
+    shape, strides, at = t.shape, t.stride(), t.data_ptr()
+    cols = shape[-1]
+    if at % 16 != 0 or (strides[-1] != 1 and cols > 1):
         return None
-    rows = t.numel() // cols if cols else 0
-    if rows <= 1:
-        return t.data_ptr(), _pitch(cols)
-    pitch = inner = None
-    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):  # the leading dimensions as one
+    pitch = inner = 0
+    for n, s in zip(shape[-2::-1], strides[-2::-1]):  # the leading dimensions as one
         if n == 1:
             continue
-        if pitch is None:
-            pitch, inner = s, n * s
+        if pitch == 0:
+            pitch = s
         elif s != inner:
             return None
-        else:
-            inner = n * s
-    return (t.data_ptr(), pitch) if pitch % 16 == 0 and pitch >= cols else None
+        inner = n * s
+    if pitch == 0:  # one row: any will do
+        return at, _pitch(cols)
+    return (at, pitch) if pitch % 16 == 0 and pitch >= cols else None
 
 
 def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -88,36 +87,41 @@ def _(x, weight, weight_scale, bias, x_scale, gelu, out_dtype):
     return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype)
 
 
+_PARAMS = struct.Struct("@IiPqPPqPPPq6iPQP")  # fdb_linear_int8_params
+
+
 def _call(x, weight, weight_scale, bias, x_scale, gelu, out_dtype):
-    k, n, dev = x.shape[-1], weight.shape[0], x.device
-    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=dev)
+    shape, n, device = x.shape, weight.shape[0], x.device
+    out = x.new_empty((*shape[:-1], n), dtype=out_dtype)
     if out.numel() == 0:
         return out
-    rows = out.numel() // n
-    weight_scale = weight_scale if weight_scale.is_contiguous() else weight_scale.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    weight = int8_rows(weight)
-    w_at, w_pitch = _rows(weight)
-    x_pitch = 0
-    if x_scale is not None:
-        x = int8_rows(x)
-        x_at, x_pitch = _rows(x)
-        x_scale = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
-    else:
-        x = x if x.is_contiguous() else x.contiguous()
-        x_at = x.data_ptr()
-    p = _lib.LinearInt8Params(
-        C.sizeof(_lib.LinearInt8Params), _lib.FDB_INT8 if x_scale is not None else TYPES[x.dtype], x_at, x_pitch,
-        None if x_scale is None else x_scale.data_ptr(), w_at, w_pitch, weight_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-        out.data_ptr(), rows, k, n, 0 if bias is None else TYPES[bias.dtype], TYPES[out_dtype], int(gelu), 0, None, 0,
-        ops._status_word(dev).data_ptr())
+    if not weight_scale.is_contiguous():
+        weight_scale = weight_scale.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    w = _rows(weight)
+    if w is None:
+        weight = int8_rows(weight)
+        w = _rows(weight)
+    rows, k = out.numel() // n, shape[-1]
     lib = _lib.load()
-    with ops.on_device(dev):
-        need = lib.fdb_linear_int8_workspace_bytes(C.byref(p))
-        if need:
-            ws = torch.empty(need + 255, dtype=torch.uint8, device=dev)
-            p.workspace, p.workspace_bytes = (ws.data_ptr() + 255) & ~255, need
-        _lib.check(lib.fdb_linear_int8(C.byref(p), ops.raw_stream(dev)))
+    with ops.on_device(device):
+        if x_scale is None:
+            x = x if x.is_contiguous() else x.contiguous()
+            x_at, x_pitch, kind, scale_at = x.data_ptr(), 0, TYPES[x.dtype], 0
+            need = lib.fdb_linear_int8_workspace_bytes(_PARAMS.pack(_PARAMS.size, kind, 0, 0, 0, 0, 0, 0, 0, 0, rows, k, n, 0, 0, 0, 0, 0, 0, 0))
+            ws = x.new_empty(need + 255, dtype=torch.uint8)
+            ws_at = (ws.data_ptr() + 255) & ~255
+        else:
+            x_scale = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
+            x = int8_rows(x)
+            (x_at, x_pitch), kind, scale_at = _rows(x), _lib.FDB_INT8, x_scale.data_ptr()
+            need = ws_at = 0
+        p = _PARAMS.pack(
+            _PARAMS.size, kind, x_at, x_pitch, scale_at, w[0], w[1], weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            out.data_ptr(), rows, k, n, 0 if bias is None else TYPES[bias.dtype], TYPES[out_dtype], gelu, 0, ws_at, need,
+            ops._status_word(device).data_ptr())
+        _lib.check(lib.fdb_linear_int8(p, ops.raw_stream(device)))
     ops._launches += 1 + int(need > 0)
     return out
 

@@ -7,7 +7,7 @@ trains, takes every width up to 8192 and bf16, fp16 and fp32 rows.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -20,58 +20,60 @@ MAX_HIDDEN = 8192
 
 def _gate_rows(gate: torch.Tensor, shape) -> Optional[int]:
     """Rows of ``shape`` that share a row of the gate, or None where the gate's rows do not each cover one run of rows."""
-    given = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
-    if given[-1] != shape[-1]:
+    own = gate.shape
+    if own[-1] != shape[-1]:
         return None
-    lead, own = tuple(shape[:-1]), given[:-1]
+    own, lead = (1,) * (len(shape) - len(own)) + tuple(own[:-1]), shape[:-1]
     i = 0
     while i < len(lead) and own[i] == lead[i]:
         i += 1
-    if any(n != 1 for n in own[i:]):
-        return None
     rows = 1
-    for n in lead[i:]:
+    for n, mine in zip(lead[i:], own[i:]):
+        if mine != 1:
+            return None
         rows *= n
     return rows
 
 
 def _checked(x, residual, weight, bias, post_weight, post_bias, gate, rms):
     """Raises on what the operator does not take; returns the gate as it is passed on (broadcast where it has to be)."""
+    shape, dtype, device = x.shape, x.dtype, x.device
     if not x.is_cuda:
         raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
-    if x.dtype not in TYPES:
-        raise TypeError(f"residual_norm takes bfloat16, float16 or float32 rows, not {x.dtype}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_HIDDEN:
+    if dtype not in TYPES:
+        raise TypeError(f"residual_norm takes bfloat16, float16 or float32 rows, not {dtype}")
+    if len(shape) < 1 or not 1 <= shape[-1] <= MAX_HIDDEN:
         raise ValueError(f"residual_norm takes rows of 1 to {MAX_HIDDEN} elements")
-    hidden = x.shape[-1]
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("residual must match x in shape and dtype")
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != dtype:
+            raise ValueError("residual must match x in shape and dtype")
+        if residual.device != device:
+            raise ValueError(f"residual is on {residual.device}, x on {device}")
     if rms and (bias is not None or post_bias is not None):
         raise ValueError("the RMS norm takes no bias")
     if post_bias is not None and post_weight is None:
         raise ValueError("post_bias needs post_weight")
+    vector, kind = shape[-1:], weight.dtype
     for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
         if t is None:
             continue
-        if t.shape != (hidden,):
-            raise ValueError(f"{name} must have shape ({hidden},), got {tuple(t.shape)}")
-        if t.dtype != weight.dtype or t.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"{name} must be {x.dtype} or float32, the norms' parameters all alike; got {t.dtype}")
-    for name, t in (("residual", residual), ("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias),
-                    ("gate", gate)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        if t.shape != vector:
+            raise ValueError(f"{name} must have shape {tuple(vector)}, got {tuple(t.shape)}")
+        if t.dtype != kind or (kind != dtype and kind != torch.float32):
+            raise TypeError(f"{name} must be {dtype} or float32, the norms' parameters all alike; got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, x on {device}")
     if gate is None:
         return None
-    if gate.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"gate must be {x.dtype} or float32, got {gate.dtype}")
-    if gate.dim() > x.dim():
-        raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
-    if _gate_rows(gate, x.shape) is None:  # shared in some other way: one per element then
+    if gate.dtype != dtype and gate.dtype != torch.float32:
+        raise TypeError(f"gate must be {dtype} or float32, got {gate.dtype}")
+    if gate.device != device:
+        raise ValueError(f"gate is on {gate.device}, x on {device}")
+    if gate.dim() == 0 or gate.dim() > len(shape) or _gate_rows(gate, shape) is None:  # shared in some other way: one per element then
         try:
-            return gate.expand(x.shape)
+            return gate.expand(shape)
         except RuntimeError:
-            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}") from None
+            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
     return gate
 
 
@@ -79,52 +81,58 @@ def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _address(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale):
-    """The C call's parameters over contiguous tensors."""
-    rows = x.numel() // x.shape[-1]
-    return _lib.ResidualNormParams(
-        C.sizeof(_lib.ResidualNormParams), TYPES[x.dtype], x.data_ptr(), _address(residual), weight.data_ptr(), _address(bias),
-        _address(post_weight), _address(post_bias), _address(gate), normed.data_ptr(), _address(stream), _address(stats), rows,
-        0 if gate is None else _gate_rows(gate, x.shape), x.shape[-1], TYPES[weight.dtype], 0 if gate is None else TYPES[gate.dtype],
-        int(rms), residual_scale, eps)
+# fdb_residual_norm_params and, behind it, what fdb_residual_norm_bwd_params adds: packed in one step (a ctypes structure of
+# so many fields takes as long as the launch)
+_FWD, _BWD = struct.Struct("@Ii10P2q4i2f"), struct.Struct("@Ii")
+_BWD_TAIL = struct.Struct("@10PQ")
+
+
+def _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale) -> bytes:
+    """fdb_residual_norm_params over contiguous tensors."""
+    shape = x.shape
+    return _FWD.pack(
+        _FWD.size, TYPES[x.dtype], x.data_ptr(), _address(residual), weight.data_ptr(), _address(bias), _address(post_weight),
+        _address(post_bias), _address(gate), normed.data_ptr(), _address(stream), _address(stats), x.numel() // shape[-1],
+        0 if gate is None else _gate_rows(gate, shape), shape[-1], TYPES[weight.dtype], 0 if gate is None else TYPES[gate.dtype], rms,
+        residual_scale, eps)
 
 
 def _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, keep):
     """(normed, stream, stats); the statistics where a backward will want them (``keep``), else None."""
-    x, residual, weight, bias, post_weight, post_bias, gate = map(_dense, (x, residual, weight, bias, post_weight, post_bias, gate))
+    x, residual, weight, bias, post_weight, post_bias, gate = [
+        t if t is None or t.is_contiguous() else t.contiguous() for t in (x, residual, weight, bias, post_weight, post_bias, gate)]
     normed, stream = torch.empty_like(x), torch.empty_like(x)
-    stats = torch.empty(x.numel() // x.shape[-1], 4, dtype=torch.float32, device=x.device) if keep else None
+    stats = x.new_empty((x.numel() // x.shape[-1], 4), dtype=torch.float32) if keep else None
     if x.numel() == 0:
         return normed, stream, stats
     p = _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale)
-    with ops.on_device(x.device):
-        _lib.check(_lib.load().fdb_residual_norm(C.byref(p), ops.raw_stream(x.device)))
+    device = x.device
+    with ops.on_device(device):
+        _lib.check(_lib.load().fdb_residual_norm(p, ops.raw_stream(device)))
     ops._launches += 1
     return normed, stream, stats
 
 
 def _backward(dnormed, dstream, x, residual, weight, bias, post_weight, post_bias, gate, stats, eps, rms, residual_scale, wanted):
     """Gradients of x, residual, weight, bias, post_weight, post_bias and gate; None where ``wanted`` is false."""
-    tensors = [_dense(t) for t in (x, residual, weight, bias, post_weight, post_bias, gate)]
+    tensors = [t if t is None or t.is_contiguous() else t.contiguous() for t in (x, residual, weight, bias, post_weight, post_bias, gate)]
     x = tensors[0]
-    grads = [torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and w else None for t, w in zip(tensors, wanted)]
+    grads = [torch.empty_like(t) if w and t is not None else None for t, w in zip(tensors, wanted)]
     if x.numel() == 0 or (dnormed is None and dstream is None):
         return [None if g is None else g.zero_() for g in grads]
     dnormed, dstream = _dense(dnormed), _dense(dstream)
     dx = grads[0] if grads[0] is not None else torch.empty_like(x)
-    lib = _lib.load()
-    p = _params(*tensors, x, None, stats, eps, rms, residual_scale)
-    b = _lib.ResidualNormBwdParams(C.sizeof(_lib.ResidualNormBwdParams), 0, C.pointer(p), _address(dnormed), _address(dstream), dx.data_ptr(),
-                                   *(_address(g) for g in grads[1:]))
-    with ops.on_device(x.device):
-        need = lib.fdb_residual_norm_bwd_workspace_bytes(C.byref(b))
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        b.workspace, b.workspace_bytes = ws.data_ptr(), need
-        _lib.check(lib.fdb_residual_norm_bwd(C.byref(b), ops.raw_stream(x.device)))
+    lib, device = _lib.load(), x.device
+    head = _BWD.pack(_BWD.size + _FWD.size + _BWD_TAIL.size, 0) + _params(*tensors, x, None, stats, eps, rms, residual_scale)
+    addresses = (_address(dnormed), _address(dstream), dx.data_ptr(), *map(_address, grads[1:]))
+    with ops.on_device(device):
+        need = lib.fdb_residual_norm_bwd_workspace_bytes(head + _BWD_TAIL.pack(*addresses, 0, 0))
+        ws = x.new_empty(need, dtype=torch.uint8)
+        _lib.check(lib.fdb_residual_norm_bwd(head + _BWD_TAIL.pack(*addresses, ws.data_ptr(), need), ops.raw_stream(device)))
     ops._launches += 1 + int(any(g is not None for g in grads[2:]))
     return grads
 
@@ -176,25 +184,23 @@ residual_norm_op.register_autograd(_op_backward, setup_context=_setup)
 
 
 class _ResidualNorm(torch.autograd.Function):
-    """The training call outside tracing."""
+    """The training call outside tracing.  (forward takes ctx: with a setup_context of its own, torch binds the arguments to the
+    signature on every call, which takes longer than the kernels of a short batch.)"""
 
     @staticmethod
-    def forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale):
-        return _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, True)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        _setup(ctx, inputs, output)
+    def forward(ctx, x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale):
+        normed, stream, stats = _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, True)
+        ctx.save_for_backward(x, residual, weight, bias, post_weight, post_bias, gate, stats)
+        ctx.norm_args = (eps, rms, residual_scale)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(output[2])
+        return normed, stream
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dnormed, dstream, _):
-        if any(ops.intercepted(g) or (g is not None and ops.batched(g)) for g in (dnormed, dstream)):
-            return _op_backward(ctx, dnormed, dstream, _)
-        *tensors, stats = ctx.saved_tensors
-        grads = _backward(dnormed, dstream, *tensors, stats, *ctx.norm_args, ctx.needs_input_grad[:7])
+    def backward(ctx, dnormed, dstream):
+        if ops.intercepted(dnormed, dstream) or any(g is not None and ops.batched(g) for g in (dnormed, dstream)):
+            return _op_backward(ctx, dnormed, dstream, None)
+        grads = _backward(dnormed, dstream, *ctx.saved_tensors, *ctx.norm_args, ctx.needs_input_grad)
         return (*grads, None, None, None)
 
 
@@ -215,5 +221,5 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: tor
     if ops.intercepted(*call[:7]):
         return residual_norm_op(*call)[:2]
     if ops.wants_grad(*call[:7]):
-        return _ResidualNorm.apply(*call)[:2]
+        return _ResidualNorm.apply(*call)
     return _forward(*call, False)[:2]

@@ -460,8 +460,8 @@ FDB_API int fdb_encoder_forward(fdb_encoder_call* c, void* stream);
  * fdb_add_layernorm this takes every type and width, keeps what a backward needs and does not round the sum before the norm.
  * x, residual, normed, stream: (rows, hidden) contiguous, all of `dtype` (bf16, fp16 or fp32), hidden at most 8192; weights and
  * biases (hidden) of that type or fp32 (`param_dtype`).  Row r takes row r / gate_rows of the gate, (rows / gate_rows, hidden) of
- * `gate_dtype`: gate_rows = rows is a gate per channel, 1 one per element.  Pointers are aligned to their elements; 16-byte pieces are
- * used where hidden and every pointer allow it.  Statistics and sums are fp32; each result is rounded once.
+ * `gate_dtype`: gate_rows = rows is a gate per channel, 1 one per element.  Pointers are aligned to their elements; pieces of eight
+ * elements are used where hidden is a multiple of 8 and every pointer allows it.  Statistics and sums are fp32; each result is rounded once.
  */
 typedef struct fdb_residual_norm_params {
   uint32_t struct_bytes;   /* sizeof(fdb_residual_norm_params), checked */
@@ -484,10 +484,10 @@ FDB_API int fdb_residual_norm(const fdb_residual_norm_params* p, void* stream);
 typedef struct fdb_residual_norm_bwd_params {
   uint32_t struct_bytes;   /* sizeof(fdb_residual_norm_bwd_params), checked */
   int32_t reserved;
-  const fdb_residual_norm_params* fwd;
+  fdb_residual_norm_params fwd;
   const void *dnormed, *dstream;
   void *dx, *dresidual, *dweight, *dbias, *dpost_weight, *dpost_bias, *dgate;
-  void* workspace;         /* device, >= fdb_residual_norm_bwd_workspace_bytes(), 16-byte aligned */
+  void* workspace;         /* device, >= fdb_residual_norm_bwd_workspace_bytes(), 32-byte aligned */
   uint64_t workspace_bytes;
 } fdb_residual_norm_bwd_params;
 FDB_API uint64_t fdb_residual_norm_bwd_workspace_bytes(const fdb_residual_norm_bwd_params* p);

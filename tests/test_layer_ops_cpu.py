@@ -60,12 +60,24 @@ def test_residual_norm_without_rows_is_a_no_op():
 ])
 def test_residual_norm_backward_argument_errors(change, fwd, code):
     p = _norm(**fwd)
-    b = _lib.ResidualNormBwdParams(C.sizeof(_lib.ResidualNormBwdParams), 0, C.pointer(p), *[P] * 10, 1 << 30)
+    b = _lib.ResidualNormBwdParams(C.sizeof(_lib.ResidualNormBwdParams), 0, p, *[P] * 10, 1 << 30)
     for k, v in change.items():
         setattr(b, k, v)
     lib = _lib.load()
     assert lib.fdb_residual_norm_bwd_workspace_bytes(C.byref(b)) == 0
     _refused(lib.fdb_residual_norm_bwd(C.byref(b), None), code)
+
+
+def test_packed_parameters_have_the_structs_layout():
+    from flashdeberta_b200 import int8, norms
+    assert norms._FWD.size == C.sizeof(_lib.ResidualNormParams) and int8._PARAMS.size == C.sizeof(_lib.LinearInt8Params)
+    assert norms._BWD.size + norms._FWD.size + norms._BWD_TAIL.size == C.sizeof(_lib.ResidualNormBwdParams)
+    p = _lib.ResidualNormParams.from_buffer_copy(norms._FWD.pack(*range(1, 19), 0.5, 0.25))
+    assert [getattr(p, f[0]) for f in p._fields_] == [*range(1, 19), 0.5, 0.25]
+    b = _lib.ResidualNormBwdParams.from_buffer_copy(norms._BWD.pack(1, 2) + bytes(p) + norms._BWD_TAIL.pack(*range(3, 14)))
+    assert [getattr(b, f[0]) for f in b._fields_ if f[0] != "fwd"] == [1, 2, *range(3, 14)] and b.fwd.eps == 0.25
+    q = _lib.LinearInt8Params.from_buffer_copy(int8._PARAMS.pack(*range(1, 21)))
+    assert [getattr(q, f[0]) for f in q._fields_] == [*range(1, 21)]
 
 
 def test_gate_rows():
@@ -160,7 +172,7 @@ def test_runs_of_memory_that_overlap():
     assert not _apart([(0, 4), (0, 4)]) and not _apart([(0, 9), (8, 9)])
     writes = [(40, 50), (10, 20)]
     assert _apart(writes, [(0, 10), (20, 40), (50, 60), (25, 35), (5, 8)])
-    for read in [(0, 11), (19, 30), (12, 13), (0, 100), (30, 41), (49, 60), (10, 20)]:
+    for read in [(0, 11), (19, 30), (12, 13), (0, 100), (30, 41), (49, 60), (10, 20), (45, 46)]:
         assert not _apart(writes, [read]), read
 
 
