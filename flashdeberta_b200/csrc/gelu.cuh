@@ -28,30 +28,37 @@ __device__ __forceinline__ uint64_t gelu_erf2(uint64_t v) {
   return ptx::fma_f32x2(av, h, ptx::mul_f32x2(v, both(0.5f)));
 }
 
-// The same for results that are kept in more than bf16, or come from values far below zero: 1/2 erfc(z) = t P(t) e^(-z^2) with
-// t = 1 / (1 + 0.375 z) and P of degree 6 fitted here for the smallest relative error (9.2e-7 over 0 <= z <= 12; 3.4e-6 in fp32 with
-// the exponential's argument rounded), and v Phi(v) = max(v, 0) - |v| 1/2 erfc(|v| / sqrt 2), which loses nothing where Phi(v) is
-// small.  +inf stays, -inf gives zero, NaN stays.
-__device__ __forceinline__ uint64_t gelu_tail2(uint64_t v) {
+// The same where results are kept in more than bf16, or values far below zero count: 1/2 erfc(z) = t P(t) e^(-z^2) with t = 1 / (1 + p z) and
+// P fitted here for the smallest relative error over 0 <= z <= 12, and v Phi(v) = max(v, 0) - |v| 1/2 erfc(|v| / sqrt 2), which loses
+// nothing where Phi(v) is small.  FINE: degree 6, 9.2e-7 (3.4e-6 in fp32 with the exponential's argument rounded).  Else degree 5,
+// 8.9e-6: a fortieth of fp16's half step, and one FMA a pair less.  +inf stays, -inf gives zero, NaN stays.
+template <bool FINE> __device__ __forceinline__ uint64_t gelu_tail2(uint64_t v) {
   auto both = [](float c) { return ptx::pack_f32x2(c, c); };
-  float v0, v1, d0, d1, e0, e1, t0, t1, r, r0, r1;
+  float v0, v1, d0, d1, e0, e1, t0, t1, r0, r1;
   ptx::unpack_f32x2(v, v0, v1);
   const uint64_t a = ptx::pack_f32x2(fminf(fabsf(v0), 1e4f), fminf(fabsf(v1), 1e4f));  // (an infinity times zero would be a NaN)
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r0) : "f"(v0));
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r1) : "f"(v1));
-  ptx::unpack_f32x2(ptx::fma_f32x2(a, both(0.375f * 0.70710678118654752f), both(1.f)), d0, d1);
-  // one reciprocal for both (of at most 2653^2): the special-function unit has the exponentials to do as well
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
-  t0 = r * d1;
-  t1 = r * d0;
+  ptx::unpack_f32x2(ptx::fma_f32x2(a, both((FINE ? 0.375f : 0.65f) * 0.70710678118654752f), both(1.f)), d0, d1);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(d0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(d1));
   ptx::unpack_f32x2(ptx::mul_f32x2(ptx::mul_f32x2(a, both(-0.5f * 1.4426950408889634f)), a), e0, e1);
   const uint64_t e = ptx::pack_f32x2(ptx::ex2(e0), ptx::ex2(e1)), t = ptx::pack_f32x2(t0, t1);
-  uint64_t p = ptx::fma_f32x2(both(0.06661498370203611f), t, both(-0.19073576888425917f));  // -P: what is taken off
-  p = ptx::fma_f32x2(p, t, both(0.06032194842606266f));
-  p = ptx::fma_f32x2(p, t, both(-0.13837509530295133f));
-  p = ptx::fma_f32x2(p, t, both(-0.08452121837156336f));
-  p = ptx::fma_f32x2(p, t, both(-0.10761853239249744f));
-  p = ptx::fma_f32x2(p, t, both(-0.10568661785036586f));
+  uint64_t p;  // -P: what is taken off
+  if constexpr (FINE) {
+    p = ptx::fma_f32x2(both(0.06661498370203611f), t, both(-0.19073576888425917f));
+    p = ptx::fma_f32x2(p, t, both(0.06032194842606266f));
+    p = ptx::fma_f32x2(p, t, both(-0.13837509530295133f));
+    p = ptx::fma_f32x2(p, t, both(-0.08452121837156336f));
+    p = ptx::fma_f32x2(p, t, both(-0.10761853239249744f));
+    p = ptx::fma_f32x2(p, t, both(-0.10568661785036586f));
+  } else {
+    p = ptx::fma_f32x2(both(-0.0718298222776901f), t, both(0.23586562590151855f));
+    p = ptx::fma_f32x2(p, t, both(-0.17785580337148693f));
+    p = ptx::fma_f32x2(p, t, both(-0.1160826767118539f));
+    p = ptx::fma_f32x2(p, t, both(-0.18690448711125093f));
+    p = ptx::fma_f32x2(p, t, both(-0.1831955746192981f));
+  }
   return ptx::fma_f32x2(ptx::mul_f32x2(a, e), ptx::mul_f32x2(p, t), ptx::pack_f32x2(r0, r1));
 }
 

@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "gelu.cuh"
 #include "internal.h"
 #include "launch.h"
@@ -41,13 +43,14 @@ struct Int8Args {
   bool wide;       // rows of the output start on 16 bytes, scales and bias too
 };
 
-constexpr int kTurnWords = 32 * 16;  // of the epilogue's stage, per warp
-
 template <int CG, int BN> struct Tile {
   static constexpr uint32_t kBytesA = kBM * kBK, kBytesW = BN / CG * kBK, kStageBytes = kBytesA + kBytesW;
-  static constexpr int kStages = BN == 64 ? 6 : (BN == 256 ? 6 : (CG == 2 ? 8 : 6));
-  static constexpr int kEpiWarps = BN == 64 ? 8 : 16, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-  static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemBars = kSmemTurn + kEpiWarps * kTurnWords * 4;
+  static constexpr int kStages = BN == 256 ? 5 : (CG == 2 ? 7 : (BN == 128 ? 5 : 6));
+  // the epilogue: columns of a warp; bytes of a row that one store takes, 32 rows of them in shared memory; scales and biases
+  static constexpr int kCols = BN == 256 ? 64 : 32, kEpiWarps = BN * 4 / kCols, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+  static constexpr int kStoreBytes = 64;
+  static constexpr uint32_t kTurnBytes = 32 * kStoreBytes, kColBytes = 2 * kCols * 4;
+  static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemCols = kSmemTurn + kEpiWarps * kTurnBytes, kSmemBars = kSmemCols + kEpiWarps * kColBytes;
   enum : uint32_t { kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2, kNumBars = 2 * kStages + 4 };
   static constexpr uint32_t kSmemBytes = kSmemBars + 8 * kNumBars + 16 + 1024;  // + tensor-memory slot, abort flag, alignment slack
   static constexpr uint32_t kTmemCols = 2 * BN;
@@ -60,23 +63,10 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, floa
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A pair of 32-bit integers as floats, each rounded once.  The conversion instruction goes through the special-function unit (16 a
-// clock and SM), where the GELU's exponentials queue; MAGIC takes the upper and the lower half of the integer (its sign bit
-// flipped) as the mantissas of 2^23 + half and puts them together in one FMA, whose rounding is the only one.
-template <bool MAGIC> __device__ __forceinline__ uint64_t float_pair(uint32_t a0, uint32_t a1) {
-  if constexpr (!MAGIC) return pack_f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1));
-  a0 ^= 0x80000000u;
-  a1 ^= 0x80000000u;
-  const uint64_t hi = pack_f32x2(__uint_as_float(__byte_perm(a0, 0x4B00u, 0x5432)), __uint_as_float(__byte_perm(a1, 0x4B00u, 0x5432)));
-  const uint64_t lo = pack_f32x2(__uint_as_float(__byte_perm(a0, 0x4B00u, 0x5410)), __uint_as_float(__byte_perm(a1, 0x4B00u, 0x5410)));
-  const float off_hi = -(8388608.f + 32768.f), off_lo = -8388608.f;
-  return fma_f32x2(add_f32x2(hi, pack_f32x2(off_hi, off_hi)), pack_f32x2(65536.f, 65536.f), add_f32x2(lo, pack_f32x2(off_lo, off_lo)));
-}
-
 // A pair of columns: the sums scaled, bias added, activation.
-template <bool GELU, bool MAGIC> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
-  const uint64_t v = fma_f32x2(mul_f32x2(float_pair<MAGIC>(a0, a1), w_scale), x_scale, bias);
-  return GELU ? gelu_tail2(v) : v;
+template <bool GELU, bool FINE> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
+  const uint64_t v = fma_f32x2(mul_f32x2(pack_f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1)), w_scale), x_scale, bias);
+  return GELU ? gelu_tail2<FINE>(v) : v;
 }
 
 template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a, int n) {
@@ -84,75 +74,39 @@ template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a
   return a.bias_fp32 ? __ldg(static_cast<const float*>(a.bias) + n) : to_float<T>(static_cast<const T*>(a.bias)[n]);
 }
 
-// 32 columns of 32 rows per warp, each thread its own row: through 64 bytes of shared memory per row and a TMA store per 64 bytes of
-// columns, which leaves out what lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 54 at
-// 16384 x 1024 -> 4096.)  Column piece p (16 bytes) of row r lies at piece p ^ (r / 2 % 4), the map's swizzle: no bank conflicts.
-template <typename T, bool GELU>
-__device__ __forceinline__ void store_tile(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, uint32_t* stage, int lane) {
-  const uint64_t sx = pack_f32x2(x_scale, x_scale);
-  constexpr int kCols = 64 / sizeof(T);  // of one store
+// 32 rows of `kStore` columns per warp, each thread its own row, into shared memory and from there by a TMA store, which leaves out what
+// lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 66 at 16384 x 1024 -> 4096.)  Piece p (16 bytes) of
+// row r lies at piece p ^ (r % 8) (128-byte rows) or p ^ (r / 2 % 4) (64-byte rows), the map's swizzle: no bank conflicts.
+// `cols`: the warp's scales, and its biases behind them, in shared memory.
+template <typename T, bool GELU, int BYTES, int COLS>
+__device__ __forceinline__ void convert_piece(const uint32_t* acc, int count, int c0, uint64_t sx, const float* cols, uint32_t* stage, int lane, int col_in_stage) {
 #pragma unroll
-  for (int part = 0; part < 32; part += kCols) {
-    uint32_t o[16];
+  for (int c = 0; c < 32; c += 16 / int(sizeof(T))) {  // a piece of 16 bytes at a time
+    if (c >= count) break;
+    uint32_t o[4];
 #pragma unroll
-    for (int c = part; c < part + kCols; c += 8) {
-      float ws[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      const bool full = n0 + c + 8 <= a.n;  // (else n is no multiple of 8: single columns)
-      if (full) {
-        *reinterpret_cast<float4*>(ws) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c));
-        *reinterpret_cast<float4*>(ws + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale + n0 + c + 4));
-        if (a.bias != nullptr) {
-          if (a.bias_fp32) {
-            *reinterpret_cast<float4*>(b) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c));
-            *reinterpret_cast<float4*>(b + 4) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + n0 + c + 4));
-          } else if constexpr (sizeof(T) == 2) {
-            RowWords<T> r;
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + n0 + c));
-            r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
-            unpack(r, b);
-          }
-        }
+    for (int e = 0; e < 16 / int(sizeof(T)); e += 4) {
+      const float4 ws = *reinterpret_cast<const float4*>(cols + c0 + c + e), b = *reinterpret_cast<const float4*>(cols + COLS + c0 + c + e);
+      float v0, v1, v2, v3;
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + e], acc[c + e + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + e + 2], acc[c + e + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
+      if constexpr (sizeof(T) == 4) {
+        o[0] = __float_as_uint(v0); o[1] = __float_as_uint(v1); o[2] = __float_as_uint(v2); o[3] = __float_as_uint(v3);
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ws[e] = n0 + c + e < a.n ? __ldg(a.w_scale + n0 + c + e) : 0.f;
-          if (n0 + c + e < a.n) b[e] = bias_at<T>(a, n0 + c + e);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        float v0, v1;
-        // (half of the integers either way: neither the special-function unit nor the issue slots are full then)
-        const uint64_t ws2 = pack_f32x2(ws[e], ws[e + 1]), b2 = pack_f32x2(b[e], b[e + 1]);
-        unpack_f32x2(e % 4 == 0 ? finish_pair<GELU, GELU>(acc[c + e], acc[c + e + 1], ws2, sx, b2) : finish_pair<GELU, false>(acc[c + e], acc[c + e + 1], ws2, sx, b2),
-                     v0, v1);
-        if constexpr (sizeof(T) == 4) {
-          o[c - part + e] = __float_as_uint(v0);
-          o[c - part + e + 1] = __float_as_uint(v1);
-        } else {
-          o[(c - part + e) >> 1] = pack_pair<T>(v0, v1);
-        }
+        o[e >> 1] = pack_pair<T>(v0, v1);
+        o[(e >> 1) + 1] = pack_pair<T>(v2, v3);
       }
     }
-    tma_store_wait_read();  // the store before has left the stage (each lane waits for its own, and there is one that issues)
-    __syncwarp();
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-      *reinterpret_cast<uint4*>(stage + lane * 16 + 4 * (p ^ ((lane >> 1) & 3))) = make_uint4(o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0 && n0 + part < a.n) {
-      tma_store_2d(&a.tm_out, smem_u32(stage), n0 + part, (int)row0);
-      tma_store_commit();
-    }
+    const int piece = (col_in_stage + c) * int(sizeof(T)) / 16, at = BYTES == 128 ? piece ^ (lane & 7) : piece ^ ((lane >> 1) & 3);
+    *reinterpret_cast<uint4*>(stage + lane * (BYTES / 4) + 4 * at) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-// The same where a row starts anywhere or columns are missing: through shared memory, two rows of 16 columns at a time across the
-// lanes.  (A thread writing its own row element by element would touch 32 sectors with every store.)  Column c of row r lies in word
+// The same where a row starts anywhere: 32 columns, turned in shared memory, two rows of 16 columns at a time across the lanes.  (A
+// thread writing its own row element by element would touch 32 sectors with every store.)  Column c of row r lies in word
 // 16 r + (c ^ (r / 2 % 16)): neither side of the turn has two lanes on one bank.
-template <typename T, bool GELU>
-__device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, uint32_t* turn, int lane) {
+template <typename T, bool GELU, int COLS>
+__device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, const float* cols, uint32_t* turn, int lane) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -160,7 +114,7 @@ __device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (
     __syncwarp();
     const int c = lane & 15, up = lane >> 4, n = n0 + half * 16 + c;
     const bool has = n < a.n;
-    const float ws = has ? __ldg(a.w_scale + n) : 0.f, b = has ? bias_at<T>(a, n) : 0.f;
+    const float ws = cols[half * 16 + c], b = cols[COLS + half * 16 + c];
     const uint64_t ws2 = pack_f32x2(ws, ws), b2 = pack_f32x2(b, b);
     T* out = static_cast<T*>(a.out) + row0 * a.n + n;
 #pragma unroll 4
@@ -168,7 +122,7 @@ __device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (
       const int r0 = r + up, r1 = r + 2 + up;
       const float s0 = __shfl_sync(0xffffffffu, x_scale, r0), s1 = __shfl_sync(0xffffffffu, x_scale, r1);
       float v0, v1;
-      unpack_f32x2(finish_pair<GELU, false>(turn[r0 * 16 + (c ^ ((r0 >> 1) & 15))], turn[r1 * 16 + (c ^ ((r1 >> 1) & 15))], ws2, pack_f32x2(s0, s1), b2), v0, v1);
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(turn[r0 * 16 + (c ^ ((r0 >> 1) & 15))], turn[r1 * 16 + (c ^ ((r1 >> 1) & 15))], ws2, pack_f32x2(s0, s1), b2), v0, v1);
       if (has && row0 + r0 < a.rows) out[(int64_t)r0 * a.n] = from_float<T>(v0);
       if (has && row0 + r1 < a.rows) out[(int64_t)r1 * a.n] = from_float<T>(v1);
     }
@@ -284,41 +238,89 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
     }
   } else {
     const int quarter = warp & 3;                // the 32 tensor-memory lanes this warp may read
-    constexpr int kCols = BN * 4 / T::kEpiWarps, kChunks = kCols / 32;  // this warp's columns of the tile; 32 at a time
-    const int part = (warp - kEpiWarp0) >> 2;
+    const int mine = warp - kEpiWarp0, part = mine >> 2;
+    constexpr int kCols = T::kCols, kStore = T::kStoreBytes / int(sizeof(OUT)), kLoad = kStore < 32 ? kStore : 32;
     const uint32_t tmem_lane = tmem_base + (uint32_t(quarter * 32) << 16);
-    uint32_t* turn = reinterpret_cast<uint32_t*>(smem_gen + T::kSmemTurn) + (warp - kEpiWarp0) * kTurnWords;
+    uint32_t* turn = reinterpret_cast<uint32_t*>(smem_gen + T::kSmemTurn + mine * T::kTurnBytes);
+    float* cols = reinterpret_cast<float*>(smem_gen + T::kSmemCols + mine * T::kColBytes);
     uint32_t acc_empty[2] = {bar(T::kBarAccEmpty), bar(T::kBarAccEmpty + 1)};
     if constexpr (CG == 2) { acc_empty[0] = map_to_rank(acc_empty[0], 0); acc_empty[1] = map_to_rank(acc_empty[1], 0); }
     uint32_t local = 0;
+    // scales and biases of a tile's columns, a column (or two) per lane: fetched a tile ahead, put into shared memory when their turn comes
+    float ws[kCols / 32], b[kCols / 32], x_scale = 0.f;
+    auto fetch = [&](int tile) {
+      const int64_t row = (int64_t)(tile / args.tiles_n) * (kBM * CG) + int(rank) * kBM + quarter * 32 + lane;
+      const int n0 = (tile % args.tiles_n) * BN + part * kCols + lane;
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        const bool has = tile < num_tiles && n0 + i * 32 < args.n;
+        ws[i] = has ? __ldg(args.w_scale + n0 + i * 32) : 0.f;
+        b[i] = has ? bias_at<OUT>(args, n0 + i * 32) : 0.f;
+      }
+      x_scale = tile < num_tiles && row < args.rows ? __ldg(args.x_scale + row) : 0.f;
+    };
+    fetch(first);
 #pragma unroll 1
     for (int tile = first; tile < num_tiles; tile += step, ++local) {
       const int64_t row0 = (int64_t)(tile / args.tiles_n) * (kBM * CG) + int(rank) * kBM + quarter * 32;
       const int n0 = (tile % args.tiles_n) * BN + part * kCols;
       const uint32_t acc = local & 1u;
-      const float x_scale = row0 + lane < args.rows ? __ldg(args.x_scale + row0 + lane) : 0.f;
+      const float xs = x_scale;
+      const uint64_t sx = pack_f32x2(xs, xs);
+      __syncwarp();  // (the tile before has been read from here)
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        cols[i * 32 + lane] = ws[i];
+        cols[kCols + i * 32 + lane] = b[i];
+      }
+      __syncwarp();
+      fetch(tile + step);
       wait(bar(T::kBarAccFull + acc), (local >> 1) & 1u);
       tc_fence_after();
+      const bool has_rows = ok && row0 < args.rows;
 #pragma unroll 1
-      for (int ch = 0; ch < kChunks; ++ch) {
-        uint32_t a[32];
-        if (ok) {  // whole warps execute the load, whatever their rows
-          tmem_ld32(tmem_lane + acc * BN + uint32_t(part * kCols + ch * 32), a);
-          tmem_wait_ld();
+      for (int at = 0; at < kCols; at += kStore > 32 ? kStore : 32) {  // a store's columns (or two stores'), 32 of tensor memory at a time
+        constexpr int kStep = kStore > 32 ? kStore : 32;
+#pragma unroll
+        for (int c0 = 0; c0 < kStep; c0 += 32) {
+          uint32_t a[32];
+          if (ok) {  // whole warps execute the load, whatever their rows
+            tmem_ld32(tmem_lane + acc * BN + uint32_t(part * kCols + at + c0), a);
+            tmem_wait_ld();
+          }
+          if (at + c0 + 32 == kCols) {  // the accumulator is in registers: the next tile but one may overwrite it
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) { if constexpr (CG == 2) mbar_arrive_peer(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
+          }
+          const int n = n0 + at + c0;
+          if (!has_rows || n >= args.n) continue;
+          if (!args.wide) {
+            store_turned<OUT, GELU, kCols>(args, a, row0, n, xs, cols + at + c0, turn, lane);
+            continue;
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += kLoad) {
+            const bool begins = (c0 + c) % kStore == 0, ends = (c0 + c + kLoad) % kStore == 0;
+            if (begins) {
+              tma_store_wait_read();  // the store before has left the stage (the lane that issues them waits)
+              __syncwarp();
+            }
+            convert_piece<OUT, GELU, T::kStoreBytes, kCols>(a + c, kLoad, at + c0 + c, sx, cols, turn, lane, (c0 + c) % kStore);
+            if (ends || n + c + kLoad >= args.n) {  // (the last columns there are end a store early)
+              fence_proxy_async();
+              __syncwarp();
+              const int n_store = n0 + at + (c0 + c) / kStore * kStore;
+              if (lane == 0 && n_store < args.n) {
+                tma_store_2d(&args.tm_out, smem_u32(turn), n_store, (int)row0);
+                tma_store_commit();
+              }
+            }
+          }
         }
-        if (ch == kChunks - 1) {  // the accumulator is in registers: the next tile but one may overwrite it
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) { if constexpr (CG == 2) mbar_arrive_cluster(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
-        }
-        const int n = n0 + ch * 32;
-        if (!ok || n >= args.n || row0 >= args.rows) continue;
-        if (args.wide) store_tile<OUT, GELU>(args, a, row0, n, x_scale, turn, lane);
-        else store_turned<OUT, GELU>(args, a, row0, n, x_scale, turn, lane);
       }
     }
   }
-
   if (warp >= kEpiWarp0 && lane == 0) tma_store_wait();
 
   // ---- teardown ----
@@ -355,9 +357,11 @@ int launch_type(const Int8Args& a, int grid, int out_dtype, bool gelu, bool chai
 #undef FDB_INT8_OUT
 }
 
-// Tile shapes, with clocks per 128 of K and clocks a launch adds on top, as in linear_sm100.cu.
-struct Config { int cg, bn, clocks, extra; };
-constexpr Config kConfigs[] = {{2, 256, 540, 2600}, {2, 128, 300, 1600}, {1, 128, 340, 1500}, {1, 64, 350, 600}};
+// Tile shapes: clocks per 128 of K and clocks of a tile's epilogue (with the GELU 1.8 times those), as measured over whole waves
+// (16384 x 4096 -> 4096: 168, 194, 259, 391 us; 16384 x 256 -> 4096: 36, 41, 40, 54).  One runs beside the other but for the first
+// tile's main loop and the last one's epilogue.
+struct Config { int cg, bn, clocks, epilogue; };
+constexpr Config kConfigs[] = {{2, 256, 680, 4800}, {2, 128, 430, 2700}, {1, 128, 535, 2650}, {1, 64, 403, 1800}};
 
 bool float_type(int t) { return t == FDB_BF16 || t == FDB_FP16 || t == FDB_FP32; }
 unsigned type_bytes(int t) { return t == FDB_FP32 ? 4u : 2u; }
@@ -425,7 +429,8 @@ extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* st
   for (const Config& f : kConfigs) {
     const int64_t tiles = (p->rows + kBM * f.cg - 1) / (kBM * f.cg) * ((p->out_features + f.bn - 1) / f.bn);
     const int64_t units = sms / f.cg, waves = (tiles + units - 1) / units;
-    const int64_t cost = waves * ((int64_t)((p->in_features + kBK - 1) / kBK) * f.clocks) + f.extra;
+    const int64_t loop = (int64_t)((p->in_features + kBK - 1) / kBK) * f.clocks, epilogue = p->gelu != 0 ? f.epilogue * 9 / 5 : f.epilogue;
+    const int64_t cost = waves * std::max(loop, epilogue) + std::min(loop, epilogue);
     if (best == nullptr || cost < best_cost) { best = &f; best_cost = cost; best_tiles = tiles; }
   }
   if (best_tiles * 2 > 2147483647LL) return fail(FDB_ERR_LIMIT, "linear_int8: %lld rows x %d features", (long long)p->rows, p->out_features);
@@ -441,7 +446,7 @@ extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* st
   if (a.wide) {
     const CUtensorMapDataType type = p->out_dtype == FDB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                               : (p->out_dtype == FDB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
-    rc = make_map_out(&a.tm_out, p->out, p->rows, p->out_features, type, (int)type_bytes(p->out_dtype), 32, "out");
+    rc = make_map_out(&a.tm_out, p->out, p->rows, p->out_features, type, (int)type_bytes(p->out_dtype), 64, 32, "out");
     if (rc != FDB_OK) return rc;
   }
   const int units = sms / best->cg;
