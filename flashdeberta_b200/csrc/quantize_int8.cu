@@ -24,15 +24,43 @@ struct QuantArgs {
   int cols, team_threads, teams;
 };
 
+// Largest magnitude of a thread's elements, as bits of T's absolute values; and such bits as fp32.
+template <int V> __device__ __forceinline__ uint32_t top_of(const RowWords<float, V>& r) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < V * kRowElems; ++j) top = max(top, r.w[j] & 0x7fffffffu);
+  return top;
+}
+template <typename T, int V> __device__ __forceinline__ uint32_t top_of(const RowWords<T, V>& r) {  // two at a time
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < V * kRowElems / 2; ++j) top = __vmaxu2(top, r.w[j] & 0x7fff7fffu);
+  return max(top & 0xffffu, top >> 16);
+}
+template <typename T> __device__ __forceinline__ float bits_to_float(uint32_t b) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(b);
+  const unsigned short h = (unsigned short)b;
+  return to_float<T>(*reinterpret_cast<const T*>(&h));
+}
+
+// Four products with the reciprocal scale, each rounded to fp32 and then to a whole number, as bytes: 1.5 * 2^23 added, the number is in
+// the lowest bits.  (float-to-int conversions run at a quarter of the rate.)
+__device__ __forceinline__ uint32_t four_bytes(const float* v, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], inv), 12582912.f));  // (as one FMA the product would not be rounded)
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
 template <typename T, bool WIDE, int V>
 __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
   constexpr int kElems = V * kRowElems;
-  __shared__ uint32_t s_top[kThreads / 32][2][8];
+  __shared__ uint32_t s_top[kThreads / 32][8];
   const int team = threadIdx.x / a.team_threads, t = threadIdx.x - team * a.team_threads;
   const int warps = a.team_threads / 32, span = a.team_threads * kElems;
   ptx::grid_launch();
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * a.teams + team; row < a.rows; row += (int64_t)gridDim.x * a.teams) {
+  const int64_t row = (int64_t)blockIdx.x * a.teams + team;
+  if (row < a.rows) {
     const T* x = static_cast<const T*>(a.x) + row * a.cols;
     uint32_t top = 0;
     RowWords<T, V> first;
@@ -41,45 +69,40 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
       const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
       RowWords<T, V> r;
       cols.load(x + at, r);
-      unpack(r, v);
-#pragma unroll
-      for (int j = 0; j < kElems; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      top = max(top, top_of(r));
       if (at == 0) first = r;
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (warps > 1) {
-      uint32_t* s = s_top[team][turn];
-      turn ^= 1;
+      uint32_t* s = s_top[team];
       if ((threadIdx.x & 31) == 0) s[t >> 5] = top;
       ptx::bar_sync((uint32_t)team + 1, (uint32_t)a.team_threads);
       for (int w = 0; w < warps; ++w) top = max(top, s[w]);
     }
-    const float amax = __uint_as_float(top);
+    const float amax = bits_to_float<T>(top);
     const bool zero = amax < 7.888609052e-31f;                       // 2^-100: the reciprocal would leave fp32's range
-    const float inv = zero || top >= 0x7f800000u ? 0.f : 127.f / amax;
+    const bool finite = amax <= 3.402823466e+38f;
+    const float inv = zero || !finite ? 0.f : 127.f / amax;
     if (t == 0) a.scale[row] = zero ? 0.f : amax / 127.f;
     for (int at = 0; at < a.cols; at += span) {
       const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
       RowWords<T, V> r = first;
       if (at != 0) cols.load(x + at, r);
       unpack(r, v);
-      int q[kElems];
+      if (!finite)
 #pragma unroll
-      for (int j = 0; j < kElems; ++j) q[j] = inv == 0.f ? 0 : __float2int_rn(v[j] * inv);
+        for (int j = 0; j < kElems; ++j) v[j] = 0.f;  // (an infinity times zero is a NaN)
       uint8_t* y = a.y + row * a.pitch + at;
-      if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int* p = q + i * kRowElems;
-          uint2 o;
-          o.x = (p[0] & 255) | (p[1] & 255) << 8 | (p[2] & 255) << 16 | p[3] << 24;
-          o.y = (p[4] & 255) | (p[5] & 255) << 8 | (p[6] & 255) << 16 | p[7] << 24;
-          if (cols.live(i * kRowElems)) *reinterpret_cast<uint2*>(y + cols.col(i * kRowElems)) = o;
+      for (int j = 0; j < kElems; j += kRowElems) {
+        const uint2 o = make_uint2(four_bytes(v + j, inv), four_bytes(v + j + 4, inv));
+        if constexpr (WIDE) {
+          if (cols.live(j)) *reinterpret_cast<uint2*>(y + cols.col(j)) = o;
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRowElems; ++i)
+            if (cols.live(j + i)) y[cols.col(j + i)] = (uint8_t)((i < 4 ? o.x : o.y) >> (8 * (i % 4)));
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kElems; ++j)
-          if (cols.live(j)) y[cols.col(j)] = (uint8_t)q[j];
       }
     }
   }
@@ -88,8 +111,7 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
 template <typename T, bool WIDE>
 cudaError_t launch(const QuantArgs& a, int v, cudaStream_t s) {
   const int threads = a.teams * a.team_threads;
-  const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (2048 / threads);
-  const unsigned grid = (unsigned)std::min(want, most);
+  const unsigned grid = (unsigned)((a.rows + a.teams - 1) / a.teams);
   if (v == 1) quantize_int8_kernel<T, WIDE, 1><<<grid, threads, 0, s>>>(a);
   else if (v == 2) quantize_int8_kernel<T, WIDE, 2><<<grid, threads, 0, s>>>(a);
   else if (v == 3) quantize_int8_kernel<T, WIDE, 3><<<grid, threads, 0, s>>>(a);
@@ -121,6 +143,7 @@ extern "C" FDB_API int fdb_quantize_int8(const void* x, int32_t dtype, int64_t r
                                          void* stream) {
   clear_error();
   if (dtype != FDB_BF16 && dtype != FDB_FP16 && dtype != FDB_FP32) return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: dtype %d", dtype);
+  if (rows > 2147483647LL) return fail(FDB_ERR_LIMIT, "quantize_int8: %lld rows", (long long)rows);
   if (rows < 0 || cols <= 0 || pitch < cols)
     return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: rows %lld, cols %d, pitch %lld", (long long)rows, cols, (long long)pitch);
   if (rows == 0) return FDB_OK;

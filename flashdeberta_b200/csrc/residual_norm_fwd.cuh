@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(ONE ? kNormFwdThreads : 256, ONE ? 5 : 2) resi
     for (int j = 0; j < kElems; ++j) v[j] += p[j];
   };
 
-  for (int64_t row = (int64_t)blockIdx.x * a.teams + team; row < a.rows; row += (int64_t)gridDim.x * a.teams) {
+  const int64_t row = (int64_t)blockIdx.x * a.teams + team;
+  if (row < a.rows) {
     const int64_t at = row * a.hidden;
     RowWords<T, V> rx, rr;
     cols.load(x + at, rx);
@@ -95,8 +96,7 @@ __global__ void __launch_bounds__(ONE ? kNormFwdThreads : 256, ONE ? 5 : 2) resi
 template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>
 int norm_fwd_launch_kernel(const ResidualNormArgs& a, cudaStream_t s) {
   const int threads = a.teams * a.team_threads;
-  const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (2048 / threads);
-  residual_norm_kernel<T, RMS, POST, WIDE, V, ONE><<<(unsigned)std::min(want, most), (unsigned)threads, 0, s>>>(a);
+  residual_norm_kernel<T, RMS, POST, WIDE, V, ONE><<<(unsigned)((a.rows + a.teams - 1) / a.teams), (unsigned)threads, 0, s>>>(a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm launch: %s", cudaGetErrorString(e));
   return FDB_OK;
