@@ -9,6 +9,10 @@
 
 namespace fdb {
 
+using ptx::add_f32x2;
+using ptx::fma_f32x2;
+using ptx::mul_f32x2;
+
 constexpr int kNormBwdTeams = kNormBwdThreads / 32;
 constexpr size_t kNormBwdPlainSmem = 40 * 1024;  // with the 8 KB of the teams' sums, what a launch may take without being asked
 
@@ -22,6 +26,7 @@ inline size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode
 
 template <typename T, bool RMS, bool POST, int GATE, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormBwdArgs b) {
+  constexpr int kPairs = kRowElems / 2;
   constexpr int kSums = RMS ? 1 : 2;  // per norm and row; and vectors of sums over rows: weight, bias
   extern __shared__ __align__(16) float s_vectors[];
   __shared__ __align__(16) float s_sums[kNormBwdTeams][TeamSum<kSums>::kSlots];
@@ -61,9 +66,9 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     vector_at(v)[0] = make_float4(q[0], q[1], q[2], q[3]);
     vector_at(v)[f.team_threads] = make_float4(q[4], q[5], q[6], q[7]);
   };
-  auto get_vector = [&](int v, float (&q)[kRowElems]) {
-    const float4 lo = vector_at(v)[0], hi = vector_at(v)[f.team_threads];
-    q[0] = lo.x; q[1] = lo.y; q[2] = lo.z; q[3] = lo.w; q[4] = hi.x; q[5] = hi.y; q[6] = hi.z; q[7] = hi.w;
+  auto get_vector = [&](int v, uint64_t (&q)[kPairs]) {
+    const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(vector_at(v)), hi = *reinterpret_cast<const ulonglong2*>(vector_at(v) + f.team_threads);
+    q[0] = lo.x; q[1] = lo.y; q[2] = hi.x; q[3] = hi.y;
   };
   if (team == 0) {
     put_vector(kWeight, f.weight, f.param_fp32);
@@ -81,28 +86,32 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
   for (int i = threadIdx.x; i < int(sizeof(s_sums) / sizeof(float)); i += blockDim.x) s_sums[0][i] = 0.f;
   __syncthreads();
 
-  float sum_w[kRowElems], sum_b[kRowElems], sum_A[kRowElems], sum_B[kRowElems];
+  uint64_t sum_w[kPairs], sum_b[kPairs], sum_A[kPairs], sum_B[kPairs];
 #pragma unroll
-  for (int j = 0; j < kRowElems; ++j) sum_w[j] = sum_b[j] = sum_A[j] = sum_B[j] = 0.f;
+  for (int j = 0; j < kPairs; ++j) sum_w[j] = sum_b[j] = sum_A[j] = sum_B[j] = both(0.f);
+  uint64_t* s_C2 = reinterpret_cast<uint64_t*>(s_C);
+  uint64_t* s_D2 = reinterpret_cast<uint64_t*>(s_D);
   // A and B of a group leave the registers
-  auto leave_group = [&](int64_t group, const float (&gate)[kRowElems]) {
+  auto leave_group = [&](int64_t group, const uint64_t (&gate)[kPairs]) {
     float* slot = b.slots + (worker + group) * 2 * f.hidden;
     cols.store(slot, sum_A);
     if constexpr (!RMS) cols.store(slot + f.hidden, sum_B);
 #pragma unroll
-    for (int j = 0; j < kRowElems; ++j) {
+    for (int j = 0; j < kPairs; ++j) {
       if constexpr (POST) {
-        s_C[j] = fmaf(gate[j], sum_A[j], s_C[j]);
-        if constexpr (!RMS) s_D[j] = fmaf(gate[j], sum_B[j], s_D[j]);
+        s_C2[j] = fma_f32x2(gate[j], sum_A[j], s_C2[j]);
+        if constexpr (!RMS) s_D2[j] = fma_f32x2(gate[j], sum_B[j], s_D2[j]);
       }
-      sum_A[j] = sum_B[j] = 0.f;
+      sum_A[j] = sum_B[j] = both(0.f);
     }
   };
 
   int64_t group = -1;
-  float g[kRowElems];
+  uint64_t g[kPairs];
 #pragma unroll
-  for (int j = 0; j < kRowElems; ++j) g[j] = 1.f;
+  for (int j = 0; j < kPairs; ++j) g[j] = both(1.f);
+  const uint64_t scale = both(f.residual_scale);
+#pragma unroll 2
   for (int64_t row = first; row < end; ++row) {
     if (row + 1 < end) fetch(row + 1, next);
     const int64_t at = row * f.hidden;
@@ -121,98 +130,109 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     }
 
     // the stream again; hat: x normalised (x itself without the norm), z: the stream normalised
-    float hat[kRowElems], u[kRowElems], z[kRowElems], d[kRowElems], p[kRowElems];
+    uint64_t hat[kPairs], u[kPairs], z[kPairs], d[kPairs], p[kPairs];
     unpack(now.x, hat);
     if constexpr (POST) {
+      const uint64_t mean = both(-now.stats.x), inv = both(now.stats.y);
       get_vector(kPostWeight, p);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) {
-        hat[j] = (RMS ? hat[j] : hat[j] - now.stats.x) * now.stats.y;
-        u[j] = hat[j] * p[j];
+      for (int j = 0; j < kPairs; ++j) {
+        hat[j] = mul_f32x2(RMS ? hat[j] : add_f32x2(hat[j], mean), inv);
+        u[j] = mul_f32x2(hat[j], p[j]);
       }
       if constexpr (!RMS) {
         get_vector(kPostBias, p);
 #pragma unroll
-        for (int j = 0; j < kRowElems; ++j) u[j] += p[j];
+        for (int j = 0; j < kPairs; ++j) u[j] = add_f32x2(u[j], p[j]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) u[j] = hat[j];
+      for (int j = 0; j < kPairs; ++j) u[j] = hat[j];
     }
 #pragma unroll
-    for (int j = 0; j < kRowElems; ++j) z[j] = g[j] * u[j];
+    for (int j = 0; j < kPairs; ++j) z[j] = mul_f32x2(g[j], u[j]);
     if (f.residual != nullptr) {
       unpack(now.residual, p);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) z[j] = fmaf(f.residual_scale, p[j], z[j]);
+      for (int j = 0; j < kPairs; ++j) z[j] = fma_f32x2(scale, p[j], z[j]);
     }
+    {
+      const uint64_t mean = both(-now.stats.z), inv = both(now.stats.w);
 #pragma unroll
-    for (int j = 0; j < kRowElems; ++j) z[j] = (RMS ? z[j] : z[j] - now.stats.z) * now.stats.w;
+      for (int j = 0; j < kPairs; ++j) z[j] = mul_f32x2(RMS ? z[j] : add_f32x2(z[j], mean), inv);
+    }
 
     // dz, the gradient of the stream in all
     float sums[kSums];
-    for (float& v : sums) v = 0.f;
     if (b.dnormed != nullptr) {
+      uint64_t s0 = both(0.f), s1 = both(0.f);
       unpack(now.dnormed, d);
       get_vector(kWeight, p);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) {
-        sum_w[j] = fmaf(d[j], z[j], sum_w[j]);
-        if constexpr (!RMS) sum_b[j] += d[j];
-        d[j] *= p[j];
-        sums[0] = fmaf(d[j], z[j], sums[0]);
-        if constexpr (!RMS) sums[kSums - 1] += d[j];
+      for (int j = 0; j < kPairs; ++j) {
+        sum_w[j] = fma_f32x2(d[j], z[j], sum_w[j]);
+        if constexpr (!RMS) sum_b[j] = add_f32x2(sum_b[j], d[j]);
+        d[j] = mul_f32x2(d[j], p[j]);
+        s0 = fma_f32x2(d[j], z[j], s0);
+        if constexpr (!RMS) s1 = add_f32x2(s1, d[j]);
       }
+      sums[kSums - 1] = fold(s1);
+      sums[0] = fold(s0);
       team_sum(sums);
-      for (float& v : sums) v *= inv_hidden;
+      // inv (y - mean(y) - z mean(y z)), the means scaled first
+      const float scaled = now.stats.w * inv_hidden;
+      const uint64_t inv = both(now.stats.w), m0 = both(-scaled * sums[0]), m1 = both(RMS ? 0.f : -scaled * sums[kSums - 1]);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.w * (d[j] - fmaf(z[j], sums[0], RMS ? 0.f : sums[kSums - 1]));
+      for (int j = 0; j < kPairs; ++j) d[j] = fma_f32x2(d[j], inv, RMS ? mul_f32x2(z[j], m0) : fma_f32x2(z[j], m0, m1));
     } else {
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] = 0.f;
+      for (int j = 0; j < kPairs; ++j) d[j] = both(0.f);
     }
     if (b.dstream != nullptr) {
       unpack(now.dstream, p);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] += p[j];
+      for (int j = 0; j < kPairs; ++j) d[j] = add_f32x2(d[j], p[j]);
     }
     if (b.dresidual != nullptr) {
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) p[j] = f.residual_scale * d[j];
+      for (int j = 0; j < kPairs; ++j) p[j] = mul_f32x2(scale, d[j]);
       cols.store(static_cast<T*>(b.dresidual) + at, p);
     }
     if constexpr (GATE == kGateElement) {
       if (b.dgate != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kRowElems; ++j) p[j] = d[j] * u[j];
+        for (int j = 0; j < kPairs; ++j) p[j] = mul_f32x2(d[j], u[j]);
         if (f.gate_fp32) cols.store(static_cast<float*>(b.dgate) + at, p);
         else cols.store(static_cast<T*>(b.dgate) + at, p);
       }
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] *= g[j];
+      for (int j = 0; j < kPairs; ++j) d[j] = mul_f32x2(d[j], g[j]);
     }
 #pragma unroll
-    for (int j = 0; j < kRowElems; ++j) {
-      sum_A[j] = fmaf(d[j], hat[j], sum_A[j]);
-      if constexpr (!RMS) sum_B[j] += d[j];
+    for (int j = 0; j < kPairs; ++j) {
+      sum_A[j] = fma_f32x2(d[j], hat[j], sum_A[j]);
+      if constexpr (!RMS) sum_B[j] = add_f32x2(sum_B[j], d[j]);
     }
     if constexpr (GATE != kGateElement) {
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] *= g[j];
+      for (int j = 0; j < kPairs; ++j) d[j] = mul_f32x2(d[j], g[j]);
     }
     if constexpr (POST) {
+      uint64_t s0 = both(0.f), s1 = both(0.f);
       get_vector(kPostWeight, p);
-      for (float& v : sums) v = 0.f;
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) {
-        d[j] *= p[j];
-        sums[0] = fmaf(d[j], hat[j], sums[0]);
-        if constexpr (!RMS) sums[kSums - 1] += d[j];
+      for (int j = 0; j < kPairs; ++j) {
+        d[j] = mul_f32x2(d[j], p[j]);
+        s0 = fma_f32x2(d[j], hat[j], s0);
+        if constexpr (!RMS) s1 = add_f32x2(s1, d[j]);
       }
+      sums[kSums - 1] = fold(s1);
+      sums[0] = fold(s0);
       team_sum(sums);
-      for (float& v : sums) v *= inv_hidden;
+      const float scaled = now.stats.y * inv_hidden;
+      const uint64_t inv = both(now.stats.y), m0 = both(-scaled * sums[0]), m1 = both(RMS ? 0.f : -scaled * sums[kSums - 1]);
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) d[j] = now.stats.y * (d[j] - fmaf(hat[j], sums[0], RMS ? 0.f : sums[kSums - 1]));
+      for (int j = 0; j < kPairs; ++j) d[j] = fma_f32x2(d[j], inv, RMS ? mul_f32x2(hat[j], m0) : fma_f32x2(hat[j], m0, m1));
     }
     cols.store(static_cast<T*>(b.dx) + at, d);
     now = next;
@@ -221,23 +241,23 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     if (group >= 0) leave_group(group, g);
     if constexpr (POST) {
 #pragma unroll
-      for (int j = 0; j < kRowElems; ++j) {
-        sum_A[j] = s_C[j];
-        sum_B[j] = s_D[j];
+      for (int j = 0; j < kPairs; ++j) {
+        sum_A[j] = s_C2[j];
+        sum_B[j] = s_D2[j];
       }
     }
   }
 
   // the CTA's sums
   float* part = b.parts + (int64_t)blockIdx.x * b.vectors * f.hidden;
-  auto write = [&](float (&v)[kRowElems], int vector) {
+  auto write = [&](const uint64_t (&v)[kPairs], int vector) {
     if (f.teams == 1) {
       cols.store(part + (int64_t)vector * f.hidden, v);
       return;
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kRowElems; ++j) s_team[threadIdx.x * kRowElems + j] = v[j];
+    for (int j = 0; j < kPairs; ++j) reinterpret_cast<uint64_t*>(s_team)[threadIdx.x * kPairs + j] = v[j];
     __syncthreads();
     const int all = f.team_threads * kRowElems;
     for (int i = threadIdx.x; i < all; i += blockDim.x) {

@@ -11,12 +11,16 @@
 
 namespace fdb {
 
+using ptx::add_f32x2;
+using ptx::fma_f32x2;
+using ptx::mul_f32x2;
+
 // Up to 1024 elements a row belongs to one warp (ONE): its sums are shuffles, and nothing keeps the next row's loads from starting.
 // Longer rows take as many warps, with barriers of their own between them.
 constexpr int kNormFwdThreads = 128, kNormFwdWarpElems = 1024;
 
 template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>
-__global__ void __launch_bounds__(ONE ? kNormFwdThreads : 256, ONE ? 5 : 2) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
+__global__ void __launch_bounds__(ONE ? kNormFwdThreads : 256, ONE ? 4 : 2) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
   constexpr int kElems = V * kRowElems;
   __shared__ __align__(16) float s_sums[ONE ? 1 : kNormFwdThreads / 32][TeamSum<1>::kSlots];
   const int team = ONE ? threadIdx.x >> 5 : threadIdx.x / a.team_threads, t = ONE ? threadIdx.x & 31 : threadIdx.x - team * a.team_threads;
@@ -31,66 +35,72 @@ __global__ void __launch_bounds__(ONE ? kNormFwdThreads : 256, ONE ? 5 : 2) resi
   const T* residual = static_cast<const T*>(a.residual);
 
   // statistics of a row; afterwards v holds its normalised form
-  auto normalise = [&](float (&v)[kElems], float& mean, float& inv) {
-    float sum[1] = {0.f};
+  auto normalise = [&](uint64_t (&v)[kElems / 2], float& mean, float& inv) {
+    uint64_t sum = both(0.f);
+    float total[1];
     mean = 0.f;
     if constexpr (!RMS) {
 #pragma unroll
-      for (int j = 0; j < kElems; ++j) sum[0] += v[j];
-      team_sum(sum);
-      mean = sum[0] * inv_hidden;
-      sum[0] = 0.f;
+      for (int j = 0; j < kElems / 2; ++j) sum = add_f32x2(sum, v[j]);
+      total[0] = fold(sum);
+      team_sum(total);
+      mean = total[0] * inv_hidden;
+#pragma unroll
+      for (int j = 0; j < kElems / 2; ++j) v[j] = add_f32x2(v[j], cols.inside(j, -mean));
+      sum = both(0.f);
     }
 #pragma unroll
-    for (int j = 0; j < kElems; ++j) {
-      if constexpr (!RMS) v[j] = cols.live(j) ? v[j] - mean : 0.f;
-      sum[0] = fmaf(v[j], v[j], sum[0]);
-    }
-    team_sum(sum);
-    inv = 1.f / sqrtf(fmaf(sum[0], inv_hidden, a.eps));
+    for (int j = 0; j < kElems / 2; ++j) sum = fma_f32x2(v[j], v[j], sum);
+    total[0] = fold(sum);
+    team_sum(total);
+    inv = 1.f / sqrtf(fmaf(total[0], inv_hidden, a.eps));
+    const uint64_t inv2 = both(inv);
 #pragma unroll
-    for (int j = 0; j < kElems; ++j) v[j] *= inv;
+    for (int j = 0; j < kElems / 2; ++j) v[j] = mul_f32x2(v[j], inv2);
   };
-  auto affine = [&](float (&v)[kElems], const void* weight, const void* bias) {
-    float p[kElems];
+  auto affine = [&](uint64_t (&v)[kElems / 2], const void* weight, const void* bias) {
+    uint64_t p[kElems / 2];
     cols.template load_param<T>(weight, a.param_fp32, 0, p);
+    if (!RMS && bias != nullptr) {
+      uint64_t q[kElems / 2];
+      cols.template load_param<T>(bias, a.param_fp32, 0, q);
 #pragma unroll
-    for (int j = 0; j < kElems; ++j) v[j] *= p[j];
-    if (RMS || bias == nullptr) return;
-    cols.template load_param<T>(bias, a.param_fp32, 0, p);
+      for (int j = 0; j < kElems / 2; ++j) v[j] = fma_f32x2(v[j], p[j], q[j]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < kElems; ++j) v[j] += p[j];
+      for (int j = 0; j < kElems / 2; ++j) v[j] = mul_f32x2(v[j], p[j]);
+    }
   };
 
   const int64_t row = (int64_t)blockIdx.x * a.teams + team;
-  if (row < a.rows) {
-    const int64_t at = row * a.hidden;
-    RowWords<T, V> rx, rr;
-    cols.load(x + at, rx);
-    if (residual != nullptr) cols.load(residual + at, rr);
-    float v[kElems], p[kElems];
-    float4 stats = make_float4(0.f, 1.f, 0.f, 1.f);
-    unpack(rx, v);
-    if constexpr (POST) {
-      normalise(v, stats.x, stats.y);
-      affine(v, a.post_weight, a.post_bias);
-    }
-    if (a.gate != nullptr) {
-      cols.template load_param<T>(a.gate, a.gate_fp32, (int64_t)((uint32_t)row / a.gate_rows) * a.hidden, p);
-#pragma unroll
-      for (int j = 0; j < kElems; ++j) v[j] *= p[j];
-    }
-    if (residual != nullptr) {
-      unpack(rr, p);
-#pragma unroll
-      for (int j = 0; j < kElems; ++j) v[j] = fmaf(a.residual_scale, p[j], v[j]);
-    }
-    if (a.stream != nullptr) cols.store(static_cast<T*>(a.stream) + at, v);
-    normalise(v, stats.z, stats.w);
-    affine(v, a.weight, a.bias);
-    cols.store(static_cast<T*>(a.normed) + at, v);
-    if (a.stats != nullptr && t == 0) a.stats[row] = stats;
+  if (row >= a.rows) return;
+  const int64_t at = row * a.hidden;
+  RowWords<T, V> rx, rr;
+  cols.load(x + at, rx);
+  if (residual != nullptr) cols.load(residual + at, rr);
+  uint64_t v[kElems / 2], p[kElems / 2];
+  float4 stats = make_float4(0.f, 1.f, 0.f, 1.f);
+  unpack(rx, v);
+  if constexpr (POST) {
+    normalise(v, stats.x, stats.y);
+    affine(v, a.post_weight, a.post_bias);
   }
+  if (a.gate != nullptr) {
+    cols.template load_param<T>(a.gate, a.gate_fp32, (int64_t)((uint32_t)row / a.gate_rows) * a.hidden, p);
+#pragma unroll
+    for (int j = 0; j < kElems / 2; ++j) v[j] = mul_f32x2(v[j], p[j]);
+  }
+  if (residual != nullptr) {
+    const uint64_t scale = both(a.residual_scale);
+    unpack(rr, p);
+#pragma unroll
+    for (int j = 0; j < kElems / 2; ++j) v[j] = fma_f32x2(scale, p[j], v[j]);
+  }
+  if (a.stream != nullptr) cols.store(static_cast<T*>(a.stream) + at, v);
+  normalise(v, stats.z, stats.w);
+  affine(v, a.weight, a.bias);
+  cols.store(static_cast<T*>(a.normed) + at, v);
+  if (a.stats != nullptr && t == 0) a.stats[row] = stats;
 }
 
 template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>

@@ -67,6 +67,27 @@ template <int N> __device__ __forceinline__ void pack(const float (&v)[N], RowWo
   }
 }
 
+// The same as pairs of fp32 in 64-bit registers, for the two-wide arithmetic: half the instructions of a kernel that has to issue some
+// forty per element.
+template <typename T, int V> __device__ __forceinline__ void unpack(const RowWords<T, V>& r, uint64_t (&v)[V * kRowElems / 2]) {
+  float f[V * kRowElems];
+  unpack(r, f);
+#pragma unroll
+  for (int j = 0; j < V * kRowElems / 2; ++j) v[j] = ptx::pack_f32x2(f[2 * j], f[2 * j + 1]);
+}
+template <typename T, int V> __device__ __forceinline__ void pack(const uint64_t (&v)[V * kRowElems / 2], RowWords<T, V>& r) {
+  float f[V * kRowElems];
+#pragma unroll
+  for (int j = 0; j < V * kRowElems / 2; ++j) ptx::unpack_f32x2(v[j], f[2 * j], f[2 * j + 1]);
+  pack(f, r);
+}
+__device__ __forceinline__ uint64_t both(float v) { return ptx::pack_f32x2(v, v); }
+__device__ __forceinline__ float fold(uint64_t v) {  // the sum of a pair
+  float lo, hi;
+  ptx::unpack_f32x2(v, lo, hi);
+  return lo + hi;
+}
+
 // Which columns of a row a thread holds.
 template <bool WIDE, int V = 1> struct RowColumns {
   static constexpr int kElems = V * kRowElems;
@@ -138,8 +159,22 @@ template <bool WIDE, int V = 1> struct RowColumns {
     pack(v, r);
     store(row, r);
   }
+  template <typename T> __device__ __forceinline__ void load(const T* row, uint64_t (&v)[kElems / 2]) const {
+    RowWords<T, V> r;
+    load(row, r);
+    unpack(r, v);
+  }
+  template <typename T> __device__ __forceinline__ void store(T* row, const uint64_t (&v)[kElems / 2]) const {
+    RowWords<T, V> r;
+    pack(v, r);
+    store(row, r);
+  }
+  // a number where the row has columns, zero behind its end
+  __device__ __forceinline__ uint64_t inside(int pair, float v) const {
+    return WIDE ? both(live(2 * pair) ? v : 0.f) : ptx::pack_f32x2(live(2 * pair) ? v : 0.f, live(2 * pair + 1) ? v : 0.f);
+  }
   // a vector over the columns, either of the rows' type or fp32
-  template <typename T> __device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at, float (&v)[kElems]) const {
+  template <typename T, typename F> __device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at, F& v) const {
     if (fp32) load(static_cast<const float*>(p) + at, v);
     else load(static_cast<const T*>(p) + at, v);
   }
