@@ -5,12 +5,13 @@ src/flashdeberta/model.py:394-920), which launches over lists of tensors per typ
 """
 from __future__ import annotations
 
-import array
 import bisect
 import ctypes as C
 import math
+import operator
 from typing import Iterable, List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from . import _lib, ops
@@ -45,51 +46,66 @@ def _apart(writes, reads=()) -> bool:
     return True
 
 
-_at, _count, _size, _whole, _card = (
-    torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.element_size, torch.Tensor.is_contiguous, torch.Tensor.get_device)
+_at, _count, _whole, _card = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype, _layout, _shape = (operator.attrgetter(n) for n in ("dtype", "layout", "shape"))
+_BYTES = np.zeros(1 + max(TYPES.values()), np.int64)
+for _t, _kind in TYPES.items():
+    _BYTES[_kind] = _t.itemsize
+
+
+def _numbers(of, tensors) -> np.ndarray:
+    return np.fromiter(map(of, tensors), np.int64, len(tensors))
+
+
+def _kinds(tensors) -> np.ndarray:
+    return np.fromiter(map(TYPES.__getitem__, map(_dtype, tensors)), np.int64, len(tensors))
 
 
 def _run(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], max_norm: float, norm_type: float) -> torch.Tensor:
     """One C call: the norm, and, with ``outs``, the scaled tensors.  All are runs of memory."""
-    table = array.array("q", bytes(32 * len(grads)))  # rows of fdb_grad_tensor: two addresses, the count, both types
-    at, count, kinds = list(map(_at, grads)), list(map(_count, grads)), [TYPES[g.dtype] for g in grads]
-    to, into = at, kinds
-    if outs is not None and outs is not grads:
-        to, into = list(map(_at, outs)), [TYPES[o.dtype] for o in outs]
-        own = [a == b for a, b in zip(at, to)]
-        if any(i and a != b for i, a, b in zip(own, kinds, into)):
-            raise ValueError("a gradient cannot be scaled in place into another type")
+    at, count, kind = _numbers(_at, grads), _numbers(_count, grads), _kinds(grads)
+    to, into = at, kind
     if outs is not None:
-        ends = [a + n * s for a, n, s in zip(to, count, map(_size, outs))]
-        more = [] if outs is grads else [(a, a + n * s) for a, n, s, i in zip(at, count, map(_size, grads), own) if not i]
+        if outs is not grads:
+            to, into = _numbers(_at, outs), _kinds(outs)
+        starts, ends = to, to + count * _BYTES[into]
+        if outs is not grads:
+            read = at != to  # (the others are their own outputs)
+            if (kind != into)[~read].any():
+                raise ValueError("a gradient cannot be scaled in place into another type")
+            starts, ends = np.concatenate((to, at[read])), np.concatenate((ends, (at + count * _BYTES[kind])[read]))
         # runs of memory are apart where each ends, in order, before the next begins
-        if any(a > b for a, b in zip(sorted(ends + [hi for _, hi in more]), sorted(to + [lo for lo, _ in more])[1:])) and not _apart(zip(to, ends), more):
-            raise ValueError("the tensors that are written overlap one another or a gradient that is read")
-    table[0::4], table[1::4], table[2::4] = array.array("q", at), array.array("q", to), array.array("q", count)
-    table[3::4] = array.array("q", [a | b << 32 for a, b in zip(kinds, into)])
+        if (np.sort(ends)[:-1] > np.sort(starts)[1:]).any():
+            n = len(to)
+            if not _apart(zip(starts[:n].tolist(), ends[:n].tolist()), zip(starts[n:].tolist(), ends[n:].tolist())):
+                raise ValueError("the tensors that are written overlap one another or a gradient that is read")
+    table = np.empty((len(grads), 4), np.int64)  # rows of fdb_grad_tensor: two addresses, the count, both types
+    table[:, 0], table[:, 1], table[:, 2], table[:, 3] = at, to, count, kind | into << 32
     device, lib = grads[0].device, _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=device)
-    p = _lib.ClipGradsParams(C.sizeof(_lib.ClipGradsParams), len(grads), table.buffer_info()[0], _NORMS[norm_type], int(outs is not None),
+    p = _lib.ClipGradsParams(C.sizeof(_lib.ClipGradsParams), len(grads), table.ctypes.data, _NORMS[norm_type], int(outs is not None),
                              max_norm, norm.data_ptr(), None, 0)
     with ops.on_device(device):
         need = lib.fdb_clip_grads_workspace_bytes(C.byref(p))
         ws = norm.new_empty(max(need, 16), dtype=torch.uint8)
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
         _lib.check(lib.fdb_clip_grads(C.byref(p), ops.raw_stream(device)))
+    if outs is not None:  # the write is seen by whoever compares versions (autograd, the caches of this package)
+        torch.autograd.graph.increment_version(outs)
     ops._launches += 2
     return norm
 
 
 def _listed(grads: Tensors, what: str) -> List[torch.Tensor]:
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if any(g.layout is not torch.strided for g in grads):
+    if not set(map(_layout, grads)) <= {torch.strided}:
         raise TypeError(f"{what} takes dense tensors")
     cards = set(map(_card, grads))
     if -1 in cards:
         raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
     if len(cards) > 1:
         raise ValueError(f"{what} takes tensors of one device, got {sorted(cards)}")
-    other = {g.dtype for g in grads} - TYPES.keys()
+    other = set(map(_dtype, grads)) - TYPES.keys()
     if other:
         raise TypeError(f"{what} takes bfloat16, float16 or float32 tensors, not {other.pop()}")
     return grads
@@ -102,17 +118,15 @@ def _norm_type(norm_type: float) -> float:
     return norm_type
 
 
-@torch.no_grad()
 def grad_norm(grads: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm (1, 2 or inf) over all elements of the tensors taken as one vector: a float32 scalar on their device, zero where there
     are none.  Tensors are bfloat16, float16 or float32 in any mixture, of one device."""
     norm_type, grads = _norm_type(norm_type), _listed(grads, "grad_norm")
     if not grads:
         return torch.tensor(0.0)
-    return _run([g if _dense(g) else g.contiguous() for g in grads], None, 0.0, norm_type)
+    return _run([g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads], None, 0.0, norm_type)
 
 
-@torch.no_grad()
 def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, norm as in ``grad_norm``, in place, or into ``out`` (tensors of the same
     shapes, of any of the three types: an optimizer's float32 buffers beside bfloat16 gradients), and returns the norm before.  Nothing
@@ -123,17 +137,26 @@ def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out:
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
     outs = grads if out is None else _listed(out, "clip_grads_")
-    if len(outs) != len(grads) or any(o is not g and o.shape != g.shape for g, o in zip(grads, outs)):
+    if out is not None and list(map(_shape, outs)) != list(map(_shape, grads)):
         raise ValueError("out must hold one tensor of the same shape for each gradient")
     if not grads:
         return torch.tensor(0.0)
     if outs[0].device != grads[0].device:
         raise ValueError(f"out is on {outs[0].device}, the gradients on {grads[0].device}")
-    if out is None and all(map(_whole, grads)):
-        if 0 in map(_count, grads):
-            grads = [g for g in grads if g.numel()] or grads[:1]
-        return _run(grads, grads, max_norm, norm_type)
-    # the kernel goes through memory: a tensor that is no run of it, or is ordered unlike its output, is taken through a copy
+    if not (all(map(_whole, grads)) and (out is None or all(map(_whole, outs)))):
+        return _clip_any(grads, outs, max_norm, norm_type)
+    if 0 in map(_count, grads):
+        keep = [i for i, g in enumerate(grads) if g.numel()]
+        if not keep:
+            return grads[0].new_zeros((), dtype=torch.float32)
+        outs = [outs[i] for i in keep]
+        grads = outs if out is None else [grads[i] for i in keep]
+    return _run(grads, outs, max_norm, norm_type)
+
+
+@torch.no_grad()
+def _clip_any(grads, outs, max_norm, norm_type):
+    """The kernel goes through memory: a tensor that is no run of it, or is ordered unlike its output, is taken through a copy."""
     reads, writes, back = [], [], []
     for g, o in zip(grads, outs):
         if g.numel() == 0:
@@ -156,7 +179,6 @@ def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out:
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_`` over this package's kernels: the gradients of the parameters that have one are clipped in
     place to ``max_norm``; returns their norm before.  ``error_if_nonfinite`` reads the norm back to the host first (and raises before

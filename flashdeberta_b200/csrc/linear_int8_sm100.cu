@@ -19,6 +19,7 @@
 #include "gelu.cuh"
 #include "internal.h"
 #include "launch.h"
+#include "linear_int8.h"
 #include "row_team.cuh"
 #include "sm100_ptx.cuh"
 #include "tensor_map.cuh"
@@ -389,7 +390,7 @@ using namespace fdb;
 
 extern "C" FDB_API uint64_t fdb_linear_int8_workspace_bytes(const fdb_linear_int8_params* p) {
   clear_error();
-  if (validate_int8(p) != FDB_OK || p->x_dtype == FDB_INT8 || p->rows == 0) return 0;
+  if (validate_int8(p) != FDB_OK || p->x_dtype == FDB_INT8 || p->rows == 0 || int8_is_small(*p)) return 0;
   return rows_bytes(*p) + uint64_t(p->rows) * sizeof(float);
 }
 
@@ -408,6 +409,7 @@ extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* st
       (p->bias != nullptr && !aligned_to(type_bytes(p->bias_dtype), p->bias)) || (!given && !aligned_to(type_bytes(p->x_dtype), p->x)))
     return fail(FDB_ERR_ALIGNMENT, "linear_int8: tensors must be aligned to their elements");
   if (p->rows == 0) return FDB_OK;
+  if (int8_is_small(*p)) return launch_linear_int8_small(*p, stream);
   const void* x = p->x;
   const float* x_scale = p->x_scale;
   int64_t pitch = p->x_pitch;

@@ -1,15 +1,14 @@
 // Rows as 8-bit integers with a scale each (fdb_quantize_int8): scale = amax / 127, y = rint(x * (127 / amax)).
 //
 // A warp per row of up to 1024 elements, up to eight warps beyond (row_team.cuh); a row of up to 8192 is read once and stays in
-// registers, a longer one is read a second time (it comes from L2 then).  HBM-bound: x read, one byte per element written.  The
-// magnitudes are compared as the bits of their absolute values: a NaN is larger than everything there, so it reaches the scale.
+// registers, a longer one is read a second time (it comes from L2 then).  HBM-bound: x read, one byte per element written.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
 #include "internal.h"
 #include "launch.h"
-#include "row_team.cuh"
+#include "quantize_int8.cuh"
 
 namespace fdb {
 namespace {
@@ -23,34 +22,6 @@ struct QuantArgs {
   int64_t rows, pitch;
   int cols, team_threads, teams;
 };
-
-// Largest magnitude of a thread's elements, as bits of T's absolute values; and such bits as fp32.
-template <int V> __device__ __forceinline__ uint32_t top_of(const RowWords<float, V>& r) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < V * kRowElems; ++j) top = max(top, r.w[j] & 0x7fffffffu);
-  return top;
-}
-template <typename T, int V> __device__ __forceinline__ uint32_t top_of(const RowWords<T, V>& r) {  // two at a time
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < V * kRowElems / 2; ++j) top = __vmaxu2(top, r.w[j] & 0x7fff7fffu);
-  return max(top & 0xffffu, top >> 16);
-}
-template <typename T> __device__ __forceinline__ float bits_to_float(uint32_t b) {
-  if constexpr (sizeof(T) == 4) return __uint_as_float(b);
-  const unsigned short h = (unsigned short)b;
-  return to_float<T>(*reinterpret_cast<const T*>(&h));
-}
-
-// Four products with the reciprocal scale, each rounded to fp32 and then to a whole number, as bytes: 1.5 * 2^23 added, the number is in
-// the lowest bits.  (float-to-int conversions run at a quarter of the rate.)
-__device__ __forceinline__ uint32_t four_bytes(const float* v, float inv) {
-  uint32_t b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], inv), 12582912.f));  // (as one FMA the product would not be rounded)
-  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-}
 
 template <typename T, bool WIDE, int V>
 __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
@@ -79,23 +50,20 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
       ptx::bar_sync((uint32_t)team + 1, (uint32_t)a.team_threads);
       for (int w = 0; w < warps; ++w) top = max(top, s[w]);
     }
-    const float amax = bits_to_float<T>(top);
-    const bool zero = amax < 7.888609052e-31f;                       // 2^-100: the reciprocal would leave fp32's range
-    const bool finite = amax <= 3.402823466e+38f;
-    const float inv = zero || !finite ? 0.f : 127.f / amax;
-    if (t == 0) a.scale[row] = zero ? 0.f : amax / 127.f;
+    const Int8Scale by = int8_scale<T>(top);
+    if (t == 0) a.scale[row] = by.scale;
     for (int at = 0; at < a.cols; at += span) {
       const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
       RowWords<T, V> r = first;
       if (at != 0) cols.load(x + at, r);
       unpack(r, v);
-      if (!finite)
+      if (!by.finite)
 #pragma unroll
         for (int j = 0; j < kElems; ++j) v[j] = 0.f;  // (an infinity times zero is a NaN)
       uint8_t* y = a.y + row * a.pitch + at;
 #pragma unroll
       for (int j = 0; j < kElems; j += kRowElems) {
-        const uint2 o = make_uint2(four_bytes(v + j, inv), four_bytes(v + j + 4, inv));
+        const uint2 o = make_uint2(four_bytes(v + j, by.inv), four_bytes(v + j + 4, by.inv));
         if constexpr (WIDE) {
           if (cols.live(j)) *reinterpret_cast<uint2*>(y + cols.col(j)) = o;
         } else {

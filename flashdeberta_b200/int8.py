@@ -87,7 +87,7 @@ def _(x, weight, weight_scale, bias, x_scale, gelu, out_dtype):
     return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype)
 
 
-_PARAMS = struct.Struct("@IiPqPPqPPPq6iPQP")  # fdb_linear_int8_params
+_PARAMS, _PARAMS_TAIL = struct.Struct("@IiPqPPqPPPq6iPQP"), struct.Struct("@PQP")  # fdb_linear_int8_params, its last three fields
 
 
 def _call(x, weight, weight_scale, bias, x_scale, gelu, out_dtype):
@@ -105,22 +105,22 @@ def _call(x, weight, weight_scale, bias, x_scale, gelu, out_dtype):
         w = _rows(weight)
     rows, k = out.numel() // n, shape[-1]
     lib = _lib.load()
+    if x_scale is None:
+        x = x if x.is_contiguous() else x.contiguous()
+        x_at, x_pitch, kind, scale_at = x.data_ptr(), 0, TYPES[x.dtype], 0
+    else:
+        x_scale = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
+        x = int8_rows(x)
+        (x_at, x_pitch), kind, scale_at = _rows(x), _lib.FDB_INT8, x_scale.data_ptr()
+    status = ops._status_word(device).data_ptr()
+    p = _PARAMS.pack(
+        _PARAMS.size, kind, x_at, x_pitch, scale_at, w[0], w[1], weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        out.data_ptr(), rows, k, n, 0 if bias is None else TYPES[bias.dtype], TYPES[out_dtype], gelu, 0, 0, 0, status)
     with ops.on_device(device):
-        if x_scale is None:
-            x = x if x.is_contiguous() else x.contiguous()
-            x_at, x_pitch, kind, scale_at = x.data_ptr(), 0, TYPES[x.dtype], 0
-            need = lib.fdb_linear_int8_workspace_bytes(_PARAMS.pack(_PARAMS.size, kind, 0, 0, 0, 0, 0, 0, 0, 0, rows, k, n, 0, 0, 0, 0, 0, 0, 0))
+        need = lib.fdb_linear_int8_workspace_bytes(p)
+        if need:  # the tokens as integers
             ws = x.new_empty(need + 255, dtype=torch.uint8)
-            ws_at = (ws.data_ptr() + 255) & ~255
-        else:
-            x_scale = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
-            x = int8_rows(x)
-            (x_at, x_pitch), kind, scale_at = _rows(x), _lib.FDB_INT8, x_scale.data_ptr()
-            need = ws_at = 0
-        p = _PARAMS.pack(
-            _PARAMS.size, kind, x_at, x_pitch, scale_at, w[0], w[1], weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
-            out.data_ptr(), rows, k, n, 0 if bias is None else TYPES[bias.dtype], TYPES[out_dtype], gelu, 0, ws_at, need,
-            ops._status_word(device).data_ptr())
+            p = p[:-_PARAMS_TAIL.size] + _PARAMS_TAIL.pack((ws.data_ptr() + 255) & ~255, need, status)
         _lib.check(lib.fdb_linear_int8(p, ops.raw_stream(device)))
     ops._launches += 1 + int(need > 0)
     return out

@@ -222,6 +222,24 @@ def test_streams_and_captures():
         _check(ts, [k * (step + 1) for k in kept], 2.0 / (w + 1e-6))
 
 
+def test_what_is_written_counts_as_modified():
+    """Version counters move, as with torch's own in-place operators: autograd and this package's caches go by them."""
+    ts = _tensors([(40, 50), 33], 9, [torch.float32])
+    out = [torch.empty_like(t) for t in ts]
+    before = [t._version for t in ts + out]
+    ops.grad_norm(ts)
+    assert [t._version for t in ts + out] == before
+    ops.clip_grads_(ts, 1.0, out=out)
+    assert [t._version for t in ts] == before[:2] and all(o._version > b for o, b in zip(out, before[2:]))
+    ops.clip_grads_(ts, 1.0)
+    assert all(t._version > b for t, b in zip(ts, before))
+    w = torch.nn.Parameter(ts[0].clone())
+    y = (w * w).sum()
+    ops.clip_grads_([w.detach()], 1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_parameters_on_a_model_with_shared_and_frozen_ones():
     model = torch.nn.Sequential(torch.nn.Linear(40, 40), torch.nn.Linear(40, 40)).to(DEV)
     model[1].weight = model[0].weight
