@@ -103,30 +103,42 @@ __device__ __forceinline__ void convert_piece(const uint32_t* acc, int count, in
   }
 }
 
-// The same where a row starts anywhere: 32 columns, turned in shared memory, two rows of 16 columns at a time across the lanes.  (A
-// thread writing its own row element by element would touch 32 sectors with every store.)  Column c of row r lies in word
-// 16 r + (c ^ (r / 2 % 16)): neither side of the turn has two lanes on one bank.
+// The same where a row starts anywhere: 32 x 32 results, turned in shared memory and written a row at a time across the lanes.  (A
+// thread writing its own row element by element would touch 32 sectors with every store.)  fp32 in two halves of 16 rows, column c
+// of row r in word 32 r + (c ^ r); 16-bit types two columns to a word, pair w of row r in word 16 r + (w ^ (r / 2 % 16)): neither side of
+// the turn has two lanes on one bank.
 template <typename T, bool GELU, int COLS>
-__device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, float x_scale, const float* cols, uint32_t* turn, int lane) {
+__device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (&acc)[32], int64_t row0, int n0, uint64_t sx, const float* cols, uint32_t* turn, int lane) {
+  float v[32];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int c = 0; c < 32; c += 4) {
+    const float4 ws = *reinterpret_cast<const float4*>(cols + c), b = *reinterpret_cast<const float4*>(cols + COLS + c);
+    unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c], acc[c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v[c], v[c + 1]);
+    unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + 2], acc[c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v[c + 2], v[c + 3]);
+  }
+  const int n = n0 + lane, rows = (int)min((int64_t)32, a.rows - row0);
+  T* out = static_cast<T*>(a.out) + row0 * a.n + n;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int c = 0; c < 16; ++c) turn[lane * 16 + (c ^ ((lane >> 1) & 15))] = acc[half * 16 + c];
-    __syncwarp();
-    const int c = lane & 15, up = lane >> 4, n = n0 + half * 16 + c;
-    const bool has = n < a.n;
-    const float ws = cols[half * 16 + c], b = cols[COLS + half * 16 + c];
-    const uint64_t ws2 = pack_f32x2(ws, ws), b2 = pack_f32x2(b, b);
-    T* out = static_cast<T*>(a.out) + row0 * a.n + n;
-#pragma unroll 4
-    for (int r = 0; r < 32; r += 4) {
-      const int r0 = r + up, r1 = r + 2 + up;
-      const float s0 = __shfl_sync(0xffffffffu, x_scale, r0), s1 = __shfl_sync(0xffffffffu, x_scale, r1);
-      float v0, v1;
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(turn[r0 * 16 + (c ^ ((r0 >> 1) & 15))], turn[r1 * 16 + (c ^ ((r1 >> 1) & 15))], ws2, pack_f32x2(s0, s1), b2), v0, v1);
-      if (has && row0 + r0 < a.rows) out[(int64_t)r0 * a.n] = from_float<T>(v0);
-      if (has && row0 + r1 < a.rows) out[(int64_t)r1 * a.n] = from_float<T>(v1);
+    for (int half = 0; half < 2; ++half) {
+      if ((lane >> 4) == half)
+#pragma unroll
+        for (int c = 0; c < 32; ++c) turn[(lane & 15) * 32 + (c ^ (lane & 15))] = __float_as_uint(v[c]);
+      __syncwarp();
+      if (n < a.n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (half * 16 + r < rows) out[(int64_t)(half * 16 + r) * a.n] = __uint_as_float(turn[r * 32 + (lane ^ r)]);
+      __syncwarp();
     }
+  } else {
+#pragma unroll
+    for (int w = 0; w < 16; ++w) turn[lane * 16 + (w ^ ((lane >> 1) & 15))] = pack_pair<T>(v[2 * w], v[2 * w + 1]);
+    __syncwarp();
+    if (n < a.n)
+#pragma unroll 16
+      for (int r = 0; r < 32; ++r)
+        if (r < rows) reinterpret_cast<unsigned short*>(out)[(int64_t)r * a.n] = (unsigned short)(turn[r * 16 + ((lane >> 1) ^ ((r >> 1) & 15))] >> (16 * (lane & 1)));
     __syncwarp();
   }
 }
@@ -266,8 +278,7 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
       const int64_t row0 = (int64_t)(tile / args.tiles_n) * (kBM * CG) + int(rank) * kBM + quarter * 32;
       const int n0 = (tile % args.tiles_n) * BN + part * kCols;
       const uint32_t acc = local & 1u;
-      const float xs = x_scale;
-      const uint64_t sx = pack_f32x2(xs, xs);
+      const uint64_t sx = pack_f32x2(x_scale, x_scale);
       __syncwarp();  // (the tile before has been read from here)
 #pragma unroll
       for (int i = 0; i < kCols / 32; ++i) {
@@ -297,7 +308,7 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
           const int n = n0 + at + c0;
           if (!has_rows || n >= args.n) continue;
           if (!args.wide) {
-            store_turned<OUT, GELU, kCols>(args, a, row0, n, xs, cols + at + c0, turn, lane);
+            store_turned<OUT, GELU, kCols>(args, a, row0, n, sx, cols + at + c0, turn, lane);
             continue;
           }
 #pragma unroll
@@ -366,7 +377,7 @@ constexpr Config kConfigs[] = {{2, 256, 680, 4800}, {2, 128, 430, 2700}, {1, 128
 
 bool float_type(int t) { return t == FDB_BF16 || t == FDB_FP16 || t == FDB_FP32; }
 unsigned type_bytes(int t) { return t == FDB_FP32 ? 4u : 2u; }
-int64_t pitch_of(const fdb_linear_int8_params& p) { return (int64_t(p.in_features) + 15) / 16 * 16; }
+int64_t pitch_of(const fdb_linear_int8_params& p) { return (int64_t(p.in_features) + 127) / 128 * 128; }  // whole lines of memory
 uint64_t rows_bytes(const fdb_linear_int8_params& p) { return (uint64_t(p.rows) * pitch_of(p) + 255) / 256 * 256; }
 
 int validate_int8(const fdb_linear_int8_params* p) {

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
 #include "launch.h"
@@ -14,6 +15,25 @@ namespace fdb {
 namespace {
 
 constexpr int kThreads = 128, kWarpElems = 1024;
+
+// Columns of a row that starts anywhere: runs of four per thread, so that what they become is stored four bytes at a time.
+template <int V> struct QuadColumns {
+  int t, threads, hidden;
+  __device__ __forceinline__ int col(int j) const { return (t + j / 4 * threads) * 4 + j % 4; }
+  template <typename T> __device__ __forceinline__ void load(const T* row, RowWords<T, V>& r) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < V * kRowElems; ++j) r.w[j] = col(j) < hidden ? __ldg(reinterpret_cast<const uint32_t*>(row) + col(j)) : 0u;
+    } else {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+      for (int j = 0; j < V * kRowElems; j += 2) {
+        const uint32_t lo = col(j) < hidden ? __ldg(p + col(j)) : 0u, hi = col(j + 1) < hidden ? __ldg(p + col(j + 1)) : 0u;
+        r.w[j / 2] = lo | (hi << 16);
+      }
+    }
+  }
+};
 
 struct QuantArgs {
   const void* x;
@@ -26,6 +46,7 @@ struct QuantArgs {
 template <typename T, bool WIDE, int V>
 __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
   constexpr int kElems = V * kRowElems;
+  using Columns = std::conditional_t<WIDE, RowColumns<true, V>, QuadColumns<V>>;
   __shared__ uint32_t s_top[kThreads / 32][8];
   const int team = threadIdx.x / a.team_threads, t = threadIdx.x - team * a.team_threads;
   const int warps = a.team_threads / 32, span = a.team_threads * kElems;
@@ -37,7 +58,7 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
     RowWords<T, V> first;
     float v[kElems];
     for (int at = 0; at < a.cols; at += span) {
-      const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
+      const Columns cols{t, a.team_threads, a.cols - at};
       RowWords<T, V> r;
       cols.load(x + at, r);
       top = max(top, top_of(r));
@@ -53,7 +74,7 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
     const Int8Scale by = int8_scale<T>(top);
     if (t == 0) a.scale[row] = by.scale;
     for (int at = 0; at < a.cols; at += span) {
-      const RowColumns<WIDE, V> cols{t, a.team_threads, a.cols - at};
+      const Columns cols{t, a.team_threads, a.cols - at};
       RowWords<T, V> r = first;
       if (at != 0) cols.load(x + at, r);
       unpack(r, v);
@@ -66,10 +87,9 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
         const uint2 o = make_uint2(four_bytes(v + j, by.inv), four_bytes(v + j + 4, by.inv));
         if constexpr (WIDE) {
           if (cols.live(j)) *reinterpret_cast<uint2*>(y + cols.col(j)) = o;
-        } else {
-#pragma unroll
-          for (int i = 0; i < kRowElems; ++i)
-            if (cols.live(j + i)) y[cols.col(j + i)] = (uint8_t)((i < 4 ? o.x : o.y) >> (8 * (i % 4)));
+        } else {  // (up to three zeros behind the row)
+          if (cols.col(j) < cols.hidden) *reinterpret_cast<uint32_t*>(y + cols.col(j)) = o.x;
+          if (cols.col(j + 4) < cols.hidden) *reinterpret_cast<uint32_t*>(y + cols.col(j + 4)) = o.y;
         }
       }
     }
@@ -94,7 +114,7 @@ int launch_quantize_int8(const void* x, int dtype, int64_t rows, int cols, void*
   const int warps = std::min(8, (cols + kWarpElems - 1) / kWarpElems), v = std::min(4, (cols + warps * 256 - 1) / (warps * 256));
   a.team_threads = warps * 32;
   a.teams = std::max(1, kThreads / a.team_threads);
-  const bool wide = cols % kRowElems == 0 && aligned_to(dtype == FDB_FP32 ? 32 : 16, x) && aligned_to(8, y) && pitch % 8 == 0;
+  const bool wide = cols % kRowElems == 0 && aligned_to(dtype == FDB_FP32 ? 32 : 16, x);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define FDB_QUANT(T) (wide ? launch<T, true>(a, v, s) : launch<T, false>(a, v, s))
   const cudaError_t e = dtype == FDB_BF16 ? FDB_QUANT(__nv_bfloat16) : (dtype == FDB_FP16 ? FDB_QUANT(__half) : FDB_QUANT(float));
@@ -116,7 +136,7 @@ extern "C" FDB_API int fdb_quantize_int8(const void* x, int32_t dtype, int64_t r
     return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: rows %lld, cols %d, pitch %lld", (long long)rows, cols, (long long)pitch);
   if (rows == 0) return FDB_OK;
   if (x == nullptr || y == nullptr || scale == nullptr) return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: x, y and scale must not be NULL");
-  if (!aligned_to(dtype == FDB_FP32 ? 4 : 2, x) || !aligned_to(4, scale))
-    return fail(FDB_ERR_ALIGNMENT, "quantize_int8: x and scale must be aligned to their elements");
+  if (!aligned_to(dtype == FDB_FP32 ? 4 : 2, x) || !aligned_to(4, scale) || !aligned_to(16, y) || pitch % 16 != 0)
+    return fail(FDB_ERR_ALIGNMENT, "quantize_int8: x and scale must be aligned to their elements, rows of y start on 16 bytes");
   return launch_quantize_int8(x, dtype, rows, cols, y, pitch, scale, stream);
 }

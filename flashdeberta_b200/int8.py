@@ -17,7 +17,9 @@ MAX_IN_FEATURES = 131071  # products of two 8-bit integers that a 32-bit sum hol
 
 
 def _pitch(cols: int) -> int:
-    return (cols + 15) // 16 * 16
+    """Bytes between rows: 16-byte pieces, and whole lines of memory where a row is longer than one (a tile's 128 bytes of a row would
+    lie on two otherwise)."""
+    return (cols + 127) // 128 * 128 if cols > 128 else (cols + 15) // 16 * 16
 
 
 def int8_rows(t: torch.Tensor) -> torch.Tensor:

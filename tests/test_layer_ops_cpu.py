@@ -124,9 +124,9 @@ def test_linear_int8_sizes():
 
 
 @pytest.mark.parametrize("args,code", [
-    ((P, 4, 2, 8, P, 8, P), -1), ((P, 0, -1, 8, P, 8, P), -1), ((P, 0, 2, 0, P, 8, P), -1), ((P, 0, 2, 8, P, 7, P), -1), ((None, 0, 2, 8, P, 8, P), -1),
-    ((P, 0, 2, 8, None, 8, P), -1), ((P, 0, 2, 8, P, 8, None), -1), ((P + 1, 0, 2, 8, P, 8, P), -3), ((P + 2, 1, 2, 8, P, 8, P), -3),
-    ((P, 0, 2, 8, P, 8, P + 2), -3),
+    ((P, 4, 2, 8, P, 16, P), -1), ((P, 0, -1, 8, P, 16, P), -1), ((P, 0, 2, 0, P, 16, P), -1), ((P, 0, 2, 18, P, 16, P), -1), ((None, 0, 2, 8, P, 16, P), -1),
+    ((P, 0, 2, 8, None, 16, P), -1), ((P, 0, 2, 8, P, 16, None), -1), ((P + 1, 0, 2, 8, P, 16, P), -3), ((P + 2, 1, 2, 8, P, 16, P), -3),
+    ((P, 0, 2, 8, P, 16, P + 2), -3), ((P, 0, 2, 8, P + 8, 16, P), -3), ((P, 0, 2, 8, P, 24, P), -3), ((P, 0, 1 << 31, 8, P, 16, P), -6),
 ])
 def test_quantize_int8_argument_errors(args, code):
     _refused(_lib.load().fdb_quantize_int8(*args, None), code)
