@@ -16,98 +16,145 @@ using ptx::fma_f32x2;
 using ptx::mul_f32x2;
 
 // Up to 1024 elements a row belongs to one warp (ONE): its sums are shuffles, and nothing keeps the next row's loads from starting.
-// Longer rows take as many warps, with barriers of their own between them.
-constexpr int kNormFwdThreads = 128, kNormFwdWarpElems = 1024;
+// Longer rows take as many warps, with barriers of their own between them.  A CTA stays and takes row after row: weights and biases
+// (and a channel's gate) are converted to fp32 once, into shared memory, and the next row is on its way while one is worked on.
+constexpr int kNormFwdWarpElems = 1024;
+constexpr int kNormFwdThreads = 512;  // of a CTA of longer rows, one per SM (at most 128 registers a thread)
+// CTAs per SM of rows of one warp, 4 rows each: what the registers of V x 8 elements per thread allow.
+constexpr int norm_fwd_ctas(int v) { return v == 1 ? 10 : (v == 2 ? 7 : 4); }
 
 template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>
-__global__ void __launch_bounds__(ONE ? kNormFwdThreads : 256, ONE ? 4 : 2) residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
-  constexpr int kElems = V * kRowElems;
-  __shared__ __align__(16) float s_sums[ONE ? 1 : kNormFwdThreads / 32][TeamSum<1>::kSlots];
-  const int team = ONE ? threadIdx.x >> 5 : threadIdx.x / a.team_threads, t = ONE ? threadIdx.x & 31 : threadIdx.x - team * a.team_threads;
-  const RowColumns<WIDE, V> cols{t, ONE ? 32 : a.team_threads, a.hidden};
-  TeamSum<1> team_sum{s_sums[ONE ? 0 : team], ONE ? 1 : a.team_threads / 32, t >> 5, team + 1, 0};
-  if constexpr (!ONE) {
-    for (int i = threadIdx.x; i < int(sizeof(s_sums) / sizeof(float)); i += blockDim.x) s_sums[0][i] = 0.f;
-    __syncthreads();
-  }
+__global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ctas(V) : 1)
+    residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
+  constexpr int kElems = V * kRowElems, kPairs = kElems / 2;
+  extern __shared__ __align__(16) float4 s_vectors[];
+  __shared__ __align__(16) float s_sums[ONE ? 1 : kNormFwdThreads / 64][TeamSum<1>::kSlots];
+  const int threads = ONE ? 32 : a.team_threads;
+  const int team = ONE ? threadIdx.x >> 5 : threadIdx.x / threads, t = ONE ? threadIdx.x & 31 : threadIdx.x - team * threads;
+  const RowColumns<WIDE, V> cols{t, threads, a.hidden};
+  TeamSum<1> team_sum{s_sums[ONE ? 0 : team], threads / 32, t >> 5, team + 1, 0};
   const float inv_hidden = 1.f / (float)a.hidden;
-  const T* x = static_cast<const T*>(a.x);
-  const T* residual = static_cast<const T*>(a.residual);
 
-  // statistics of a row; afterwards v holds its normalised form
-  auto normalise = [&](uint64_t (&v)[kElems / 2], float& mean, float& inv) {
+  RowWords<T, V> rx, rr, nx, nr;
+  auto fetch = [&](int64_t row, RowWords<T, V>& wx, RowWords<T, V>& wr) {
+    cols.load(static_cast<const T*>(a.x) + row * a.hidden, wx);
+    if (a.residual != nullptr) cols.load(static_cast<const T*>(a.residual) + row * a.hidden, wr);
+  };
+  const int64_t step = (int64_t)gridDim.x * a.teams;
+  int64_t row = (int64_t)blockIdx.x * a.teams + team;
+  constexpr bool kAhead = sizeof(T) == 2 && WIDE;  // (fp32 rows would take too many registers, single elements are put into words at once)
+  if (kAhead && row < a.rows) fetch(row, nx, nr);
+
+  // vectors over the columns: 16-byte pieces, each piece of the team's threads side by side
+  enum : int { kWeight = 0, kBias = 1, kPostWeight = 2, kPostBias = 3, kGateVector = 4 };
+  const bool channel_gate = a.gate != nullptr && a.gate_rows == a.rows;
+  auto put_vector = [&](int v, const void* p, bool fp32) {
+    float q[kElems];
+    if (p != nullptr) cols.template load_param<T>(p, fp32, 0, q);
+    else
+#pragma unroll
+      for (int j = 0; j < kElems; ++j) q[j] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kElems; j += 4) s_vectors[(v * (kElems / 4) + j / 4) * threads + t] = make_float4(q[j], q[j + 1], q[j + 2], q[j + 3]);
+  };
+  // two pairs of a vector
+  auto get = [&](int v, int j) { return *reinterpret_cast<const ulonglong2*>(s_vectors + (v * (kElems / 4) + j / 2) * threads + t); };
+  if (team == 0) {
+    put_vector(kWeight, a.weight, a.param_fp32);
+    if (!RMS) put_vector(kBias, a.bias, a.param_fp32);
+    if (POST) put_vector(kPostWeight, a.post_weight, a.param_fp32);
+    if (POST && !RMS) put_vector(kPostBias, a.post_bias, a.param_fp32);
+    if (channel_gate) put_vector(kGateVector, a.gate, a.gate_fp32);
+  }
+  if constexpr (!ONE)
+    for (int i = threadIdx.x; i < int(sizeof(s_sums) / sizeof(float)); i += blockDim.x) s_sums[0][i] = 0.f;
+  __syncthreads();
+
+  // statistics of a row; afterwards v holds its normalised form, weighted
+  auto normalise = [&](uint64_t (&v)[kPairs], float& mean, float& inv, int weight, int bias) {
     uint64_t sum = both(0.f);
     float total[1];
     mean = 0.f;
     if constexpr (!RMS) {
 #pragma unroll
-      for (int j = 0; j < kElems / 2; ++j) sum = add_f32x2(sum, v[j]);
+      for (int j = 0; j < kPairs; ++j) sum = add_f32x2(sum, v[j]);
       total[0] = fold(sum);
       team_sum(total);
       mean = total[0] * inv_hidden;
 #pragma unroll
-      for (int j = 0; j < kElems / 2; ++j) v[j] = add_f32x2(v[j], cols.inside(j, -mean));
+      for (int j = 0; j < kPairs; ++j) v[j] = add_f32x2(v[j], cols.inside(j, -mean));
       sum = both(0.f);
     }
 #pragma unroll
-    for (int j = 0; j < kElems / 2; ++j) sum = fma_f32x2(v[j], v[j], sum);
+    for (int j = 0; j < kPairs; ++j) sum = fma_f32x2(v[j], v[j], sum);
     total[0] = fold(sum);
     team_sum(total);
     inv = 1.f / sqrtf(fmaf(total[0], inv_hidden, a.eps));
     const uint64_t inv2 = both(inv);
 #pragma unroll
-    for (int j = 0; j < kElems / 2; ++j) v[j] = mul_f32x2(v[j], inv2);
-  };
-  auto affine = [&](uint64_t (&v)[kElems / 2], const void* weight, const void* bias) {
-    uint64_t p[kElems / 2];
-    cols.template load_param<T>(weight, a.param_fp32, 0, p);
-    if (!RMS && bias != nullptr) {
-      uint64_t q[kElems / 2];
-      cols.template load_param<T>(bias, a.param_fp32, 0, q);
-#pragma unroll
-      for (int j = 0; j < kElems / 2; ++j) v[j] = fma_f32x2(v[j], p[j], q[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kElems / 2; ++j) v[j] = mul_f32x2(v[j], p[j]);
+    for (int j = 0; j < kPairs; j += 2) {
+      const ulonglong2 w = get(weight, j);
+      v[j] = mul_f32x2(v[j], inv2);
+      v[j + 1] = mul_f32x2(v[j + 1], inv2);
+      if constexpr (RMS) {
+        v[j] = mul_f32x2(v[j], w.x);
+        v[j + 1] = mul_f32x2(v[j + 1], w.y);
+      } else {
+        const ulonglong2 b = get(bias, j);
+        v[j] = fma_f32x2(v[j], w.x, b.x);
+        v[j + 1] = fma_f32x2(v[j + 1], w.y, b.y);
+      }
     }
   };
 
-  const int64_t row = (int64_t)blockIdx.x * a.teams + team;
-  if (row >= a.rows) return;
-  const int64_t at = row * a.hidden;
-  RowWords<T, V> rx, rr;
-  cols.load(x + at, rx);
-  if (residual != nullptr) cols.load(residual + at, rr);
-  uint64_t v[kElems / 2], p[kElems / 2];
-  float4 stats = make_float4(0.f, 1.f, 0.f, 1.f);
-  unpack(rx, v);
-  if constexpr (POST) {
-    normalise(v, stats.x, stats.y);
-    affine(v, a.post_weight, a.post_bias);
-  }
-  if (a.gate != nullptr) {
-    cols.template load_param<T>(a.gate, a.gate_fp32, (int64_t)((uint32_t)row / a.gate_rows) * a.hidden, p);
+#pragma unroll 1
+  for (; row < a.rows; row += step) {
+    const int64_t at = row * a.hidden;
+    if constexpr (kAhead) {
+      rx = nx;
+      rr = nr;
+      if (row + step < a.rows) fetch(row + step, nx, nr);
+    } else {
+      fetch(row, rx, rr);
+    }
+    uint64_t v[kPairs], p[kPairs];
+    float4 stats = make_float4(0.f, 1.f, 0.f, 1.f);
+    unpack(rx, v);
+    if constexpr (POST) normalise(v, stats.x, stats.y, kPostWeight, kPostBias);
+    if (channel_gate) {
 #pragma unroll
-    for (int j = 0; j < kElems / 2; ++j) v[j] = mul_f32x2(v[j], p[j]);
-  }
-  if (residual != nullptr) {
-    const uint64_t scale = both(a.residual_scale);
-    unpack(rr, p);
+      for (int j = 0; j < kPairs; j += 2) {
+        const ulonglong2 g = get(kGateVector, j);
+        v[j] = mul_f32x2(v[j], g.x);
+        v[j + 1] = mul_f32x2(v[j + 1], g.y);
+      }
+    } else if (a.gate != nullptr) {
+      cols.template load_param<T>(a.gate, a.gate_fp32, (int64_t)((uint32_t)row / a.gate_rows) * a.hidden, p);
 #pragma unroll
-    for (int j = 0; j < kElems / 2; ++j) v[j] = fma_f32x2(scale, p[j], v[j]);
+      for (int j = 0; j < kPairs; ++j) v[j] = mul_f32x2(v[j], p[j]);
+    }
+    if (a.residual != nullptr) {
+      const uint64_t scale = both(a.residual_scale);
+      unpack(rr, p);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) v[j] = fma_f32x2(scale, p[j], v[j]);
+    }
+    if (a.stream != nullptr) cols.store(static_cast<T*>(a.stream) + at, v);
+    normalise(v, stats.z, stats.w, kWeight, kBias);
+    cols.store(static_cast<T*>(a.normed) + at, v);
+    if (a.stats != nullptr && t == 0) a.stats[row] = stats;
   }
-  if (a.stream != nullptr) cols.store(static_cast<T*>(a.stream) + at, v);
-  normalise(v, stats.z, stats.w);
-  affine(v, a.weight, a.bias);
-  cols.store(static_cast<T*>(a.normed) + at, v);
-  if (a.stats != nullptr && t == 0) a.stats[row] = stats;
 }
 
 template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>
 int norm_fwd_launch_kernel(const ResidualNormArgs& a, cudaStream_t s) {
-  const int threads = a.teams * a.team_threads;
-  residual_norm_kernel<T, RMS, POST, WIDE, V, ONE><<<(unsigned)((a.rows + a.teams - 1) / a.teams), (unsigned)threads, 0, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  static std::atomic<uint64_t> smem_done{0};
+  auto kernel = residual_norm_kernel<T, RMS, POST, WIDE, V, ONE>;
+  const int threads = a.teams * a.team_threads, smem = 5 * V * kRowElems * a.team_threads * (int)sizeof(float);
+  constexpr int kMost = 5 * V * kRowElems * (ONE ? 32 : 256) * (int)sizeof(float);
+  const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (ONE ? norm_fwd_ctas(V) : 1);
+  cudaError_t e = smem > 40 * 1024 ? allow_smem(smem_done, reinterpret_cast<const void*>(kernel), kMost) : cudaSuccess;
+  if (e == cudaSuccess) e = launch_kernel<ResidualNormArgs>(kernel, a, dim3((unsigned)std::min(want, most)), threads, smem, false, s);
   if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm launch: %s", cudaGetErrorString(e));
   return FDB_OK;
 }
@@ -117,7 +164,7 @@ template <typename T> int norm_fwd_launch(ResidualNormArgs a, bool wide, cudaStr
   const int warps = (a.hidden + kNormFwdWarpElems - 1) / kNormFwdWarpElems;
   const int v = (a.hidden + warps * 32 * kRowElems - 1) / (warps * 32 * kRowElems);
   a.team_threads = warps * 32;
-  a.teams = std::max(1, kNormFwdThreads / a.team_threads);
+  a.teams = (warps == 1 ? 128 : kNormFwdThreads) / a.team_threads;
 #define FDB_FWD4(R, P, W, V, ONE) norm_fwd_launch_kernel<T, R, P, W, V, ONE>(a, s)
 #define FDB_FWD3(R, P, W)                                                                  \
   (warps > 1 ? (v == 3 ? FDB_FWD4(R, P, W, 3, false) : FDB_FWD4(R, P, W, 4, false))       \
