@@ -47,43 +47,62 @@ def _apart(writes, reads=()) -> bool:
 
 
 _at, _count, _whole, _card = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
-_dtype, _layout, _shape = (operator.attrgetter(n) for n in ("dtype", "layout", "shape"))
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
 _BYTES = np.zeros(1 + max(TYPES.values()), np.int64)
 for _t, _kind in TYPES.items():
     _BYTES[_kind] = _t.itemsize
 
 
-def _numbers(of, tensors) -> np.ndarray:
-    return np.fromiter(map(of, tensors), np.int64, len(tensors))
+class _Listed:
+    """Tensors of one device as the C call sees them: addresses, counts, types."""
+
+    def __init__(self, tensors: Tensors, what: str):
+        tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        if not set(map(type, tensors)) <= _PLAIN:
+            raise TypeError(f"{what} takes plain tensors (it goes by their memory: no traced, fake or distributed ones)")
+        cards = set(map(_card, tensors))
+        if -1 in cards:
+            raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
+        if len(cards) > 1:
+            raise ValueError(f"{what} takes tensors of one device, got {sorted(cards)}")
+        self.tensors, n = tensors, len(tensors)
+        try:
+            self.kind = np.fromiter(map(TYPES.__getitem__, map(_dtype, tensors)), np.int64, n)
+        except KeyError as e:
+            raise TypeError(f"{what} takes bfloat16, float16 or float32 tensors, not {e.args[0]}") from None
+        try:
+            self.at = np.fromiter(map(_at, tensors), np.int64, n)
+        except (RuntimeError, NotImplementedError):  # no memory to point at
+            raise TypeError(f"{what} takes dense tensors") from None
+        self.count = np.fromiter(map(_count, tensors), np.int64, n)
+
+    def whole(self) -> bool:
+        return all(map(_whole, self.tensors))
 
 
-def _kinds(tensors) -> np.ndarray:
-    return np.fromiter(map(TYPES.__getitem__, map(_dtype, tensors)), np.int64, len(tensors))
-
-
-def _run(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], max_norm: float, norm_type: float) -> torch.Tensor:
+def _run(grads: _Listed, outs: Optional[_Listed], max_norm: float, norm_type: float) -> torch.Tensor:
     """One C call: the norm, and, with ``outs``, the scaled tensors.  All are runs of memory."""
-    at, count, kind = _numbers(_at, grads), _numbers(_count, grads), _kinds(grads)
-    to, into = at, kind
+    at, count, kind = grads.at, grads.count, grads.kind
+    to, into = (at, kind) if outs is None else (outs.at, outs.kind)
     if outs is not None:
-        if outs is not grads:
-            to, into = _numbers(_at, outs), _kinds(outs)
         starts, ends = to, to + count * _BYTES[into]
         if outs is not grads:
-            read = at != to  # (the others are their own outputs)
-            if (kind != into)[~read].any():
+            read = (at != to) & (count > 0)  # (the others are their own outputs)
+            if (kind != into)[(at == to) & (count > 0)].any():
                 raise ValueError("a gradient cannot be scaled in place into another type")
             starts, ends = np.concatenate((to, at[read])), np.concatenate((ends, (at + count * _BYTES[kind])[read]))
-        # runs of memory are apart where each ends, in order, before the next begins
+        # runs of memory are apart where each ends, in order, before the next begins (one of no bytes begins and ends between two)
         if (np.sort(ends)[:-1] > np.sort(starts)[1:]).any():
             n = len(to)
             if not _apart(zip(starts[:n].tolist(), ends[:n].tolist()), zip(starts[n:].tolist(), ends[n:].tolist())):
                 raise ValueError("the tensors that are written overlap one another or a gradient that is read")
-    table = np.empty((len(grads), 4), np.int64)  # rows of fdb_grad_tensor: two addresses, the count, both types
+    table = np.empty((len(at), 4), np.int64)  # rows of fdb_grad_tensor: two addresses, the count, both types
     table[:, 0], table[:, 1], table[:, 2], table[:, 3] = at, to, count, kind | into << 32
-    device, lib = grads[0].device, _lib.load()
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    p = _lib.ClipGradsParams(C.sizeof(_lib.ClipGradsParams), len(grads), table.ctypes.data, _NORMS[norm_type], int(outs is not None),
+    first, lib = grads.tensors[0], _lib.load()
+    device = first.device
+    norm = first.new_empty((), dtype=torch.float32)
+    p = _lib.ClipGradsParams(C.sizeof(_lib.ClipGradsParams), len(at), table.ctypes.data, _NORMS[norm_type], int(outs is not None),
                              max_norm, norm.data_ptr(), None, 0)
     with ops.on_device(device):
         need = lib.fdb_clip_grads_workspace_bytes(C.byref(p))
@@ -91,24 +110,9 @@ def _run(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], 
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
         _lib.check(lib.fdb_clip_grads(C.byref(p), ops.raw_stream(device)))
     if outs is not None:  # the write is seen by whoever compares versions (autograd, the caches of this package)
-        torch.autograd.graph.increment_version(outs)
+        torch.autograd.graph.increment_version(outs.tensors)
     ops._launches += 2
     return norm
-
-
-def _listed(grads: Tensors, what: str) -> List[torch.Tensor]:
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if not set(map(_layout, grads)) <= {torch.strided}:
-        raise TypeError(f"{what} takes dense tensors")
-    cards = set(map(_card, grads))
-    if -1 in cards:
-        raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
-    if len(cards) > 1:
-        raise ValueError(f"{what} takes tensors of one device, got {sorted(cards)}")
-    other = set(map(_dtype, grads)) - TYPES.keys()
-    if other:
-        raise TypeError(f"{what} takes bfloat16, float16 or float32 tensors, not {other.pop()}")
-    return grads
 
 
 def _norm_type(norm_type: float) -> float:
@@ -121,10 +125,12 @@ def _norm_type(norm_type: float) -> float:
 def grad_norm(grads: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm (1, 2 or inf) over all elements of the tensors taken as one vector: a float32 scalar on their device, zero where there
     are none.  Tensors are bfloat16, float16 or float32 in any mixture, of one device."""
-    norm_type, grads = _norm_type(norm_type), _listed(grads, "grad_norm")
-    if not grads:
+    norm_type, grads = _norm_type(norm_type), _Listed(grads, "grad_norm")
+    if not grads.tensors:
         return torch.tensor(0.0)
-    return _run([g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads], None, 0.0, norm_type)
+    if not grads.whole():
+        grads = _Listed([g if g.is_contiguous() or _dense(g) else g.detach().contiguous() for g in grads.tensors], "grad_norm")
+    return _run(grads, None, 0.0, norm_type)
 
 
 def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
@@ -132,26 +138,20 @@ def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out:
     shapes, of any of the three types: an optimizer's float32 buffers beside bfloat16 gradients), and returns the norm before.  Nothing
     is read back to the host.  Where the factor is one, tensors scaled in place are not written.  The tensors that are written must not
     overlap one another or, but for a tensor that is its own output, those that are read."""
-    norm_type, grads = _norm_type(norm_type), _listed(grads, "clip_grads_")
+    norm_type, grads = _norm_type(norm_type), _Listed(grads, "clip_grads_")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
-    outs = grads if out is None else _listed(out, "clip_grads_")
-    if out is not None and list(map(_shape, outs)) != list(map(_shape, grads)):
+    outs = grads if out is None else _Listed(out, "clip_grads_")
+    if out is not None and list(map(_shape, outs.tensors)) != list(map(_shape, grads.tensors)):
         raise ValueError("out must hold one tensor of the same shape for each gradient")
-    if not grads:
+    if not grads.tensors:
         return torch.tensor(0.0)
-    if outs[0].device != grads[0].device:
-        raise ValueError(f"out is on {outs[0].device}, the gradients on {grads[0].device}")
-    if not (all(map(_whole, grads)) and (out is None or all(map(_whole, outs)))):
-        return _clip_any(grads, outs, max_norm, norm_type)
-    if 0 in map(_count, grads):
-        keep = [i for i, g in enumerate(grads) if g.numel()]
-        if not keep:
-            return grads[0].new_zeros((), dtype=torch.float32)
-        outs = [outs[i] for i in keep]
-        grads = outs if out is None else [grads[i] for i in keep]
-    return _run(grads, outs, max_norm, norm_type)
+    if outs.tensors[0].device != grads.tensors[0].device:
+        raise ValueError(f"out is on {outs.tensors[0].device}, the gradients on {grads.tensors[0].device}")
+    if grads.whole() and (out is None or outs.whole()):
+        return _run(grads, outs, max_norm, norm_type)
+    return _clip_any(grads.tensors, outs.tensors, max_norm, norm_type)
 
 
 @torch.no_grad()
@@ -173,7 +173,7 @@ def _clip_any(grads, outs, max_norm, norm_type):
             back.append((o, writes[-1]))
     if not reads:
         return grads[0].new_zeros((), dtype=torch.float32)
-    norm = _run(reads, writes, max_norm, norm_type)
+    norm = _run(_Listed(reads, "clip_grads_"), _Listed(writes, "clip_grads_"), max_norm, norm_type)
     for o, scaled in back:
         o.copy_(scaled)
     return norm

@@ -65,6 +65,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         raise TypeError(f"quantize_int8 takes bfloat16, float16 or float32, not {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("quantize_int8 takes rows of at least one element")
+    if ops.intercepted(x):
+        raise RuntimeError("quantize_int8 goes by the memory of plain tensors: call it outside tracing, or linear_int8, which rounds within")
     cols = x.shape[-1]
     x = x if x.is_contiguous() else x.contiguous()
     q = torch.empty(*x.shape[:-1], _pitch(cols), dtype=torch.int8, device=x.device)[..., :cols]

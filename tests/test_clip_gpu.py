@@ -191,6 +191,11 @@ def test_refusals():
                      (lambda: ops.clip_grads_([a.expand(2, 100)], 1.0), (ValueError, RuntimeError))]:
         with pytest.raises(err):
             bad()
+    class Odd(torch.Tensor):
+        pass
+
+    with pytest.raises(TypeError, match="plain tensors"):
+        ops.grad_norm([a.as_subclass(Odd)])
     assert (a == 1).all() and (b == 1).all()
     assert abs(ops.grad_norm([a, a]).item() - math.sqrt(200)) < 1e-4  # (read twice, counted twice)
 

@@ -1,0 +1,107 @@
+"""The operators around the attention together, as an encoder layer uses them."""
+import copy
+import threading
+
+import pytest
+import torch
+
+from flashdeberta_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _block(h, f, seed, dtype):
+    g = torch.Generator().manual_seed(seed)
+    normal = lambda *s, std: (torch.randn(*s, generator=g) * std).to(DEV)
+    return {"wi": normal(f, h, std=h ** -0.5), "bi": normal(f, std=0.1).to(dtype), "wd": normal(h, f, std=f ** -0.5), "bd": normal(h, std=0.1).to(dtype),
+            "gamma": (1 + normal(h, std=0.1)).to(dtype), "beta": normal(h, std=0.1).to(dtype)}
+
+
+@pytest.mark.parametrize("rows,dtype", [(1, torch.bfloat16), (29, torch.float16), (777, torch.bfloat16)])
+def test_feed_forward_block_in_8_bits(rows, dtype):
+    """linear + GELU, linear, residual + LayerNorm, against the same block in float64 over unrounded weights.  8 bits of uniform steps leave
+    a product of random factors off by about (1/127) * amax / rms / sqrt(12) = 0.9 % of its size for each factor (amax of a few hundred
+    normal numbers is four times their rms): 1.3 % per layer, 1.9 % behind two, of values of order one that the LayerNorm keeps so."""
+    p = _block(512, 2048, rows, dtype)
+    x = torch.randn(rows, 512, generator=torch.Generator().manual_seed(rows + 1)).to(dtype).to(DEV)
+    wi, si = ops.quantize_int8(p["wi"])
+    wd, sd = ops.quantize_int8(p["wd"])
+    hidden = ops.linear_int8(x, wi, si, p["bi"], gelu=True)
+    out, stream = ops.residual_norm(ops.linear_int8(hidden, wd, sd, p["bd"]), x, p["gamma"], p["beta"], 1e-7)
+    d = {k: v.double() for k, v in p.items()}
+    want = torch.nn.functional.gelu(x.double() @ d["wi"].t() + d["bi"]) @ d["wd"].t() + d["bd"] + x.double()
+    normed = torch.nn.functional.layer_norm(want, (512,), d["gamma"], d["beta"], 1e-7)
+    assert ((stream.double() - want).norm() / want.norm()).item() < 0.02
+    assert ((out.double() - normed).norm() / normed.norm()).item() < 0.02
+    ops.check_status()
+
+
+def test_training_steps_against_float64():
+    """Three steps of gradient descent on a residual block with gated norms, its gradients clipped: parameters against the same steps in
+    float64 by torch.  fp32 throughout, so what differs is rounding: a few hundred operations of 2^-24 each way, 2^-15 of the largest."""
+    torch.manual_seed(0)
+    h = 96
+    mine = torch.nn.ParameterDict({
+        "w": torch.nn.Parameter(torch.randn(h, h) / h ** 0.5), "gate": torch.nn.Parameter(torch.rand(4, 1, h)),
+        "post": torch.nn.Parameter(1 + 0.1 * torch.randn(h)), "post_b": torch.nn.Parameter(0.1 * torch.randn(h)),
+        "gamma": torch.nn.Parameter(1 + 0.1 * torch.randn(h)), "beta": torch.nn.Parameter(0.1 * torch.randn(h))}).to(DEV)
+    theirs = copy.deepcopy(mine).double()
+    x, y = torch.randn(4, 30, h, device=DEV), torch.randn(4, 30, h, device=DEV)
+    prev = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        for _ in range(3):
+            out, stream = ops.residual_norm(x @ mine["w"].t(), x, mine["gamma"], mine["beta"], 1e-5, post_weight=mine["post"], post_bias=mine["post_b"],
+                                            gate=mine["gate"], residual_scale=0.9)
+            ((out - y).square().mean() + stream.square().mean()).backward()
+            u = torch.nn.functional.layer_norm(x.double() @ theirs["w"].t(), (h,), theirs["post"], theirs["post_b"], 1e-5)
+            s = 0.9 * x.double() + theirs["gate"] * u
+            o = torch.nn.functional.layer_norm(s, (h,), theirs["gamma"], theirs["beta"], 1e-5)
+            ((o - y.double()).square().mean() + s.square().mean()).backward()
+            got, want = ops.clip_grad_norm_(mine.parameters(), 0.05), torch.nn.utils.clip_grad_norm_(theirs.parameters(), 0.05)
+            assert abs(got.item() / want.item() - 1) < 2.0 ** -15
+            with torch.no_grad():
+                for a, b in zip(mine.parameters(), theirs.parameters()):
+                    a -= 10 * a.grad
+                    b -= 10 * b.grad
+                    a.grad = b.grad = None
+        for (n, a), b in zip(mine.items(), theirs.values()):
+            assert (a.double() - b).abs().max().item() <= 2.0 ** -15 * b.abs().max().item(), n
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = prev
+
+
+def test_host_threads_at_once():
+    """Four threads, each on its own stream, all operators: the results of one thread alone."""
+    p = _block(256, 768, 3, torch.bfloat16)
+    wi, si = ops.quantize_int8(p["wi"])
+    xs = [torch.randn(40 + 30 * i, 256, device=DEV, dtype=torch.bfloat16) for i in range(4)]
+
+    def work(x):
+        a = ops.linear_int8(x, wi, si, p["bi"], gelu=True)
+        n, s = ops.residual_norm(a[:, :256].contiguous(), x, p["gamma"], p["beta"])
+        out = [torch.empty_like(n, dtype=torch.float32), torch.empty_like(s, dtype=torch.float32)]
+        return [a, n, s, ops.clip_grads_([n, s], 0.5, out=out), *out]
+
+    want = [work(x) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = work(xs[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -114,6 +114,19 @@ def test_largest_integers(rows, k, n):
     assert torch.equal(out, want.expand(rows, n))
 
 
+@pytest.mark.parametrize("rows", [3, 200])
+def test_large_sums_through_the_gelu(rows):
+    """Sums on either side of 2^24, where the conversion rounds, scaled to the GELU's range."""
+    k, n = 4096, 72
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randint(100, 128, (rows, k), generator=g, dtype=torch.int8)
+    w = torch.randint(-128, 128, (n, 1), generator=g, dtype=torch.int8).expand(n, k).contiguous()
+    xs, ws = torch.rand(rows, generator=g) * 1e-4, torch.rand(n, generator=g) * 1e-3
+    for dtype in TYPES:
+        out = ops.linear_int8(x.to(DEV), w.to(DEV), ws.to(DEV), x_scale=xs.to(DEV), gelu=True, out_dtype=dtype)
+        _check(out, x, xs, w, ws, None, True)
+
+
 def test_random_integers_and_signs_of_every_size():
     g = torch.Generator().manual_seed(5)
     x = torch.randint(-128, 128, (150, 777), generator=g, dtype=torch.int8)
