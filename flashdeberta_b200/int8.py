@@ -120,12 +120,11 @@ def _call(x, weight, weight_scale, bias, x_scale, gelu, out_dtype):
     p = _PARAMS.pack(
         _PARAMS.size, kind, x_at, x_pitch, scale_at, w[0], w[1], weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
         out.data_ptr(), rows, k, n, 0 if bias is None else TYPES[bias.dtype], TYPES[out_dtype], gelu, 0, 0, 0, status)
-    with ops.on_device(device):
-        need = lib.fdb_linear_int8_workspace_bytes(p)
-        if need:  # the tokens as integers
-            ws = x.new_empty(need + 255, dtype=torch.uint8)
-            p = p[:-_PARAMS_TAIL.size] + _PARAMS_TAIL.pack((ws.data_ptr() + 255) & ~255, need, status)
-        _lib.check(lib.fdb_linear_int8(p, ops.raw_stream(device)))
+    need = lib.fdb_linear_int8_workspace_bytes(p)
+    if need:  # the tokens as integers
+        ws = x.new_empty(need + 255, dtype=torch.uint8)
+        p = p[:-_PARAMS_TAIL.size] + _PARAMS_TAIL.pack((ws.data_ptr() + 255) & ~255, need, status)
+    ops.call_on(device, lib.fdb_linear_int8, p)
     ops._launches += 1 + int(need > 0)
     return out
 

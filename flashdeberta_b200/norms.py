@@ -35,45 +35,58 @@ def _gate_rows(gate: torch.Tensor, shape) -> Optional[int]:
     return rows
 
 
-def _checked(x, residual, weight, bias, post_weight, post_bias, gate, rms):
-    """Raises on what the operator does not take; returns the gate as it is passed on (broadcast where it has to be)."""
-    shape, dtype, device = x.shape, x.dtype, x.device
+def _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms) -> Exception:
+    """What is wrong with a call that ``_gate_of`` does not take."""
+    shape, dtype = x.shape, x.dtype
     if not x.is_cuda:
-        raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
+        return RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
     if dtype not in TYPES:
-        raise TypeError(f"residual_norm takes bfloat16, float16 or float32 rows, not {dtype}")
+        return TypeError(f"residual_norm takes bfloat16, float16 or float32 rows, not {dtype}")
     if len(shape) < 1 or not 1 <= shape[-1] <= MAX_HIDDEN:
-        raise ValueError(f"residual_norm takes rows of 1 to {MAX_HIDDEN} elements")
-    if residual is not None:
-        if residual.shape != shape or residual.dtype != dtype:
-            raise ValueError("residual must match x in shape and dtype")
-        if residual.device != device:
-            raise ValueError(f"residual is on {residual.device}, x on {device}")
+        return ValueError(f"residual_norm takes rows of 1 to {MAX_HIDDEN} elements")
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype):
+        return ValueError("residual must match x in shape and dtype")
     if rms and (bias is not None or post_bias is not None):
-        raise ValueError("the RMS norm takes no bias")
+        return ValueError("the RMS norm takes no bias")
     if post_bias is not None and post_weight is None:
-        raise ValueError("post_bias needs post_weight")
-    vector, kind = shape[-1:], weight.dtype
-    for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
-        if t is None:
-            continue
-        if t.shape != vector:
-            raise ValueError(f"{name} must have shape {tuple(vector)}, got {tuple(t.shape)}")
-        if t.dtype != kind or (kind != dtype and kind != torch.float32):
-            raise TypeError(f"{name} must be {dtype} or float32, the norms' parameters all alike; got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, x on {device}")
+        return ValueError("post_bias needs post_weight")
+    named = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias}
+    for name, t in named.items():
+        if t is not None and t.shape != shape[-1:]:
+            return ValueError(f"{name} must have shape ({shape[-1]},), got {tuple(t.shape)}")
+        if t is not None and (t.dtype != weight.dtype or t.dtype not in (dtype, torch.float32)):
+            return TypeError(f"{name} must be {dtype} or float32, the norms' parameters all alike; got {t.dtype}")
+    for name, t in {"residual": residual, **named, "gate": gate}.items():
+        if t is not None and t.device != x.device:
+            return ValueError(f"{name} is on {t.device}, x on {x.device}")
+    if gate.dtype not in (dtype, torch.float32):
+        return TypeError(f"gate must be {dtype} or float32, got {gate.dtype}")
+    return ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+
+
+def _gate_of(x, residual, weight, bias, post_weight, post_bias, gate, rms):
+    """The gate as it is passed on (broadcast where it has to be); raises on what the operator does not take.  (Written for the calls that
+    go through: on a single token the checks take as long as anything else.)"""
+    shape, dtype, card, kind = x.shape, x.dtype, x.get_device(), weight.dtype
+    vector = shape[-1:]
+    if (card < 0 or dtype not in TYPES or len(shape) < 1 or not 1 <= shape[-1] <= MAX_HIDDEN
+            or weight.shape != vector or weight.get_device() != card or (kind != dtype and kind != torch.float32)
+            or (residual is not None and (residual.shape != shape or residual.dtype != dtype or residual.get_device() != card))):
+        raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms)
+    for t in (bias, post_weight, post_bias):
+        if t is not None and (t.shape != vector or t.dtype != kind or t.get_device() != card):
+            raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms)
+    if (rms and (bias is not None or post_bias is not None)) or (post_bias is not None and post_weight is None):
+        raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms)
     if gate is None:
         return None
-    if gate.dtype != dtype and gate.dtype != torch.float32:
-        raise TypeError(f"gate must be {dtype} or float32, got {gate.dtype}")
-    if gate.device != device:
-        raise ValueError(f"gate is on {gate.device}, x on {device}")
-    if gate.dim() == 0 or gate.dim() > len(shape) or _gate_rows(gate, shape) is None:  # shared in some other way: one per element then
+    if (gate.dtype != dtype and gate.dtype != torch.float32) or gate.get_device() != card or gate.dim() > len(shape):
+        raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms)
+    if gate.shape != vector and (gate.dim() == 0 or _gate_rows(gate, shape) is None):  # shared in some other way: one per element then
         try:
             return gate.expand(shape)
         except RuntimeError:
-            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
+            raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms) from None
     return gate
 
 
@@ -93,12 +106,17 @@ _BWD_TAIL = struct.Struct("@10PQ")
 
 def _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale) -> bytes:
     """fdb_residual_norm_params over contiguous tensors."""
-    shape = x.shape
+    shape, kind = x.shape, TYPES[x.dtype]
+    rows = x.numel() // shape[-1]
+    if gate is None:
+        gate_at = gate_rows = gate_kind = 0
+    else:
+        gate_at, gate_rows, gate_kind = gate.data_ptr(), rows if gate.dim() == 1 else _gate_rows(gate, shape), TYPES[gate.dtype]
     return _FWD.pack(
-        _FWD.size, TYPES[x.dtype], x.data_ptr(), _address(residual), weight.data_ptr(), _address(bias), _address(post_weight),
-        _address(post_bias), _address(gate), normed.data_ptr(), _address(stream), _address(stats), x.numel() // shape[-1],
-        0 if gate is None else _gate_rows(gate, shape), shape[-1], TYPES[weight.dtype], 0 if gate is None else TYPES[gate.dtype], rms,
-        residual_scale, eps)
+        _FWD.size, kind, x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if post_weight is None else post_weight.data_ptr(), 0 if post_bias is None else post_bias.data_ptr(), gate_at, normed.data_ptr(),
+        0 if stream is None else stream.data_ptr(), 0 if stats is None else stats.data_ptr(), rows, gate_rows, shape[-1], TYPES[weight.dtype],
+        gate_kind, rms, residual_scale, eps)
 
 
 def _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, residual_scale, keep):
@@ -110,9 +128,7 @@ def _forward(x, residual, weight, bias, post_weight, post_bias, gate, eps, rms, 
     if x.numel() == 0:
         return normed, stream, stats
     p = _params(x, residual, weight, bias, post_weight, post_bias, gate, normed, stream, stats, eps, rms, residual_scale)
-    device = x.device
-    with ops.on_device(device):
-        _lib.check(_lib.load().fdb_residual_norm(p, ops.raw_stream(device)))
+    ops.call_on(x.device, _lib.load().fdb_residual_norm, p)
     ops._launches += 1
     return normed, stream, stats
 
@@ -131,8 +147,8 @@ def _backward(dnormed, dstream, x, residual, weight, bias, post_weight, post_bia
     addresses = (_address(dnormed), _address(dstream), dx.data_ptr(), *map(_address, grads[1:]))
     with ops.on_device(device):
         need = lib.fdb_residual_norm_bwd_workspace_bytes(head + _BWD_TAIL.pack(*addresses, 0, 0))
-        ws = x.new_empty(need, dtype=torch.uint8)
-        _lib.check(lib.fdb_residual_norm_bwd(head + _BWD_TAIL.pack(*addresses, ws.data_ptr(), need), ops.raw_stream(device)))
+    ws = x.new_empty(need, dtype=torch.uint8)
+    ops.call_on(device, lib.fdb_residual_norm_bwd, head + _BWD_TAIL.pack(*addresses, ws.data_ptr(), need))
     ops._launches += 1 + int(any(g is not None for g in grads[2:]))
     return grads
 
@@ -216,10 +232,13 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: tor
     a gate of one.  ``residual`` may be None.  Rows are bfloat16, float16 or float32; the norms' parameters are of that type or all
     float32, the gate of either.  Statistics and sums are float32, every result is rounded once (``normed`` is made of the stream
     before it is rounded).  Gradients of every input, in the inputs' types; no second derivative."""
-    gate = _checked(x, residual, weight, bias, post_weight, post_bias, gate, rms)
-    call = (x, residual, weight, bias, post_weight, post_bias, gate, float(eps), bool(rms), float(residual_scale))
-    if ops.intercepted(*call[:7]):
-        return residual_norm_op(*call)[:2]
-    if ops.wants_grad(*call[:7]):
-        return _ResidualNorm.apply(*call)
-    return _forward(*call, False)[:2]
+    gate = _gate_of(x, residual, weight, bias, post_weight, post_bias, gate, rms)
+    tensors = (x, residual, weight, bias, post_weight, post_bias, gate)
+    eps, rms, residual_scale = float(eps), bool(rms), float(residual_scale)
+    if ops.intercepted(*tensors):
+        return residual_norm_op(*tensors, eps, rms, residual_scale)[:2]
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return _ResidualNorm.apply(*tensors, eps, rms, residual_scale)
+    return _forward(*tensors, eps, rms, residual_scale, False)[:2]

@@ -97,6 +97,18 @@ def raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
+def call_on(device: torch.device, entry, params) -> None:
+    """One C call with a device current, on its current stream; raises what it reports."""
+    card = torch._C._cuda_getDevice()
+    if device.index is None or device.index == card:
+        code = entry(params, torch._C._cuda_getCurrentRawStream(card))
+    else:
+        with torch.cuda.device(device):
+            code = entry(params, torch._C._cuda_getCurrentRawStream(device.index))
+    if code:
+        _lib.check(code)
+
+
 def global_module_hooks() -> bool:
     """Whether hooks on every module are registered (profilers, module trackers): modules have to be called one by one then."""
     m = _nn_module

@@ -314,6 +314,24 @@ def test_captured_step_is_replayed():
     assert all(torch.equal(a, b.detach()) for a, b in zip(kept, step()))
 
 
+def test_refusals():
+    t, _ = _inputs((2, 3, 64), torch.bfloat16, False, True, (64,), 20)
+    x, r, w, b, g = (t[k] for k in ("x", "residual", "weight", "bias", "gate"))
+    for bad, err in [
+            (lambda: ops.residual_norm(x.double(), None, w), TypeError), (lambda: ops.residual_norm(x, r[:1], w), ValueError),
+            (lambda: ops.residual_norm(x, r.float(), w), ValueError), (lambda: ops.residual_norm(x, r, w[:8]), ValueError),
+            (lambda: ops.residual_norm(x, r, w.half()), TypeError), (lambda: ops.residual_norm(x, r, w, b.float()), TypeError),
+            (lambda: ops.residual_norm(x, r, w, b, rms=True), ValueError), (lambda: ops.residual_norm(x, r, w, post_bias=b), ValueError),
+            (lambda: ops.residual_norm(x, r, w, post_weight=w[None]), ValueError), (lambda: ops.residual_norm(x, r, w, gate=g.double()), TypeError),
+            (lambda: ops.residual_norm(x, r, w, gate=g[:8]), ValueError), (lambda: ops.residual_norm(x, r, w, gate=x[:, :2]), ValueError),
+            (lambda: ops.residual_norm(x, r, w, gate=x[None]), ValueError), (lambda: ops.residual_norm(x, r, w.cpu()), ValueError),
+            (lambda: ops.residual_norm(x, r.cpu(), w), ValueError), (lambda: ops.residual_norm(x, r, w, gate=g.cpu()), ValueError),
+            (lambda: ops.residual_norm(torch.zeros(2, 8193, device=DEV), None, torch.zeros(8193, device=DEV)), ValueError),
+            (lambda: ops.residual_norm(x[..., :0], None, w[:0]), ValueError)]:
+        with pytest.raises(err):
+            bad()
+
+
 def test_in_a_layer_beside_add_layernorm():
     """The tail of this package's own output blocks: the same result as ops.add_layernorm up to the sum that it rounds first."""
     t, _ = _inputs((64, 768), torch.bfloat16, False, False, None, 18)
