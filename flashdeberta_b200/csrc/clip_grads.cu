@@ -61,7 +61,7 @@ __device__ __forceinline__ void load_chunk(const T* p, int64_t left, bool wide, 
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     const int64_t at = (int64_t)i * kThreads * kRowElems;
-    const RowColumns<false> cols{(int)threadIdx.x, kThreads, (int)max((int64_t)0, min(left - at, (int64_t)kThreads * kRowElems))};
+    const RowColumns<kRowSingle> cols{(int)threadIdx.x, kThreads, (int)max((int64_t)0, min(left - at, (int64_t)kThreads * kRowElems))};
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int j = 0; j < kRowElems; ++j) r[i].w[j] = cols.live(j) ? reinterpret_cast<const uint32_t*>(p + at)[cols.col(j)] : 0u;
@@ -86,7 +86,7 @@ __device__ __forceinline__ void store_vector(T* p, int64_t left, bool wide, int 
     return;
   }
   const int64_t at = (int64_t)i * kThreads * kRowElems;
-  const RowColumns<false> cols{(int)threadIdx.x, kThreads, (int)max((int64_t)0, min(left - at, (int64_t)kThreads * kRowElems))};
+  const RowColumns<kRowSingle> cols{(int)threadIdx.x, kThreads, (int)max((int64_t)0, min(left - at, (int64_t)kThreads * kRowElems))};
   cols.store(p + at, r);
 }
 

@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(kThreads) linear_int8_small_kernel(const __gri
       const X* x = static_cast<const X*>(a.x) + (int64_t)(has ? r : 0) * a.k;
       auto load = [&](int at, RowWords<X, V>& w) {
         const int left = max(0, min(span, a.k - at));
-        if (a.wide) RowColumns<true, V>{lane, 32, left}.load(x + at, w);
-        else RowColumns<false, V>{lane, 32, left}.load(x + at, w);
+        if (a.wide) RowColumns<kRowWide, V>{lane, 32, left}.load(x + at, w);
+        else RowColumns<kRowSingle, V>{lane, 32, left}.load(x + at, w);
       };
       RowWords<X, V> first, w;
       uint32_t top = 0;
@@ -136,12 +136,12 @@ __global__ void __launch_bounds__(kThreads) linear_int8_small_kernel(const __gri
         for (int j = 0; j < V * kRowElems; j += kRowElems) {
           const uint2 o = make_uint2(four_bytes(v + j, by.inv), four_bytes(v + j + 4, by.inv));
           if (a.wide) {
-            const int c = RowColumns<true, V>{lane, 32, 0}.col(j);
+            const int c = RowColumns<kRowWide, V>{lane, 32, 0}.col(j);
             if (c < room) *reinterpret_cast<uint2*>(s + c) = o;
           } else {
 #pragma unroll
             for (int i = 0; i < kRowElems; ++i) {
-              const int c = RowColumns<false, V>{lane, 32, 0}.col(j + i);
+              const int c = RowColumns<kRowSingle, V>{lane, 32, 0}.col(j + i);
               if (c < room) s[c] = (uint8_t)((i < 4 ? o.x : o.y) >> (8 * (i % 4)));
             }
           }

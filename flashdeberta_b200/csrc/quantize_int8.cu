@@ -16,22 +16,13 @@ namespace {
 
 constexpr int kThreads = 128, kWarpElems = 1024;
 
-// Columns of a row that starts anywhere: runs of four per thread, so that what they become is stored four bytes at a time.
+// Columns of an fp32 row that starts anywhere: runs of four per thread, so that what they become is stored four bytes at a time.
 template <int V> struct QuadColumns {
   int t, threads, hidden;
   __device__ __forceinline__ int col(int j) const { return (t + j / 4 * threads) * 4 + j % 4; }
-  template <typename T> __device__ __forceinline__ void load(const T* row, RowWords<T, V>& r) const {
-    if constexpr (sizeof(T) == 4) {
+  __device__ __forceinline__ void load(const float* row, RowWords<float, V>& r) const {
 #pragma unroll
-      for (int j = 0; j < V * kRowElems; ++j) r.w[j] = col(j) < hidden ? __ldg(reinterpret_cast<const uint32_t*>(row) + col(j)) : 0u;
-    } else {
-      const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
-#pragma unroll
-      for (int j = 0; j < V * kRowElems; j += 2) {
-        const uint32_t lo = col(j) < hidden ? __ldg(p + col(j)) : 0u, hi = col(j + 1) < hidden ? __ldg(p + col(j + 1)) : 0u;
-        r.w[j / 2] = lo | (hi << 16);
-      }
-    }
+    for (int j = 0; j < V * kRowElems; ++j) r.w[j] = col(j) < hidden ? __ldg(reinterpret_cast<const uint32_t*>(row) + col(j)) : 0u;
   }
 };
 
@@ -46,7 +37,8 @@ struct QuantArgs {
 template <typename T, bool WIDE, int V>
 __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constant__ QuantArgs a) {
   constexpr int kElems = V * kRowElems;
-  using Columns = std::conditional_t<WIDE, RowColumns<true, V>, QuadColumns<V>>;
+  constexpr bool kPieces = WIDE || sizeof(T) == 2;  // of eight elements
+  using Columns = std::conditional_t<kPieces, RowColumns<row_mode<T>(WIDE), V>, QuadColumns<V>>;
   __shared__ uint32_t s_top[kThreads / 32][8];
   const int team = threadIdx.x / a.team_threads, t = threadIdx.x - team * a.team_threads;
   const int warps = a.team_threads / 32, span = a.team_threads * kElems;
@@ -85,9 +77,9 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const __grid_constan
 #pragma unroll
       for (int j = 0; j < kElems; j += kRowElems) {
         const uint2 o = make_uint2(four_bytes(v + j, by.inv), four_bytes(v + j + 4, by.inv));
-        if constexpr (WIDE) {
+        if constexpr (kPieces) {  // (up to seven zeros behind the row)
           if (cols.live(j)) *reinterpret_cast<uint2*>(y + cols.col(j)) = o;
-        } else {  // (up to three zeros behind the row)
+        } else {
           if (cols.col(j) < cols.hidden) *reinterpret_cast<uint32_t*>(y + cols.col(j)) = o.x;
           if (cols.col(j + 4) < cols.hidden) *reinterpret_cast<uint32_t*>(y + cols.col(j + 4)) = o.y;
         }

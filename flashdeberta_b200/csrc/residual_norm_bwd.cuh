@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
   __shared__ __align__(16) float s_sums[kNormBwdTeams][TeamSum<kSums>::kSlots];
   const ResidualNormArgs& f = b.f;
   const int team = threadIdx.x / f.team_threads, t = threadIdx.x - team * f.team_threads;
-  const RowColumns<WIDE> cols{t, f.team_threads, f.hidden};
+  const RowColumns<row_mode<T>(WIDE)> cols{t, f.team_threads, f.hidden};
   TeamSum<kSums> team_sum{s_sums[team], f.team_threads / 32, t >> 5, team + 1, 0};
   const float inv_hidden = 1.f / (float)f.hidden;
   const int64_t worker = (int64_t)blockIdx.x * f.teams + team;
@@ -51,8 +51,8 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     if (element_gate) cols.load(static_cast<const T*>(f.gate) + at, r.gate);
     r.stats = __ldg(f.stats + row);
   };
-  // the next row is on its way while one is worked on, where registers allow it (fp32 rows and 1024 threads do not; single elements are
-  // put into words at once)
+  // the next row is on its way while one is worked on, where registers allow it (fp32 rows and 1024 threads do not; single
+  // elements and shifted pieces are put into words at once)
   constexpr bool kAhead = sizeof(T) == 2 && WIDE && THREADS <= kNormBwdThreads;
   Row now, next;
   if (kAhead && first < end) fetch(first, now);
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     __syncthreads();
     const int all = f.team_threads * kRowElems;
     for (int i = threadIdx.x; i < all; i += blockDim.x) {
-      const int c = WIDE ? i : (i % kRowElems) * f.team_threads + i / kRowElems;
+      const int c = row_mode<T>(WIDE) != kRowSingle ? i : (i % kRowElems) * f.team_threads + i / kRowElems;
       float sum = 0.f;
       for (int k = 0; k < f.teams; ++k) sum += s_team[k * all + i];
       if (c < f.hidden) part[(int64_t)vector * f.hidden + c] = sum;

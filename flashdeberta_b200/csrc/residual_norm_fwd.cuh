@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ct
   __shared__ __align__(16) float s_sums[ONE ? 1 : kNormFwdThreads / 64][TeamSum<1>::kSlots];
   const int threads = ONE ? 32 : a.team_threads;
   const int team = ONE ? threadIdx.x >> 5 : threadIdx.x / threads, t = ONE ? threadIdx.x & 31 : threadIdx.x - team * threads;
-  const RowColumns<WIDE, V> cols{t, threads, a.hidden};
+  const RowColumns<row_mode<T>(WIDE), V> cols{t, threads, a.hidden};
   TeamSum<1> team_sum{s_sums[ONE ? 0 : team], threads / 32, t >> 5, team + 1, 0};
   const float inv_hidden = 1.f / (float)a.hidden;
 
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ct
   };
   const int64_t step = (int64_t)gridDim.x * a.teams;
   int64_t row = (int64_t)blockIdx.x * a.teams + team;
-  constexpr bool kAhead = sizeof(T) == 2 && WIDE;  // (fp32 rows would take too many registers, single elements are put into words at once)
+  constexpr bool kAhead = sizeof(T) == 2 && WIDE;  // (fp32 rows would take too many registers, single elements and shifted pieces are put into words at once)
   if (kAhead && row < a.rows) fetch(row, nx, nr);
 
   // vectors over the columns: 16-byte pieces, each piece of the team's threads side by side

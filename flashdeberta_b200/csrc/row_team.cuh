@@ -1,7 +1,7 @@
 // Rows of activations held by teams of warps: eight elements of a row per thread, or V times eight; sums over the team.
 //
-// Where eight elements may be read in one piece (WIDE: hidden a multiple of 8, pointers aligned to eight elements) thread t holds columns
-// 8 (t + i threads) .. + 7, i < V; otherwise columns t + j threads, j < 8 V, so that the lanes of a warp still read neighbours.
+// Where rows are read in pieces of eight, thread t holds columns 8 (t + i threads) .. + 7, i < V; otherwise columns t + j threads, j < 8 V, so
+// that the lanes of a warp still read neighbours.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -88,19 +88,37 @@ __device__ __forceinline__ float fold(uint64_t v) {  // the sum of a pair
   return lo + hi;
 }
 
+// How rows are read and written: single elements (fp32 that starts anywhere), pieces of eight (WIDE: every row starts on a piece), pieces
+// of eight 16-bit elements that start anywhere (SHIFTED: two aligned 16-byte pieces are loaded and moved into place; on the way
+// out neighbouring lanes put aligned pieces together, and only the ends of a warp's run are written element by element).
+enum : int { kRowSingle = 0, kRowWide = 1, kRowShifted = 2 };
+template <typename T> constexpr int row_mode(bool wide) { return wide ? kRowWide : (sizeof(T) == 2 ? kRowShifted : kRowSingle); }
+
+// Four words from byte `at` < 16 of eight.  (Selects, not branches: loads that come later can be issued before the words are there.)
+__device__ __forceinline__ void shifted(const uint32_t (&c)[8], uint32_t at, uint32_t (&w)[4]) {
+  uint32_t d[6], e[5];
+#pragma unroll
+  for (int k = 0; k < 6; ++k) d[k] = (at & 8u) != 0u ? c[k + 2] : c[k];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) e[k] = (at & 4u) != 0u ? d[k + 1] : d[k];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(e[k], e[k + 1], (at & 3u) * 8u);
+}
+
 // Which columns of a row a thread holds.
-template <bool WIDE, int V = 1> struct RowColumns {
+template <int MODE, int V = 1> struct RowColumns {
   static constexpr int kElems = V * kRowElems;
-  int t, threads, hidden;  // thread and threads of the team
+  int t, threads, hidden;  // thread and threads of the team (whole warps)
 
   __device__ __forceinline__ int col(int j) const {
-    return WIDE ? (t + j / kRowElems * threads) * kRowElems + j % kRowElems : j * threads + t;
+    if (MODE == kRowShifted) return (((t >> 5) * V + j / kRowElems) * 32 + (t & 31)) * kRowElems + j % kRowElems;
+    return MODE == kRowWide ? (t + j / kRowElems * threads) * kRowElems + j % kRowElems : j * threads + t;
   }
-  __device__ __forceinline__ bool live(int j) const { return col(WIDE ? j / kRowElems * kRowElems : j) < hidden; }
+  __device__ __forceinline__ bool live(int j) const { return col(MODE == kRowWide ? j / kRowElems * kRowElems : j) < hidden; }
 
   // The thread's elements of a row; zeros behind its end.
   template <typename T> __device__ __forceinline__ void load(const T* row, RowWords<T, V>& r) const {
-    if constexpr (WIDE) {
+    if constexpr (MODE == kRowWide) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const T* p = row + col(i * kRowElems);
@@ -119,6 +137,23 @@ template <bool WIDE, int V = 1> struct RowColumns {
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int j = 0; j < kElems; ++j) r.w[j] = live(j) ? __ldg(reinterpret_cast<const uint32_t*>(row) + col(j)) : 0u;
+    } else if constexpr (MODE == kRowShifted) {
+      const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;  // bytes; the same for every piece
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c0 = col(i * kRowElems), have = hidden - c0;
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + c0) - shift);
+        // (an aligned piece with an element of the row in it never leaves the allocation)
+        uint4 q = make_uint4(0, 0, 0, 0), n = q;
+        if (have > 0) q = __ldg(p);
+        if (2 * min(have, kRowElems) > 16 - (int)shift) n = __ldg(p + 1);
+        const uint32_t c[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
+        uint32_t* w = r.w + i * 4;
+        shifted(c, shift, *reinterpret_cast<uint32_t(*)[4]>(w));
+        if (have < kRowElems)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = 2 * k + 1 < have ? w[k] : (2 * k < have ? w[k] & 0xffffu : 0u);
+      }
     } else {
       const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
 #pragma unroll
@@ -128,8 +163,18 @@ template <bool WIDE, int V = 1> struct RowColumns {
       }
     }
   }
+  // Bytes from <= b < to of an aligned piece (both even): whole words, and the half ones at the ends.
+  static __device__ __forceinline__ void ends(char* p, const uint32_t (&o)[4], int from, int to) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (4 * k >= from && 4 * k + 4 <= to) *reinterpret_cast<uint32_t*>(p + 4 * k) = o[k];
+    auto word = [&](int k) { return k < 2 ? (k == 0 ? o[0] : o[1]) : (k == 2 ? o[2] : o[3]); };
+    if ((from & 2) != 0) *reinterpret_cast<unsigned short*>(p + from) = (unsigned short)(word(from >> 2) >> 16);
+    if ((to & 2) != 0 && to - 2 >= from) *reinterpret_cast<unsigned short*>(p + to - 2) = (unsigned short)word(to >> 2);
+  }
+  // (SHIFTED: by all lanes of a warp)
   template <typename T> __device__ __forceinline__ void store(T* row, const RowWords<T, V>& r) const {
-    if constexpr (WIDE) {
+    if constexpr (MODE == kRowWide) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         if (!live(i * kRowElems)) continue;
@@ -140,6 +185,41 @@ template <bool WIDE, int V = 1> struct RowColumns {
 #pragma unroll
       for (int j = 0; j < kElems; ++j)
         if (live(j)) reinterpret_cast<uint32_t*>(row)[col(j)] = r.w[j];
+    } else if constexpr (MODE == kRowShifted) {
+      // The warp's run: 32 V pieces from column c0 on, `bytes` of them in the row.  Aligned piece b begins 16 b - shift into the run, the end of
+      // one lane's piece and the beginning of the next lane's; a lane keeps one that is not whole for the end (the first of the run and
+      // the last of the row).
+      const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+      const int lane = t & 31, c0 = (t >> 5) * V * 256, bytes = min(512 * V, 2 * (hidden - c0));
+      char* run = reinterpret_cast<char*>(row + c0);
+      uint32_t before[4] = {0u, 0u, 0u, 0u}, part[4] = {0u, 0u, 0u, 0u};  // lane 0: what lane 31 had; the piece that is kept
+      int part_at = -16;
+#pragma unroll
+      for (int i = 0; i <= V; ++i) {
+        uint32_t c[8], o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          c[k + 4] = i < V ? r.w[i < V ? i * 4 + k : 0] : 0u;
+          const uint32_t left = i < V ? __shfl_sync(0xffffffffu, c[k + 4], (lane + 31) & 31) : 0u;
+          c[k] = lane == 0 ? before[k] : left;
+          before[k] = left;
+        }
+        shifted(c, 16u - shift, o);
+        if (shift == 0u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = c[k + 4];
+        const int at = 16 * (32 * i + lane) - (int)shift;
+        if (i == V && lane != 0) continue;
+        if (at >= 0 && at + 16 <= bytes) {
+          *reinterpret_cast<uint4*>(run + at) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else if (at < bytes && at + 16 > 0) {
+          if (part_at > -16) ends(run + part_at, part, max(0, -part_at), min(16, bytes - part_at));  // (a lane that has both)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) part[k] = o[k];
+          part_at = at;
+        }
+      }
+      if (part_at > -16) ends(run + part_at, part, max(0, -part_at), min(16, bytes - part_at));
     } else {
       unsigned short* p = reinterpret_cast<unsigned short*>(row);
 #pragma unroll
@@ -171,7 +251,7 @@ template <bool WIDE, int V = 1> struct RowColumns {
   }
   // a number where the row has columns, zero behind its end
   __device__ __forceinline__ uint64_t inside(int pair, float v) const {
-    return WIDE ? both(live(2 * pair) ? v : 0.f) : ptx::pack_f32x2(live(2 * pair) ? v : 0.f, live(2 * pair + 1) ? v : 0.f);
+    return MODE == kRowWide ? both(live(2 * pair) ? v : 0.f) : ptx::pack_f32x2(live(2 * pair) ? v : 0.f, live(2 * pair + 1) ? v : 0.f);
   }
   // a vector over the columns, either of the rows' type or fp32
   template <typename T, typename F> __device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at, F& v) const {

@@ -360,3 +360,47 @@ def test_tracing_and_batched_gradients():
     one = torch.autograd.grad(_call(t)[0], [t["x"], t["weight"]], grads[0])
     for a, b in zip(got, one):
         assert torch.equal(a[0], b) and torch.equal(a[1], 2 * b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hidden", [1, 5, 9, 250, 257, 263, 767, 1023, 1027, 2050, 4099])
+def test_16_bit_rows_that_start_anywhere(dtype, hidden):
+    """Every shift of a row against 16 bytes, in results and gradients, with what lies around the tensors left alone."""
+    for off in range(0, 8, 1 if hidden < 300 else 3):
+        t, grads = _inputs((3, 5, hidden), dtype, False, True, (3, 5, hidden), hidden + off)
+        want, bound = _want(t, grads, 1e-5, False, 1.0)
+        hold = {}
+        for k in ("x", "residual", "gate"):
+            hold[k] = torch.full((15 * hidden + 24,), 9.0, dtype=dtype, device=DEV)
+            v = hold[k][8 + off:8 + off + 15 * hidden].view(3, 5, hidden)
+            v.copy_(t[k])
+            t[k] = v
+        for k in NAMES:
+            t[k].requires_grad_()
+        n, s = _call(t)
+        got = torch.autograd.grad((n, s), [t[k] for k in NAMES], grads)
+        _check("normed", n.detach(), want["normed"], bound["normed"])
+        _check("stream", s.detach(), want["stream"], bound["stream"])
+        for k, a in zip(NAMES, got):
+            _check("d" + k, a, want[k], bound[k])
+        for k, h in hold.items():
+            assert (h[:8 + off] == 9).all() and (h[8 + off + 15 * hidden:] == 9).all()
+
+
+def test_results_end_where_they_end():
+    """Through the C entry, into the middle of larger buffers, at every shift."""
+    import ctypes as C
+    from flashdeberta_b200 import _lib
+    for dtype, kind in ((torch.bfloat16, 0), (torch.float16, 3), (torch.float32, 1)):
+        for rows, hidden in ((1, 3), (4, 33), (3, 515), (2, 1030)):
+            t, _ = _inputs((rows, hidden), dtype, True, False, None, 30)
+            want = ops.residual_norm(t["x"], t["residual"], t["weight"], eps=1e-5, rms=True)
+            for off in range(8):
+                out = [torch.full((rows * hidden + 32,), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+                at = [o.data_ptr() + (16 + off) * o.element_size() for o in out]
+                p = _lib.ResidualNormParams(C.sizeof(_lib.ResidualNormParams), kind, t["x"].data_ptr(), t["residual"].data_ptr(), t["weight"].data_ptr(), None, None,
+                                            None, None, at[0], at[1], None, rows, 0, hidden, kind, 0, 1, 1.0, 1e-5)
+                _lib.check(_lib.load().fdb_residual_norm(C.byref(p), ops.raw_stream(t["x"].device)))
+                for o, w in zip(out, want):
+                    assert (o[:16 + off] == 7).all() and (o[16 + off + rows * hidden:] == 7).all()
+                    assert torch.equal(o[16 + off:16 + off + rows * hidden].view(rows, hidden), w)
