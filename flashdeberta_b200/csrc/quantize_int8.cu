@@ -2,6 +2,7 @@
 //
 // A warp per row of up to 1024 elements, up to eight warps beyond (row_team.cuh); a row of up to 8192 is read once and stays in
 // registers, a longer one is read a second time (it comes from L2 then).  HBM-bound: x read, one byte per element written.
+// 16384 x 1024 bf16: 11.4 us = 4.4 TB/s.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -77,17 +77,17 @@ inline int make_map_bytes(CUtensorMap* m, const void* base, int64_t rows, int co
   return FDB_OK;
 }
 
-// (rows, cols) elements of 2 or 4 bytes, contiguous -> 2-D map (col, row), box `width` (64 or 128) bytes x box_rows, swizzle of that width
-inline int make_map_out(CUtensorMap* m, void* base, int64_t rows, int cols, CUtensorMapDataType type, int bytes, int width, int box_rows,
+// (rows, cols) elements of 2 or 4 bytes, contiguous -> 2-D map (col, row), box 64 bytes x box_rows, 64-byte swizzle
+inline int make_map_out(CUtensorMap* m, void* base, int64_t rows, int cols, CUtensorMapDataType type, int bytes, int box_rows,
                         const char* what) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(FDB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)cols * bytes};
-  const cuuint32_t box[2] = {(cuuint32_t)(width / bytes), (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {64u / (cuuint32_t)bytes, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = fn(m, type, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FDB_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, (int)r);
   return FDB_OK;
 }
