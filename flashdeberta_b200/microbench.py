@@ -14,6 +14,11 @@ times the fused residual + LayerNorm kernel instead (algorithmic bytes: 3 * rows
 
 times the fused linear + GELU kernel (2 * rows * hidden * out_features FLOP) beside torch's linear followed by gelu.
 
+    python -m flashdeberta_b200.microbench --residual-norm | --linear-int8 | --clip-grads  [--rows --hidden --out-features]
+
+times ops.residual_norm (LayerNorms on both sides and a gate per channel, forward and forward + backward), ops.linear_int8 (GELU, tokens rounded
+within the call) or ops.clip_grads_ (rows x hidden gradients in bf16 into float32 buffers).
+
     python -m flashdeberta_b200.microbench --reference-triton --batch 8 --seq 2048
 
 times the reference's own attention path on the same GPU and the same q, k, v: the two bias GEMMs of
@@ -61,6 +66,64 @@ def bench_add_layernorm(rows: int, hidden: int, iters: int, warmup: int, sets: i
     print(json.dumps({"op": "add_layernorm", "rows": rows, "hidden": hidden, "ms_median": med, "ms_min": mn,
                       "gbs_median": nbytes / med / 1e6, "gbs_best": nbytes / mn / 1e6, "bytes": nbytes,
                       "l2": f"{sets} buffer sets rotated ({sets * 3 * rows * hidden * 2 >> 20} MiB; the output is allocated per call)"}))
+
+
+def _timed(fns, iters: int, warmup: int):
+    """Median and best ms of calls taken in turn."""
+    for i in range(warmup):
+        fns[i % len(fns)]()
+    torch.cuda.synchronize()
+    times = []
+    for i in range(iters):
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        fns[i % len(fns)]()
+        e1.record()
+        torch.cuda.synchronize()
+        times.append(e0.elapsed_time(e1))
+    return statistics.median(times), min(times)
+
+
+def bench_residual_norm(rows: int, hidden: int, iters: int, warmup: int, sets: int):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    fns, steps = [], []
+    for _ in range(sets):
+        x, r, dn, ds = (torch.randn(rows, hidden, generator=g, device="cuda").bfloat16() for _ in range(4))
+        w, b, gate = (torch.rand(hidden, generator=g, device="cuda").bfloat16() for _ in range(3))
+
+        def call(x=x, r=r, w=w, b=b, gate=gate):
+            return ops.residual_norm(x, r, w, b, post_weight=w, post_bias=b, gate=gate)
+
+        def step(call=call, leaves=[t.clone().requires_grad_() for t in (x, r, w, b, gate)], grads=(dn, ds)):
+            return torch.autograd.grad(call(*leaves), leaves, grads)
+
+        fns.append(call)
+        steps.append(step)
+    for name, f, passes in (("residual_norm", fns, 4), ("residual_norm forward + backward", steps, 10)):
+        med, mn = _timed(f, iters, warmup)
+        print(json.dumps({"op": name, "rows": rows, "hidden": hidden, "ms_median": med, "ms_min": mn, "gbs_median": passes * rows * hidden * 2 / med / 1e6,
+                          "bytes": passes * rows * hidden * 2, "l2": f"{sets} input sets rotated"}))
+
+
+def bench_linear_int8(rows: int, k: int, n: int, iters: int, warmup: int, sets: int):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w, scale = ops.quantize_int8(torch.randn(n, k, generator=g, device="cuda") * 0.02)
+    b = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    xs = [torch.randn(rows, k, generator=g, device="cuda").bfloat16() for _ in range(sets)]
+    med, mn = _timed([lambda x=x: ops.linear_int8(x, w, scale, b, gelu=True) for x in xs], iters, warmup)
+    ops.check_status()
+    print(json.dumps({"op": "linear_int8", "rows": rows, "in_features": k, "out_features": n, "ms_median": med, "ms_min": mn,
+                      "tops_median": 2 * rows * k * n / med / 1e9, "l2": f"{sets} input sets rotated"}))
+
+
+def bench_clip_grads(rows: int, hidden: int, iters: int, warmup: int):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    grads = [torch.randn(rows // 16, hidden, generator=g, device="cuda").bfloat16() for _ in range(16)]
+    out = [torch.empty_like(t, dtype=torch.float32) for t in grads]
+    med, mn = _timed([lambda: ops.clip_grads_(grads, 1.0, out=out)], iters, warmup)
+    count = sum(t.numel() for t in grads)
+    print(json.dumps({"op": "clip_grads_", "elements": count, "ms_median": med, "ms_min": mn, "gbs_median": 8 * count / med / 1e6,
+                      "bytes": 8 * count, "l2": f"{6 * count >> 20} MiB in one set"}))
 
 
 def bench_linear_gelu(rows: int, k: int, n: int, iters: int, warmup: int, sets: int):
@@ -306,6 +369,9 @@ def main():
     ap.add_argument("--valid", type=int, default=0, help="valid length of every sequence (default: all)")
     ap.add_argument("--add-layernorm", action="store_true", help="time fdb_add_layernorm instead of the attention")
     ap.add_argument("--linear-gelu", action="store_true", help="time fdb_linear_gelu (rows x hidden -> out-features)")
+    ap.add_argument("--residual-norm", action="store_true", help="time ops.residual_norm and its backward")
+    ap.add_argument("--linear-int8", action="store_true", help="time ops.linear_int8 (rows x hidden -> out-features)")
+    ap.add_argument("--clip-grads", action="store_true", help="time ops.clip_grads_ (rows x hidden gradients)")
     ap.add_argument("--eager-gpu", action="store_true",
                     help="time transformers' eager attention module on the GPU (fp32, bf16) beside this package's module")
     ap.add_argument("--reference-triton", action="store_true",
@@ -323,6 +389,12 @@ def main():
         return bench_reference_triton(args.batch, args.seq, args.heads, args.iters, args.warmup, args.sets)
     if args.linear_gelu:
         return bench_linear_gelu(args.rows, args.hidden, args.out_features, args.iters, args.warmup, args.sets)
+    if args.residual_norm:
+        return bench_residual_norm(args.rows, args.hidden, args.iters, args.warmup, args.sets)
+    if args.linear_int8:
+        return bench_linear_int8(args.rows, args.hidden, args.out_features, args.iters, args.warmup, args.sets)
+    if args.clip_grads:
+        return bench_clip_grads(args.rows, args.hidden, args.iters, args.warmup)
     if args.add_layernorm:
         return bench_add_layernorm(args.rows, args.hidden, args.iters, args.warmup, max(args.sets, 8))
     dev = torch.device("cuda")
