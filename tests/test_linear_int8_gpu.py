@@ -29,8 +29,8 @@ def _quantized(x):
     return torch.from_numpy(q).view(x.shape), torch.from_numpy(scale).view(x.shape[:-1])
 
 
-def _check(out, xq, xs, wq, ws, bias, gelu):
-    acc = xq.double().cpu() @ wq.double().cpu().t()
+def _check(out, xq, xs, wq, ws, bias, gelu, acc=None):
+    acc = xq.double().cpu() @ wq.double().cpu().t() if acc is None else acc
     scaled = acc * ws.double().cpu() * xs.double().cpu()[..., None]
     b = 0.0 if bias is None else bias.double().cpu()
     v = scaled + b
@@ -99,6 +99,28 @@ def test_product(rows, k, n, dtype):
         _check(out, xq, xs, wq, ws, b, gelu)
         given = ops.linear_int8(xq, wq, ws, b, x_scale=xs, gelu=gelu, out_dtype=dtype)
         assert torch.equal(given, out)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("rows,k,n", [(40, 1, 8), (100, 3, 40), (64, 96, 8), (50, 64, 1), (33, 17, 4), (90, 130, 12)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product_of_few_features(rows, k, n, dtype):
+    x, wq, ws, b = _problem(rows, k, n, dtype, dtype, rows + k + n)
+    xq, xs = ops.quantize_int8(x)
+    _check(ops.linear_int8(x, wq, ws, b), xq, xs, wq, ws, b, False)
+    _check(ops.linear_int8(xq, wq, ws, b, x_scale=xs, out_dtype=dtype, gelu=True), xq, xs, wq, ws, b, True)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("n", [1104, 1101, 1028])
+@pytest.mark.parametrize("rows,k", [(9001, 2000), (5003, 300)])
+def test_product_of_many_tiles(rows, k, n):
+    """Every accumulator and stage used many times over, tiles that end inside the matrix, in every form of the store."""
+    for dtype, gelu in ((torch.bfloat16, True), (torch.float32, False)):
+        x, wq, ws, b = _problem(rows, k, n, dtype, torch.float32, n)
+        xq, xs = ops.quantize_int8(x)
+        acc = (xq.double() @ wq.double().t()).cpu()
+        _check(ops.linear_int8(x, wq, ws, b, gelu=gelu), xq, xs, wq, ws, b, gelu, acc)
     ops.check_status()
 
 
