@@ -5,11 +5,11 @@
 // (CG = 1) or 256 rows (CG = 2, a pair of CTAs on two SMs) x BN output features, K in steps of 128 bytes through a ring of stages:
 //   warp 0  TMA, the CTA's 128 x 128 bytes of x and its BN / CG rows of the weight; what lies behind the ends arrives as zeros
 //   warp 1  (of the pair's even CTA) tcgen05.mma, four per stage; two accumulators in tensor memory
-//   the other warps (16, or 8 for BN = 64): epilogue, 64 or 32 columns of 32 rows each: both scales, bias, activation in fp32, one
-//           rounding, a TMA store.  Scales and biases of the next tile are fetched while one is worked on.
+//   the other warps: epilogue, 32 rows and 128, 64 or 32 columns each: both scales, bias, activation in fp32, one rounding, a TMA
+//           store.  Scales and biases of the next tile are fetched while one is worked on.
 // Bound by the tensor cores at the power limit where K is long, by the epilogue where it is short (4800 clocks a 256 x 256 tile, with the
-// GELU 8700, against 680 per 128 of K).  Measured: 16384 x 4096 -> 4096 168 us = 3.27 POP/s (twice the measured bf16 rate is 3.31);
-// 16384 x 4096 -> 1024 50 us = 2.77; 16384 x 1024 -> 4096 57 us = 2.39, with the GELU 67 us = 2.06; 16384 x 256 -> 4096 32 us, 134 MB
+// GELU 8700, against 680 per 128 of K).  Measured: 16384 x 4096 -> 4096 167 us = 3.30 POP/s (twice the measured bf16 rate is 3.31);
+// 16384 x 4096 -> 1024 49 us = 2.81; 16384 x 1024 -> 4096 54 us = 2.55, with the GELU 66 us = 2.09; 16384 x 256 -> 4096 32 us, 134 MB
 // written.  On the way (16384 x 1024 -> 4096 with GELU, the product alone): eight epilogue warps that store from registers 137 us;
 // sixteen 90; TMA stores 84; scales a tile ahead 73; tensor memory handed over without a cluster-wide release 66.
 // Every wait is bounded; on a timeout the CTA raises FDB_DEV_TIMEOUT in the status word, frees its tensor memory and returns.
@@ -51,11 +51,11 @@ struct Int8Args {
 
 constexpr int kStoreBytes = 64;  // of a row, in one TMA store
 
-template <int CG, int BN> struct Tile {
+template <int CG, int BN, int COLS> struct Tile {
   static constexpr uint32_t kBytesA = kBM * kBK, kBytesW = BN / CG * kBK, kStageBytes = kBytesA + kBytesW;
   static constexpr int kStages = BN == 256 ? 5 : (CG == 2 ? 7 : (BN == 128 ? 5 : 6));
   // the epilogue: columns of a warp; what of them lies in shared memory: 32 rows of a store's bytes, scales and biases
-  static constexpr int kCols = BN == 256 ? 64 : 32, kEpiWarps = BN * 4 / kCols, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+  static constexpr int kCols = COLS, kEpiWarps = BN * 4 / kCols, kThreads = 32 * (kEpiWarp0 + kEpiWarps);
   static constexpr uint32_t kTurnBytes = 32 * kStoreBytes, kColBytes = 2 * kCols * 4;
   static constexpr uint32_t kSmemTurn = kStages * kStageBytes, kSmemCols = kSmemTurn + kEpiWarps * kTurnBytes, kSmemBars = kSmemCols + kEpiWarps * kColBytes;
   enum : uint32_t { kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2, kNumBars = 2 * kStages + 4 };
@@ -81,23 +81,24 @@ template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a
   return a.bias_fp32 ? __ldg(static_cast<const float*>(a.bias) + n) : to_float<T>(static_cast<const T*>(a.bias)[n]);
 }
 
-// A store's columns (16 of fp32, 32 of the others) of 32 rows per warp, each thread its own row, into shared memory, from where a TMA
-// store takes them and leaves out what lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 66 at
+// N columns of 32 rows per warp, each thread its own row, into shared memory, from where a TMA store takes a row's 64 bytes (16 columns of
+// fp32, 32 of the others) and leaves out what lies behind the ends.  (Stores from registers touch 32 lines each: 81 us against 66 at
 // 16384 x 1024 -> 4096.)  Piece p (16 bytes) of row r lies at piece p ^ (r / 2 % 4), the swizzle of the map's 64-byte rows: no bank
-// conflicts.  `cols`: the scales, and the biases COLS behind them, in shared memory.
-template <typename T, bool GELU, int COLS>
-__device__ __forceinline__ void convert_rows(const uint32_t* acc, uint64_t sx, const float* cols, uint32_t* stage, int lane) {
+// conflicts.  `cols`: the scales, and the biases COLS behind them, in shared memory; AT, of the accumulator, and `first`, of the store: where
+// the columns begin.
+template <typename T, bool GELU, int COLS, int N, int AT, int A>
+__device__ __forceinline__ void convert_rows(const uint32_t (&acc)[A], uint64_t sx, const float* cols, uint32_t* stage, int first, int lane) {
   constexpr int kPiece = 16 / int(sizeof(T));
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
+  for (int p = 0; p < N / kPiece; ++p) {
     uint32_t o[4];
 #pragma unroll
     for (int e = 0; e < kPiece; e += 4) {
       const int c = p * kPiece + e;
       const float4 ws = *reinterpret_cast<const float4*>(cols + c), b = *reinterpret_cast<const float4*>(cols + COLS + c);
       float v0, v1, v2, v3;
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c], acc[c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + 2], acc[c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[AT + c], acc[AT + c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
+      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[AT + c + 2], acc[AT + c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
       if constexpr (sizeof(T) == 4) {
         o[0] = __float_as_uint(v0); o[1] = __float_as_uint(v1); o[2] = __float_as_uint(v2); o[3] = __float_as_uint(v3);
       } else {
@@ -105,7 +106,8 @@ __device__ __forceinline__ void convert_rows(const uint32_t* acc, uint64_t sx, c
         o[(e >> 1) + 1] = pack_pair<T>(v2, v3);
       }
     }
-    *reinterpret_cast<uint4*>(stage + lane * 16 + 4 * (p ^ ((lane >> 1) & 3))) = make_uint4(o[0], o[1], o[2], o[3]);
+    const int piece = first * int(sizeof(T)) / 16 + p;
+    *reinterpret_cast<uint4*>(stage + lane * 16 + 4 * (piece ^ ((lane >> 1) & 3))) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -149,9 +151,9 @@ __device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (
   }
 }
 
-template <int CG, int BN, typename OUT, bool GELU>
-__global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(const __grid_constant__ Int8Args args) {
-  using T = Tile<CG, BN>;
+template <int CG, int BN, int COLS, typename OUT, bool GELU>
+__global__ void __launch_bounds__(Tile<CG, BN, COLS>::kThreads, 1) linear_int8_kernel(const __grid_constant__ Int8Args args) {
+  using T = Tile<CG, BN, COLS>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem - smem_u32(smem_raw));
@@ -296,34 +298,71 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
       wait(bar(T::kBarAccFull + acc), (local >> 1) & 1u);
       tc_fence_after();
       const bool has_rows = ok && row0 < args.rows;
+      const uint32_t acc_at = tmem_lane + acc * BN + uint32_t(part * kCols);
+      auto release = [&] {  // the accumulator is in registers: the next tile but one may overwrite it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) { if constexpr (CG == 2) mbar_arrive_peer(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
+      };
+      auto begin_store = [&] {  // the store before has left the stage (the lane that issues them waits)
+        tma_store_wait_read();
+        __syncwarp();
+      };
+      auto end_store = [&](int at) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && n0 + at < args.n) {
+          tma_store_2d(&args.tm_out, smem_u32(turn), n0 + at, (int)row0);
+          tma_store_commit();
+        }
+      };
+      if (kCols == 128 && args.wide) {  // few warps with many registers: the next 16 columns leave tensor memory while 16 are worked on
+        uint32_t a0[16], a1[16];
+        auto load = [&](int at, uint32_t (&a)[16]) { if (ok) tmem_ld16(acc_at + uint32_t(at), a); };
+        load(0, a0);
+        tmem_wait_ld();
 #pragma unroll 1
-      for (int at = 0; at < kCols; at += 32) {
-        uint32_t a[32];
-        if (ok) {  // whole warps execute the load, whatever their rows
-          tmem_ld32(tmem_lane + acc * BN + uint32_t(part * kCols + at), a);
+        for (int at = 0; at < kCols; at += 32) {
+          const bool live = has_rows && n0 + at < args.n;
+          load(at + 16, a1);
+          if (live) {
+            begin_store();
+            convert_rows<OUT, GELU, kCols, 16, 0>(a0, sx, cols + at, turn, 0, lane);
+            if constexpr (kStore == 16) {
+              end_store(at);
+              begin_store();
+            }
+          }
+          tmem_wait_ld();
+          if (at + 32 < kCols) load(at + 32, a0); else release();
+          if (live) {
+            convert_rows<OUT, GELU, kCols, 16, 0>(a1, sx, cols + at + 16, turn, 16 % kStore, lane);
+            end_store(at + 32 - kStore);
+          }
           tmem_wait_ld();
         }
-        if (at + 32 == kCols) {  // the accumulator is in registers: the next tile but one may overwrite it
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) { if constexpr (CG == 2) mbar_arrive_peer(acc_empty[acc]); else mbar_arrive(acc_empty[acc]); }
-        }
-        const int n = n0 + at;
-        if (!has_rows || n >= args.n) continue;
-        if (!args.wide) {
-          store_turned<OUT, GELU, kCols>(args, a, row0, n, sx, cols + at, turn, lane);
-          continue;
-        }
-#pragma unroll
-        for (int c = 0; c < 32; c += kStore) {
-          tma_store_wait_read();  // the store before has left the stage (the lane that issues them waits)
-          __syncwarp();
-          convert_rows<OUT, GELU, kCols>(a + c, sx, cols + at + c, turn, lane);
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0 && n + c < args.n) {
-            tma_store_2d(&args.tm_out, smem_u32(turn), n + c, (int)row0);
-            tma_store_commit();
+      } else {
+#pragma unroll 1
+        for (int at = 0; at < kCols; at += 32) {
+          uint32_t a[32];
+          if (ok) {  // whole warps execute the load, whatever their rows
+            tmem_ld32(acc_at + uint32_t(at), a);
+            tmem_wait_ld();
+          }
+          if (at + 32 == kCols) release();
+          if (!has_rows || n0 + at >= args.n) continue;
+          if (!args.wide) {
+            store_turned<OUT, GELU, kCols>(args, a, row0, n0 + at, sx, cols + at, turn, lane);
+            continue;
+          }
+          if constexpr (kCols == 128) continue;  // (done above)
+          begin_store();
+          convert_rows<OUT, GELU, kCols, kStore, 0>(a, sx, cols + at, turn, 0, lane);
+          end_store(at);
+          if constexpr (kStore == 16) {
+            begin_store();
+            convert_rows<OUT, GELU, kCols, kStore, 16>(a, sx, cols + at + 16, turn, 0, lane);
+            end_store(at + 16);
           }
         }
       }
@@ -347,29 +386,32 @@ __global__ void __launch_bounds__(Tile<CG, BN>::kThreads, 1) linear_int8_kernel(
   }
 }
 
-template <int CG, int BN, typename OUT, bool GELU>
+template <int CG, int BN, int COLS, typename OUT, bool GELU>
 int launch(const Int8Args& a, int grid, bool chained, cudaStream_t stream) {
+  using T = Tile<CG, BN, COLS>;
   static std::atomic<uint64_t> smem_done{0};
-  auto kernel = linear_int8_kernel<CG, BN, OUT, GELU>;
-  cudaError_t e = allow_smem(smem_done, reinterpret_cast<const void*>(kernel), (int)Tile<CG, BN>::kSmemBytes);
-  if (e == cudaSuccess) e = launch_kernel<Int8Args>(kernel, a, dim3((unsigned)grid), Tile<CG, BN>::kThreads, Tile<CG, BN>::kSmemBytes, chained, stream, CG);
+  auto kernel = linear_int8_kernel<CG, BN, COLS, OUT, GELU>;
+  cudaError_t e = allow_smem(smem_done, reinterpret_cast<const void*>(kernel), (int)T::kSmemBytes);
+  if (e == cudaSuccess) e = launch_kernel<Int8Args>(kernel, a, dim3((unsigned)grid), T::kThreads, T::kSmemBytes, chained, stream, CG);
   if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "linear_int8 launch: %s", cudaGetErrorString(e));
   return FDB_OK;
 }
 
-template <int CG, int BN>
+template <int CG, int BN, int COLS>
 int launch_type(const Int8Args& a, int grid, int out_dtype, bool gelu, bool chained, cudaStream_t s) {
-#define FDB_INT8_OUT(OUT) (gelu ? launch<CG, BN, OUT, true>(a, grid, chained, s) : launch<CG, BN, OUT, false>(a, grid, chained, s))
+#define FDB_INT8_OUT(OUT) (gelu ? launch<CG, BN, COLS, OUT, true>(a, grid, chained, s) : launch<CG, BN, COLS, OUT, false>(a, grid, chained, s))
   if (out_dtype == FDB_BF16) return FDB_INT8_OUT(__nv_bfloat16);
   return out_dtype == FDB_FP16 ? FDB_INT8_OUT(__half) : FDB_INT8_OUT(float);
 #undef FDB_INT8_OUT
 }
 
 // Tile shapes: clocks per 128 of K and clocks of a tile's epilogue (with the GELU 1.8 times those), as measured over whole waves
-// (16384 x 4096 -> 4096: 168, 194, 259, 391 us; 16384 x 256 -> 4096: 36, 41, 40, 54).  One runs beside the other but for the first
-// tile's main loop and the last one's epilogue.
-struct Config { int cg, bn, clocks, epilogue; };
-constexpr Config kConfigs[] = {{2, 256, 680, 4800}, {2, 128, 430, 2700}, {1, 128, 535, 2650}, {1, 64, 403, 1800}};
+// (16384 x 4096 -> 4096: 169, 166, 194, 259, 391 us; 16384 x 256 -> 4096: 32, 38, 41, 40, 54).  One runs beside the other but for the
+// first tile's main loop and the last one's epilogue.  The 256 x 256 tile has two forms of the epilogue: 16 warps of 64 columns hide more
+// latency, 8 of 128 columns leave the main loop more of the issue slots.  16384 rows, 16 against 8 warps: 256 -> 4096 32 and 38 us,
+// 1024 -> 4096 57 and 54, with the GELU 66 and 73, 2048 -> 4096 with the GELU 97 and 95.
+struct Config { int cg, bn, cols, clocks, epilogue; };
+constexpr Config kConfigs[] = {{2, 256, 64, 680, 4800}, {2, 256, 128, 640, 5300}, {2, 128, 32, 430, 2700}, {1, 128, 32, 535, 2650}, {1, 64, 32, 403, 1800}};
 
 bool float_type(int t) { return t == FDB_BF16 || t == FDB_FP16 || t == FDB_FP32; }
 unsigned type_bytes(int t) { return t == FDB_FP32 ? 4u : 2u; }
@@ -462,7 +504,9 @@ extern "C" FDB_API int fdb_linear_int8(const fdb_linear_int8_params* p, void* st
   const int grid = (int)(best_tiles < units ? best_tiles : units) * best->cg;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool gelu = p->gelu != 0, chained = !given;
-  if (best->cg == 2)
-    return best->bn == 256 ? launch_type<2, 256>(a, grid, p->out_dtype, gelu, chained, s) : launch_type<2, 128>(a, grid, p->out_dtype, gelu, chained, s);
-  return best->bn == 128 ? launch_type<1, 128>(a, grid, p->out_dtype, gelu, chained, s) : launch_type<1, 64>(a, grid, p->out_dtype, gelu, chained, s);
+#define FDB_INT8_TILE(CG, BN, COLS) launch_type<CG, BN, COLS>(a, grid, p->out_dtype, gelu, chained, s)
+  if (best->bn == 256) return best->cols == 128 ? FDB_INT8_TILE(2, 256, 128) : FDB_INT8_TILE(2, 256, 64);
+  if (best->cg == 2) return FDB_INT8_TILE(2, 128, 32);
+  return best->bn == 128 ? FDB_INT8_TILE(1, 128, 32) : FDB_INT8_TILE(1, 64, 32);
+#undef FDB_INT8_TILE
 }

@@ -124,6 +124,17 @@ def test_product_of_many_tiles(rows, k, n):
     ops.check_status()
 
 
+@pytest.mark.parametrize("n", [1104, 1101, 1028])
+@pytest.mark.parametrize("dtype,gelu", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float16, False), (torch.float32, True)])
+def test_product_of_many_long_tiles(n, dtype, gelu):
+    """The epilogue of few warps that long rows take, the last columns and rows of the matrix inside a tile."""
+    x, wq, ws, b = _problem(7001, 2100, n, dtype, torch.float32, n + 1)
+    xq, xs = ops.quantize_int8(x)
+    acc = (xq.double() @ wq.double().t()).cpu()
+    _check(ops.linear_int8(x, wq, ws, b, gelu=gelu), xq, xs, wq, ws, b, gelu, acc)
+    ops.check_status()
+
+
 @pytest.mark.parametrize("rows,k,n", [(5, 2000, 96), (70, 5000, 256), (300, 131071, 64), (1, 131071, 8)])
 def test_largest_integers(rows, k, n):
     """Every product at its largest: the sums reach 2^31 - 2^14 and stay exact."""
