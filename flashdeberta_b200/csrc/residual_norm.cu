@@ -15,9 +15,9 @@
 // (RMSNorm without the mean terms).  The stream is computed again from x and residual, in fp32 as the forward had it: the rounded one
 // would cost as many bytes and put its rounding into zhat.  HBM-bound by its bytes (four tensors of rows read, two written), in fact by
 // its instructions, some 45 per element, and the chain of two sums a row on 16 warps per SM: 32768 x 1024 bf16 81 us = 76 % with one
-// LayerNorm, 95 us = 65 % with RMS norms on both sides and a gate per sequence, 115 us = 53 % with LayerNorms; above 4096 columns a
+// LayerNorm, 92 us = 67 % with RMS norms on both sides and a gate per sequence, 101 us = 61 % with LayerNorms; above 4096 columns a
 // CTA of 1024 threads has too few registers (232 us at 4096 x 8192).  On the way (32768 x 1024, RMS norms): sums through a loop over
-// the warps and parameters loaded for every row 125 us; parameters in shared memory 107; two-wide arithmetic 92 to 95.
+// the warps and parameters loaded for every row 125 us; parameters in shared memory 107; two-wide arithmetic 92 to 95; with LayerNorms 114, and 101 once rows waited in shared memory.
 //
 // Sums over rows (gradients of weights, biases and gate) stay in registers while a thread walks its rows, one per column and sum;
 // they go to memory once per CTA and a second kernel adds them up in a fixed order: no atomics, the same bits every time.

@@ -29,6 +29,7 @@ struct ResidualNormBwdArgs {
   float* slots;        // (workers + groups, 2, hidden): A and B of a worker's rows in a group
   int64_t workers;     // teams that have rows: worker w the rows [rows w / workers, rows (w + 1) / workers)
   int ctas, vectors, mode, groups;
+  int ring_at;         // where in shared memory rows lie that are on their way
 };
 
 constexpr int kNormBwdThreads = 512;  // threads of a backward CTA whose rows take fewer: one CTA per SM, of several rows at a time

@@ -15,6 +15,7 @@ using ptx::mul_f32x2;
 
 constexpr int kNormBwdTeams = kNormBwdThreads / 32;
 constexpr size_t kNormBwdPlainSmem = 40 * 1024;  // with the 8 KB of the teams' sums, what a launch may take without being asked
+constexpr int kNormBwdRows = 3;                  // of a team in shared memory: one that is worked on, two on their way
 
 // Shared memory of a CTA: weight, post_weight, post_bias and a channel's gate in fp32 (read for every row, converted once), one vector of
 // sums per thread for adding teams up and, where the gate has groups, what C = sum gate A and D = sum gate B have come to (touched
@@ -23,6 +24,11 @@ inline size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode
   const size_t vector = size_t(threads) * kRowElems * sizeof(float), params = size_t(threads / teams) * kRowElems * sizeof(float);
   return 4 * params + (teams > 1 ? vector : 0) + (post && mode == kGateGroups ? 2 * vector : 0);
 }
+
+// Whether rows of 16-bit types are on their way in shared memory (the kernel says why), and what they take of it: x, residual, dnormed,
+// dstream and an element's gate, 16 bytes of each per thread.  With what there is otherwise that is at most 200 KB.
+__host__ __device__ constexpr bool norm_bwd_ring(bool post, int mode) { return post && mode != kGateChannel; }
+inline size_t norm_bwd_ring_smem(int threads, int mode) { return size_t(kNormBwdRows) * (mode == kGateElement ? 5 : 4) * 16 * threads; }
 
 template <typename T, bool RMS, bool POST, int GATE, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormBwdArgs b) {
@@ -40,22 +46,62 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
   const int64_t first = has_rows ? f.rows * worker / b.workers : 0, end = has_rows ? f.rows * (worker + 1) / b.workers : 0;
   ptx::grid_launch();
 
-  struct Row { RowWords<T> x, residual, dnormed, dstream, gate; float4 stats; };
+  // Rows on their way.  With a norm after the block and a gate per group or element there is much to keep in registers: rows come
+  // through shared memory then, two ahead, by copies that nobody waits for until they are due; every thread copies what it reads
+  // itself, so there is nothing to wait for but its own copies.  Otherwise the next row is on its way in registers while one is worked on.
+  // 32768 x 1024 bf16, registers against shared memory, both LayerNorms: gate per group 114 and 101 us, per element 158 and 106, per
+  // channel 96 and 110; one LayerNorm 81 and 84; RMS norms, gate per group 94 and 92.  fp32 rows and 1024 threads have room for neither
+  // (8192 x 768 fp32: 40 us, through shared memory 49); single elements and shifted pieces are put into words at once.
+  constexpr bool kPrefetch = sizeof(T) == 2 && WIDE && THREADS <= kNormBwdThreads;
+  constexpr bool kRing = kPrefetch && norm_bwd_ring(POST, GATE), kAhead = kPrefetch && !kRing;
+  constexpr int kTensors = GATE == kGateElement ? 5 : 4;
+  enum : int { kX = 0, kResidual = 1, kDnormed = 2, kDstream = 3, kGateRow = 4 };
   const bool element_gate = GATE == kGateElement && f.gate != nullptr && !f.gate_fp32;
+  uint4* s_ring = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(s_vectors) + b.ring_at) + threadIdx.x;
+  auto slot_at = [&](int slot, int tensor) { return s_ring + (slot * kTensors + tensor) * blockDim.x; };
+  auto copy = [&](const void* p, int64_t at, int slot, int tensor) {
+    ptx::copy_async_16B(ptx::smem_u32(slot_at(slot, tensor)), static_cast<const T*>(p) + at + t * kRowElems);
+  };
+  auto send = [&](int64_t row, int slot) {
+    if (row < end && cols.live(0)) {
+      const int64_t at = row * f.hidden;
+      copy(f.x, at, slot, kX);
+      if (f.residual != nullptr) copy(f.residual, at, slot, kResidual);
+      if (b.dnormed != nullptr) copy(b.dnormed, at, slot, kDnormed);
+      if (b.dstream != nullptr) copy(b.dstream, at, slot, kDstream);
+      if constexpr (GATE == kGateElement) { if (element_gate) copy(f.gate, at, slot, kGateRow); }
+    }
+    ptx::copy_async_commit();  // (a group per row, empty or not: they are counted)
+  };
+  struct Row { RowWords<T> tensor[kTensors]; float4 stats; };
   auto fetch = [&](int64_t row, Row& r) {
     const int64_t at = row * f.hidden;
-    cols.load(static_cast<const T*>(f.x) + at, r.x);
-    if (f.residual != nullptr) cols.load(static_cast<const T*>(f.residual) + at, r.residual);
-    if (b.dnormed != nullptr) cols.load(static_cast<const T*>(b.dnormed) + at, r.dnormed);
-    if (b.dstream != nullptr) cols.load(static_cast<const T*>(b.dstream) + at, r.dstream);
-    if (element_gate) cols.load(static_cast<const T*>(f.gate) + at, r.gate);
+    cols.load(static_cast<const T*>(f.x) + at, r.tensor[kX]);
+    if (f.residual != nullptr) cols.load(static_cast<const T*>(f.residual) + at, r.tensor[kResidual]);
+    if (b.dnormed != nullptr) cols.load(static_cast<const T*>(b.dnormed) + at, r.tensor[kDnormed]);
+    if (b.dstream != nullptr) cols.load(static_cast<const T*>(b.dstream) + at, r.tensor[kDstream]);
+    if constexpr (GATE == kGateElement) { if (element_gate) cols.load(static_cast<const T*>(f.gate) + at, r.tensor[kGateRow]); }
     r.stats = __ldg(f.stats + row);
   };
-  // the next row is on its way while one is worked on, where registers allow it (fp32 rows and 1024 threads do not; single
-  // elements and shifted pieces are put into words at once)
-  constexpr bool kAhead = sizeof(T) == 2 && WIDE && THREADS <= kNormBwdThreads;
+  int slot = 0;
   Row now, next;
-  if (kAhead && first < end) fetch(first, now);
+  auto take = [&](int tensor, uint64_t (&v)[kPairs]) {
+    if constexpr (kRing) {
+      RowWords<T> r;
+      *reinterpret_cast<uint4*>(r.w) = *slot_at(slot, tensor);
+      unpack(r, v);
+    } else {
+      unpack(now.tensor[tensor], v);
+    }
+  };
+  if constexpr (kRing) {
+    if (!cols.live(0))  // a thread behind the end of the row reads zeros all the time
+      for (int i = 0; i < kNormBwdRows * kTensors; ++i) s_ring[i * blockDim.x] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < kNormBwdRows - 1; ++i) send(first + i, i);
+    if (first < end) now.stats = __ldg(f.stats + first);
+  } else if constexpr (kAhead) {
+    if (first < end) fetch(first, now);
+  }
 
   // vectors over the columns: two 16-byte pieces per thread, each piece of the team's threads side by side
   enum : int { kWeight = 0, kPostWeight = 1, kPostBias = 2, kGateVector = 3 };
@@ -116,7 +162,11 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
   const uint64_t scale = both(f.residual_scale);
 #pragma unroll(kAhead && RMS ? 2 : 1)  // (two rows a round save the copy of the words, 105 -> 95 us at 32768 x 1024; with a LayerNorm's sums they spill)
   for (int64_t row = first; row < end; ++row) {
-    if constexpr (kAhead) {
+    if constexpr (kRing) {
+      send(row + kNormBwdRows - 1, slot == 0 ? kNormBwdRows - 1 : slot - 1);  // where the row before was
+      if (row + 1 < end) next.stats = __ldg(f.stats + row + 1);
+      ptx::copy_async_wait<kNormBwdRows - 1>();
+    } else if constexpr (kAhead) {
       if (row + 1 < end) fetch(row + 1, next);
     } else {
       fetch(row, now);
@@ -130,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
         cols.template load_param<T>(f.gate, f.gate_fp32, group * f.hidden, g);
       }
     } else if constexpr (GATE == kGateElement) {
-      if (element_gate) unpack(now.gate, g);
+      if (element_gate) take(kGateRow, g);
       else if (f.gate != nullptr) cols.load(static_cast<const float*>(f.gate) + at, g);
     } else {
       get_vector(kGateVector, g);
@@ -138,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
 
     // the stream again; hat: x normalised (x itself without the norm), z: the stream normalised
     uint64_t hat[kPairs], u[kPairs], z[kPairs], d[kPairs], p[kPairs];
-    unpack(now.x, hat);
+    take(kX, hat);
     if constexpr (POST) {
       const uint64_t mean = both(-now.stats.x), inv = both(now.stats.y);
       get_vector(kPostWeight, p);
@@ -159,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) z[j] = mul_f32x2(g[j], u[j]);
     if (f.residual != nullptr) {
-      unpack(now.residual, p);
+      take(kResidual, p);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) z[j] = fma_f32x2(scale, p[j], z[j]);
     }
@@ -173,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
     float sums[kSums];
     if (b.dnormed != nullptr) {
       uint64_t s0 = both(0.f), s1 = both(0.f);
-      unpack(now.dnormed, d);
+      take(kDnormed, d);
       get_vector(kWeight, p);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
@@ -196,7 +246,7 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
       for (int j = 0; j < kPairs; ++j) d[j] = both(0.f);
     }
     if (b.dstream != nullptr) {
-      unpack(now.dstream, p);
+      take(kDstream, p);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) d[j] = add_f32x2(d[j], p[j]);
     }
@@ -242,7 +292,12 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
       for (int j = 0; j < kPairs; ++j) d[j] = fma_f32x2(d[j], inv, RMS ? mul_f32x2(hat[j], m0) : fma_f32x2(hat[j], m0, m1));
     }
     cols.store(static_cast<T*>(b.dx) + at, d);
-    if constexpr (kAhead) now = next;
+    if constexpr (kRing) {
+      slot = slot + 1 == kNormBwdRows ? 0 : slot + 1;
+      now.stats = next.stats;
+    } else if constexpr (kAhead) {
+      now = next;
+    }
   }
   if constexpr (GATE == kGateGroups) {
     if (group >= 0) leave_group(group, g);
@@ -293,11 +348,14 @@ auto with_norm_bwd_kernel(bool rms, bool post, int mode, bool wide, int threads,
 #undef FDB_BWD2
 }
 
-template <typename T> int norm_bwd_launch(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s) {
+template <typename T> int norm_bwd_launch(const ResidualNormBwdArgs& args, bool wide, cudaStream_t s) {
+  ResidualNormBwdArgs b = args;
   const int threads = b.f.teams * b.f.team_threads;
   const bool post = b.f.post_weight != nullptr;
   return with_norm_bwd_kernel<T>(b.f.rms, post, b.mode, wide, threads, [&](auto kernel) {
-    const size_t smem = residual_norm_bwd_smem(threads, b.f.teams, post, b.mode);
+    size_t smem = residual_norm_bwd_smem(threads, b.f.teams, post, b.mode);
+    b.ring_at = (int)smem;
+    if (sizeof(T) == 2 && wide && threads <= kNormBwdThreads && norm_bwd_ring(post, b.mode)) smem += norm_bwd_ring_smem(threads, b.mode);
     cudaError_t e = smem > kNormBwdPlainSmem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
     if (e == cudaSuccess) e = launch_kernel<ResidualNormBwdArgs>(kernel, b, dim3((unsigned)b.ctas), threads, smem, false, s);
     if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm backward launch: %s", cudaGetErrorString(e));

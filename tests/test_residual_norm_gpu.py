@@ -158,6 +158,16 @@ def test_rows_and_groups(batch, seqlen, hidden, rms):
     _compare(t, grads, rms=rms, scale=0.7)
 
 
+@pytest.mark.parametrize("dtype,rms,gate", [(torch.bfloat16, False, "sequence"), (torch.float16, True, "sequence"), (torch.float16, False, "element"),
+                                            (torch.bfloat16, True, "element"), (torch.bfloat16, False, None)])
+@pytest.mark.parametrize("batch,seqlen,hidden,residual", [(31, 331, 40, True), (7, 401, 1000, False), (3, 650, 2056, True), (2, 383, 4096, True)])
+def test_many_rows_per_team(dtype, rms, gate, batch, seqlen, hidden, residual):
+    """Rows on their way ahead of the one that is worked on, several times around, in groups that end in between."""
+    gate = {None: None, "sequence": (batch, 1, hidden), "element": (batch, seqlen, hidden)}[gate]
+    t, grads = _inputs((batch, seqlen, hidden), dtype, rms, True, gate, 11, residual=residual)
+    _compare(t, grads, rms=rms, scale=0.7)
+
+
 def test_without_residual_and_with_parameters_in_fp32():
     t, grads = _inputs((2, 33, 768), torch.bfloat16, False, True, (768,), 5, residual=False, params=torch.float32)
     t["gate"] = t["gate"].float()
