@@ -5,8 +5,8 @@
 // team: mean, then centred squares (two passes over registers: rows whose mean is far from zero lose nothing).  Sums in fp32, `normed`
 // from the sum before it is rounded to the rows' type.  HBM-bound: x and residual read, both results written.  Measured (four sets of
 // inputs in turn, of the copy bandwidth of 6548 GB/s): 16384 x 1024 bf16, one LayerNorm 20.7 us = 99 %, RMS norms on both sides and a
-// gate 23.8 us = 86 %, LayerNorms on both sides 28.9 us = 71 % (four sums one after another, 16 rows on an SM); 8192 x 1024 fp32
-// 21.7 us = 94 %; rows of several warps 55 to 71 %; 16-bit rows that start anywhere 30 %.
+// gate 23.8 us = 86 %, LayerNorms on both sides 28 us = 73 % (four sums one after another, 16 rows on an SM), 65536 x 256
+// 30 us = 68 %, one LayerNorm 21 us = 97 %; 8192 x 1024 fp32 21.7 us = 94 %; rows of several warps 55 to 71 %; 16-bit rows that start anywhere 30 %.
 //
 // Backward (residual_norm_bwd.cuh), for every row with the statistics that the forward kept (mean and inverse deviation of both norms):
 //     dz = dstream + inv2 (y - mean(y) - zhat mean(y zhat)),   y = weight dnormed,  zhat = (stream - mean2) inv2
@@ -17,7 +17,8 @@
 // its instructions, some 45 per element, and the chain of two sums a row on 16 warps per SM: 32768 x 1024 bf16 81 us = 76 % with one
 // LayerNorm, 92 us = 67 % with RMS norms on both sides and a gate per sequence, 101 us = 61 % with LayerNorms; above 4096 columns a
 // CTA of 1024 threads has too few registers (232 us at 4096 x 8192).  On the way (32768 x 1024, RMS norms): sums through a loop over
-// the warps and parameters loaded for every row 125 us; parameters in shared memory 107; two-wide arithmetic 92 to 95; with LayerNorms 114, and 101 once rows waited in shared memory.
+// the warps and parameters loaded for every row 125 us; parameters in shared memory 107; two-wide arithmetic 92 to 95; with
+// LayerNorms 114, and 101 once rows waited in shared memory.
 //
 // Sums over rows (gradients of weights, biases and gate) stay in registers while a thread walks its rows, one per column and sum;
 // they go to memory once per CTA and a second kernel adds them up in a fixed order: no atomics, the same bits every time.

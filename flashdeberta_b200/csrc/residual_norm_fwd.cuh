@@ -17,14 +17,22 @@ using ptx::mul_f32x2;
 
 // Up to 1024 elements a row belongs to one warp (ONE): its sums are shuffles, and nothing keeps the next row's loads from starting.
 // Longer rows take as many warps, with barriers of their own between them.  A CTA stays and takes row after row: weights and biases
-// (and a channel's gate) are converted to fp32 once, into shared memory, and the next row is on its way while one is worked on.
+// (and a channel's gate) are converted to fp32 once, into shared memory, and the next rows are on their way while one is worked on.
 constexpr int kNormFwdWarpElems = 1024;
 constexpr int kNormFwdThreads = 512;  // of a CTA of longer rows, one per SM (at most 128 registers a thread)
+// Whether 16-bit rows of one warp are on their way in shared memory, two ahead, instead of one ahead in registers.  16 M elements, registers
+// against shared memory, both LayerNorms with a gate per sequence, then one LayerNorm: 256 columns 37 and 31 us, 24 and 21; 512 30 and 27, 23
+// and 20; 768 28 and 27, 22 and 21 (with a
+// gate per channel 24 and 26); 1024 29 and 28, 21 and 21.5 (with a gate per element 24 and 25.5).
+constexpr int kNormFwdRows = 2;
+template <typename T> __host__ __device__ constexpr bool norm_fwd_ring(bool rms, bool post, bool wide, int v, bool one) {
+  return sizeof(T) == 2 && wide && one && (v < 4 || (post && !rms));
+}
 // CTAs per SM of rows of one warp, 4 rows each: what the registers of V x 8 elements per thread allow.
-constexpr int norm_fwd_ctas(int v) { return v == 1 ? 10 : (v == 2 ? 7 : 4); }
+constexpr int norm_fwd_ctas(int v, bool ring) { return v == 1 ? 10 : (v == 2 ? 7 : (v == 3 && ring ? 5 : 4)); }
 
 template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>
-__global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ctas(V) : 1)
+__global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ctas(V, norm_fwd_ring<T>(RMS, POST, WIDE, V, ONE)) : 1)
     residual_norm_kernel(const __grid_constant__ ResidualNormArgs a) {
   constexpr int kElems = V * kRowElems, kPairs = kElems / 2;
   extern __shared__ __align__(16) float4 s_vectors[];
@@ -42,8 +50,31 @@ __global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ct
   };
   const int64_t step = (int64_t)gridDim.x * a.teams;
   int64_t row = (int64_t)blockIdx.x * a.teams + team;
-  constexpr bool kAhead = sizeof(T) == 2 && WIDE;  // (fp32 rows would take too many registers, single elements and shifted pieces are put into words at once)
+  constexpr bool kRing = norm_fwd_ring<T>(RMS, POST, WIDE, V, ONE);
+  constexpr bool kAhead = sizeof(T) == 2 && WIDE && !kRing;  // (fp32 rows would take too many registers, single elements and shifted pieces are put into words at once)
   if (kAhead && row < a.rows) fetch(row, nx, nr);
+  // rows on their way in shared memory: each thread copies what it reads itself, so it waits for its own copies alone
+  uint4* s_ring = reinterpret_cast<uint4*>(s_vectors + 5 * (kElems / 4) * threads) + threadIdx.x;
+  auto send = [&](int64_t r, int slot) {
+    if (r < a.rows) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!cols.live(i * kRowElems)) continue;
+        const int64_t from = r * a.hidden + cols.col(i * kRowElems);
+        ptx::copy_async_16B(ptx::smem_u32(s_ring + (slot * 2 * V + i) * 128), static_cast<const T*>(a.x) + from);
+        if (a.residual != nullptr) ptx::copy_async_16B(ptx::smem_u32(s_ring + (slot * 2 * V + V + i) * 128), static_cast<const T*>(a.residual) + from);
+      }
+    }
+    ptx::copy_async_commit();
+  };
+  int slot = 0;
+  if constexpr (kRing) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)  // what lies behind the end of the row reads as zeros all the time
+      if (!cols.live(i * kRowElems))
+        for (int k = 0; k < 2 * kNormFwdRows; ++k) s_ring[(k * V + i) * 128] = make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < kNormFwdRows; ++k) send(row + k * step, k);
+  }
 
   // vectors over the columns: 16-byte pieces, each piece of the team's threads side by side
   enum : int { kWeight = 0, kBias = 1, kPostWeight = 2, kPostBias = 3, kGateVector = 4 };
@@ -110,7 +141,16 @@ __global__ void __launch_bounds__(ONE ? 128 : kNormFwdThreads, ONE ? norm_fwd_ct
 #pragma unroll 1
   for (; row < a.rows; row += step) {
     const int64_t at = row * a.hidden;
-    if constexpr (kAhead) {
+    if constexpr (kRing) {
+      ptx::copy_async_wait<kNormFwdRows - 1>();
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        reinterpret_cast<uint4*>(rx.w)[i] = s_ring[(slot * 2 * V + i) * 128];
+        reinterpret_cast<uint4*>(rr.w)[i] = s_ring[(slot * 2 * V + V + i) * 128];
+      }
+      send(row + kNormFwdRows * step, slot);
+      slot = slot + 1 == kNormFwdRows ? 0 : slot + 1;
+    } else if constexpr (kAhead) {
       rx = nx;
       rr = nr;
       if (row + step < a.rows) fetch(row + step, nx, nr);
@@ -150,9 +190,10 @@ template <typename T, bool RMS, bool POST, bool WIDE, int V, bool ONE>
 int norm_fwd_launch_kernel(const ResidualNormArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> smem_done{0};
   auto kernel = residual_norm_kernel<T, RMS, POST, WIDE, V, ONE>;
-  const int threads = a.teams * a.team_threads, smem = 5 * V * kRowElems * a.team_threads * (int)sizeof(float);
-  constexpr int kMost = 5 * V * kRowElems * (ONE ? 32 : 256) * (int)sizeof(float);
-  const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (ONE ? norm_fwd_ctas(V) : 1);
+  constexpr bool kRing = norm_fwd_ring<T>(RMS, POST, WIDE, V, ONE);
+  constexpr int kRingBytes = kRing ? kNormFwdRows * 2 * V * 16 * 128 : 0, kMost = 5 * V * kRowElems * (ONE ? 32 : 256) * (int)sizeof(float) + kRingBytes;
+  const int threads = a.teams * a.team_threads, smem = 5 * V * kRowElems * a.team_threads * (int)sizeof(float) + kRingBytes;
+  const int64_t want = (a.rows + a.teams - 1) / a.teams, most = (int64_t)std::max(1, sm_count()) * (ONE ? norm_fwd_ctas(V, kRing) : 1);
   cudaError_t e = smem > 40 * 1024 ? allow_smem(smem_done, reinterpret_cast<const void*>(kernel), kMost) : cudaSuccess;
   if (e == cudaSuccess) e = launch_kernel<ResidualNormArgs>(kernel, a, dim3((unsigned)std::min(want, most)), threads, smem, false, s);
   if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm launch: %s", cudaGetErrorString(e));
