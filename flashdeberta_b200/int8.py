@@ -40,17 +40,18 @@ def _rows(t: torch.Tensor):
     cols = shape[-1]
     if at % 16 != 0 or (strides[-1] != 1 and cols > 1):
         return None
-    pitch = inner = 0
+    pitch = inner = None
     for n, s in zip(shape[-2::-1], strides[-2::-1]):  # the leading dimensions as one
         if n == 1:
             continue
-        if pitch == 0:
+        if pitch is None:
             pitch = s
         elif s != inner:
             return None
         inner = n * s
-    if pitch == 0:  # one row: any will do
+    if pitch is None:  # one row: any will do
         return at, _pitch(cols)
+    # (an expanded dimension has a stride of zero: no pitch, and nothing that further dimensions could go on from)
     return (at, pitch) if pitch % 16 == 0 and pitch >= cols else None
 
 

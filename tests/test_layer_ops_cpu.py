@@ -148,6 +148,19 @@ def test_int8_rows_layout():
         int8_rows(torch.zeros(2, 2))
 
 
+@pytest.mark.parametrize("shape,expanded", [((1, 16), (8, 16)), ((1, 64), (32, 64)), ((4, 1, 48), (4, 3, 48)), ((4, 1, 64), (4, 8, 64)), ((1, 5, 32), (6, 5, 32)),
+                                            ((2, 1, 3, 16), (2, 4, 3, 16)), ((1, 1, 16), (2, 3, 16)), ((5, 1), (5, 16))])
+def test_expanded_rows_of_integers_are_copied(shape, expanded):
+    """A row that stands for several is in memory once: taken as rows behind one another it would be read far past its end."""
+    a = torch.randint(-128, 128, shape, dtype=torch.int8).expand(expanded)
+    assert _rows(a) is None
+    b = int8_rows(a)
+    at, pitch = _rows(b)
+    assert torch.equal(a, b) and pitch >= expanded[-1]
+    end = b.untyped_storage().data_ptr() + b.untyped_storage().nbytes()
+    assert at + (a.numel() // expanded[-1] - 1) * pitch + expanded[-1] <= end
+
+
 # ---- gradients ---------------------------------------------------------------------------------------------------------
 def _clip(entry=(P, P, 5, 0, 0), **kw):
     t = (_lib.GradTensor * 2)(_lib.GradTensor(P, P, 3, 1, 1), _lib.GradTensor(*entry))

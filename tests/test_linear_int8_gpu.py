@@ -197,6 +197,24 @@ def test_views_that_have_to_be_copied():
     assert torch.equal(ops.linear_int8(x, wq, ws, off[1:]), want)
 
 
+@pytest.mark.parametrize("shape,expanded", [((1, 192), (6, 192)), ((2, 1, 192), (2, 4, 192)), ((1, 192), (300, 192)), ((5, 1, 192), (5, 40, 192)),
+                                            ((1, 50, 192), (3, 50, 192))])
+def test_expanded_integers_count_as_often_as_they_stand_for(shape, expanded):
+    """x, its scales and the weight as views that repeat rows, against their copies."""
+    g = torch.Generator().manual_seed(sum(expanded))
+    x = torch.randint(-128, 128, shape, generator=g, dtype=torch.int8).to(DEV).expand(expanded)
+    xs = torch.rand(shape[:-1], generator=g).to(DEV).expand(expanded[:-1])
+    w = torch.randint(-128, 128, (72, 192), generator=g, dtype=torch.int8).to(DEV)
+    ws = torch.rand(72, generator=g).to(DEV)
+    want = ops.linear_int8(x.contiguous(), w, ws, x_scale=xs.contiguous(), out_dtype=torch.float32)
+    _check(want.view(-1, 72), x.reshape(-1, 192), xs.reshape(-1), w, ws, None, False)
+    assert torch.equal(ops.linear_int8(x, w, ws, x_scale=xs, out_dtype=torch.float32), want)
+    one = w[:1].expand(72, 192)
+    want = ops.linear_int8(x.contiguous(), one.contiguous(), ws, x_scale=xs.contiguous())
+    assert torch.equal(ops.linear_int8(x, one, ws, x_scale=xs), want)
+    ops.check_status()
+
+
 def test_rows_that_are_not_finite_stay_apart():
     x, wq, ws, b = _problem(50, 300, 64, torch.bfloat16, torch.bfloat16, 8)
     want = ops.linear_int8(x, wq, ws, b, gelu=True)
