@@ -16,6 +16,7 @@ namespace fdb {
 namespace {
 
 constexpr int kThreads = 128, kWarpElems = 1024;
+constexpr int kMostCols = 1 << 30;  // columns are counted in 32 bits, up to a team's 8192 behind the last one
 
 // Columns of an fp32 row that starts anywhere: runs of four per thread, so that what they become is stored four bytes at a time.
 template <int V> struct QuadColumns {
@@ -124,7 +125,7 @@ extern "C" FDB_API int fdb_quantize_int8(const void* x, int32_t dtype, int64_t r
                                          void* stream) {
   clear_error();
   if (dtype != FDB_BF16 && dtype != FDB_FP16 && dtype != FDB_FP32) return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: dtype %d", dtype);
-  if (rows > 2147483647LL) return fail(FDB_ERR_LIMIT, "quantize_int8: %lld rows", (long long)rows);
+  if (rows > 2147483647LL || cols > kMostCols) return fail(FDB_ERR_LIMIT, "quantize_int8: %lld rows of %d; at most 2^31 - 1 of 2^30", (long long)rows, cols);
   if (rows < 0 || cols <= 0 || pitch < cols)
     return fail(FDB_ERR_INVALID_ARGUMENT, "quantize_int8: rows %lld, cols %d, pitch %lld", (long long)rows, cols, (long long)pitch);
   if (rows == 0) return FDB_OK;

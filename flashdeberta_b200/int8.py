@@ -14,6 +14,7 @@ from . import _lib, ops
 from .norms import TYPES
 
 MAX_IN_FEATURES = 131071  # products of two 8-bit integers that a 32-bit sum holds
+MAX_COLS = 1 << 30        # of a row that quantize_int8 takes
 
 
 def _pitch(cols: int) -> int:
@@ -64,8 +65,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
     if x.dtype not in TYPES:
         raise TypeError(f"quantize_int8 takes bfloat16, float16 or float32, not {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("quantize_int8 takes rows of at least one element")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_COLS:
+        raise ValueError(f"quantize_int8 takes rows of 1 to {MAX_COLS} elements")
     if ops.intercepted(x):
         raise RuntimeError("quantize_int8 goes by the memory of plain tensors: call it outside tracing, or linear_int8, which rounds within")
     cols = x.shape[-1]

@@ -497,8 +497,8 @@ FDB_API int fdb_residual_norm_bwd(const fdb_residual_norm_bwd_params* p, void* s
  * Rows as 8-bit integers with a scale each: scale = amax / 127, y = x * (127 / amax) rounded to the nearest whole number, ties to even
  * (both quotients and the product in fp32).  A row of zeros, or one whose largest magnitude is below 2^-100, has scale and integers
  * zero; a row with an infinity or a NaN has integers zero and a scale that is infinite or NaN, so whatever is made of it is NaN.
- * x: (rows, cols) of FDB_BF16, FDB_FP16 or FDB_FP32, contiguous; y: rows of `pitch` bytes, at least cols and a multiple of 16, y 16-byte
- * aligned; of the bytes behind a row up to seven are written as zeros; scale: (rows).
+ * x: (rows, cols) of FDB_BF16, FDB_FP16 or FDB_FP32, contiguous, cols at most 2^30; y: rows of `pitch` bytes, at least cols and a multiple of
+ * 16, y 16-byte aligned; of the bytes behind a row up to seven are written as zeros; scale: (rows).
  * The same kernel scales tokens and the output channels of a weight.
  */
 FDB_API int fdb_quantize_int8(const void* x, int32_t dtype, int64_t rows, int32_t cols, void* y, int64_t pitch, float* scale, void* stream);

@@ -132,6 +132,12 @@ def test_quantize_int8_argument_errors(args, code):
     _refused(_lib.load().fdb_quantize_int8(*args, None), code)
 
 
+@pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 1])
+def test_quantize_int8_refuses_rows_that_it_cannot_count(cols):
+    """A 32-bit column counter would pass its end."""
+    _refused(_lib.load().fdb_quantize_int8(P, 0, 1, cols, P, 1 << 31, P, None), -6)
+
+
 def test_quantize_int8_without_rows_is_a_no_op():
     assert _lib.load().fdb_quantize_int8(None, 0, 0, 8, None, 8, None, None) == 0
 

@@ -242,6 +242,13 @@ def test_gelu_over_its_range():
     _check(out, xq, xs, w, torch.ones(8), None, True)
 
 
+@pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) + 8, (1 << 32) + 8])
+def test_rows_that_are_too_long_are_refused(cols):
+    """Before anything is read or copied, in the last case before 8 columns are left of them in 32 bits."""
+    with pytest.raises(ValueError, match="elements"):
+        ops.quantize_int8(torch.ones(1, 1, device=DEV).expand(1, cols))
+
+
 def test_rows_behind_the_last_one_are_left_alone():
     import ctypes as C
     from flashdeberta_b200 import _lib
