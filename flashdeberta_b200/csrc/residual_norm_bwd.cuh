@@ -20,7 +20,7 @@ constexpr int kNormBwdRows = 3;                  // of a team in shared memory: 
 // Shared memory of a CTA: weight, post_weight, post_bias and a channel's gate in fp32 (read for every row, converted once), one vector of
 // sums per thread for adding teams up and, where the gate has groups, what C = sum gate A and D = sum gate B have come to (touched
 // only when a group ends).
-inline size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode) {
+__host__ __device__ constexpr size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode) {
   const size_t vector = size_t(threads) * kRowElems * sizeof(float), params = size_t(threads / teams) * kRowElems * sizeof(float);
   return 4 * params + (teams > 1 ? vector : 0) + (post && mode == kGateGroups ? 2 * vector : 0);
 }
@@ -28,7 +28,7 @@ inline size_t residual_norm_bwd_smem(int threads, int teams, bool post, int mode
 // Whether rows of 16-bit types are on their way in shared memory (the kernel says why), and what they take of it: x, residual, dnormed,
 // dstream and an element's gate, 16 bytes of each per thread.  With what there is otherwise that is at most 200 KB.
 __host__ __device__ constexpr bool norm_bwd_ring(bool post, int mode) { return post && mode != kGateChannel; }
-inline size_t norm_bwd_ring_smem(int threads, int mode) { return size_t(kNormBwdRows) * (mode == kGateElement ? 5 : 4) * 16 * threads; }
+__host__ __device__ constexpr size_t norm_bwd_ring_smem(int threads, int mode) { return size_t(kNormBwdRows) * (mode == kGateElement ? 5 : 4) * 16 * threads; }
 
 template <typename T, bool RMS, bool POST, int GATE, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResidualNormBwdArgs b) {
@@ -335,32 +335,35 @@ __global__ void __launch_bounds__(THREADS, 1) residual_norm_bwd_kernel(const __g
   if constexpr (!RMS) write(sum_B, kSums + 1);
 }
 
+template <typename T, bool RMS, bool POST, int GATE, bool WIDE, int THREADS>
+int norm_bwd_launch_kernel(ResidualNormBwdArgs b, cudaStream_t s) {
+  static std::atomic<uint64_t> smem_done{0};
+  constexpr bool kRing = sizeof(T) == 2 && WIDE && THREADS <= kNormBwdThreads && norm_bwd_ring(POST, GATE);
+  // what the widest row of this form takes: asked for once, since calls of other widths on other host threads launch the same kernel
+  constexpr int kMost = int(residual_norm_bwd_smem(THREADS, 1, POST, GATE) + (kRing ? norm_bwd_ring_smem(THREADS, GATE) : 0));
+  auto kernel = residual_norm_bwd_kernel<T, RMS, POST, GATE, WIDE, THREADS>;
+  const int threads = b.f.teams * b.f.team_threads;
+  size_t smem = residual_norm_bwd_smem(threads, b.f.teams, POST, GATE);
+  b.ring_at = (int)smem;
+  if (kRing) smem += norm_bwd_ring_smem(threads, GATE);
+  cudaError_t e = smem > kNormBwdPlainSmem ? allow_smem(smem_done, reinterpret_cast<const void*>(kernel), kMost) : cudaSuccess;
+  if (e == cudaSuccess) e = launch_kernel<ResidualNormBwdArgs>(kernel, b, dim3((unsigned)b.ctas), threads, smem, false, s);
+  if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm backward launch: %s", cudaGetErrorString(e));
+  return FDB_OK;
+}
+
 // WIDE stores of fp32 sums need rows of them to start on 16 bytes: they do, hidden being a multiple of 8 there.
-template <typename T, typename F>
-auto with_norm_bwd_kernel(bool rms, bool post, int mode, bool wide, int threads, F&& use) {
-#define FDB_BWD4(R, P, G, W) (threads <= kNormBwdThreads ? use(residual_norm_bwd_kernel<T, R, P, G, W, kNormBwdThreads>) : use(residual_norm_bwd_kernel<T, R, P, G, W, 1024>))
+template <typename T> int norm_bwd_launch(const ResidualNormBwdArgs& b, bool wide, cudaStream_t s) {
+  const bool narrow = b.f.teams * b.f.team_threads <= kNormBwdThreads;
+#define FDB_BWD4(R, P, G, W) (narrow ? norm_bwd_launch_kernel<T, R, P, G, W, kNormBwdThreads>(b, s) : norm_bwd_launch_kernel<T, R, P, G, W, 1024>(b, s))
 #define FDB_BWD3(R, P, G) (wide ? FDB_BWD4(R, P, G, true) : FDB_BWD4(R, P, G, false))
-#define FDB_BWD2(R, P) (mode == kGateChannel ? FDB_BWD3(R, P, kGateChannel) : (mode == kGateGroups ? FDB_BWD3(R, P, kGateGroups) : FDB_BWD3(R, P, kGateElement)))
-  if (rms) return post ? FDB_BWD2(true, true) : FDB_BWD2(true, false);
+#define FDB_BWD2(R, P) (b.mode == kGateChannel ? FDB_BWD3(R, P, kGateChannel) : (b.mode == kGateGroups ? FDB_BWD3(R, P, kGateGroups) : FDB_BWD3(R, P, kGateElement)))
+  const bool post = b.f.post_weight != nullptr;
+  if (b.f.rms) return post ? FDB_BWD2(true, true) : FDB_BWD2(true, false);
   return post ? FDB_BWD2(false, true) : FDB_BWD2(false, false);
 #undef FDB_BWD4
 #undef FDB_BWD3
 #undef FDB_BWD2
-}
-
-template <typename T> int norm_bwd_launch(const ResidualNormBwdArgs& args, bool wide, cudaStream_t s) {
-  ResidualNormBwdArgs b = args;
-  const int threads = b.f.teams * b.f.team_threads;
-  const bool post = b.f.post_weight != nullptr;
-  return with_norm_bwd_kernel<T>(b.f.rms, post, b.mode, wide, threads, [&](auto kernel) {
-    size_t smem = residual_norm_bwd_smem(threads, b.f.teams, post, b.mode);
-    b.ring_at = (int)smem;
-    if (sizeof(T) == 2 && wide && threads <= kNormBwdThreads && norm_bwd_ring(post, b.mode)) smem += norm_bwd_ring_smem(threads, b.mode);
-    cudaError_t e = smem > kNormBwdPlainSmem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-    if (e == cudaSuccess) e = launch_kernel<ResidualNormBwdArgs>(kernel, b, dim3((unsigned)b.ctas), threads, smem, false, s);
-    if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "residual_norm backward launch: %s", cudaGetErrorString(e));
-    return (int)FDB_OK;
-  });
 }
 
 }  // namespace fdb

@@ -105,3 +105,50 @@ def test_host_threads_at_once():
     assert not errors
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype,gate", [(torch.bfloat16, "sequence"), (torch.float16, "element"), (torch.float32, "sequence")])
+def test_backward_of_several_widths_on_host_threads_at_once(dtype, gate):
+    """One form of the norms' backward, rows of four widths, a host thread and a stream for each, through the C entry: what one
+    thread's launch needs of the kernel no other thread may take away."""
+    from flashdeberta_b200 import _lib, norms
+    lib = _lib.load()
+
+    def problem(hidden):
+        g = torch.Generator().manual_seed(hidden)
+        normal = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)
+        shape = (2, 3, hidden)
+        tensors = [normal(*shape), normal(*shape), normal(hidden), normal(hidden), normal(hidden), normal(hidden),
+                   normal(2, 1, hidden) if gate == "sequence" else normal(*shape)]
+        grads = [normal(*shape), normal(*shape)]
+        stats = norms._forward(*tensors, 1e-5, False, 1.0, True)[2]
+        outs = [torch.empty_like(t) for t in tensors]
+        head = norms._BWD.pack(norms._BWD.size + norms._FWD.size + norms._BWD_TAIL.size, 0) + norms._params(
+            *tensors, tensors[0], None, stats, 1e-5, False, 1.0)
+        at = [t.data_ptr() for t in grads + outs]
+        need = lib.fdb_residual_norm_bwd_workspace_bytes(head + norms._BWD_TAIL.pack(*at, 0, 0))
+        ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+        want = norms._backward(*grads, *tensors, stats, 1e-5, False, 1.0, (True,) * 7)
+        return head + norms._BWD_TAIL.pack(*at, ws.data_ptr(), need), outs, want, (tensors, grads, stats, ws)
+
+    problems = [problem(h) for h in (4096, 264, 2304, 1032)]
+    torch.cuda.synchronize()
+    streams, errors = [torch.cuda.Stream() for _ in problems], []
+
+    def run(i):
+        try:
+            torch.cuda.set_device(0)
+            for _ in range(400):
+                _lib.check(lib.fdb_residual_norm_bwd(problems[i][0], streams[i].cuda_stream))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(problems))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for _, outs, want, _ in problems:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
