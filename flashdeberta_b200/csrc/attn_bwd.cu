@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include "internal.h"
+#include "launch.h"
 
 namespace fdb {
 namespace {
@@ -365,12 +366,15 @@ extern "C" FDB_API int fdb_attn_bwd_bucket_sums(const fdb_bwd_block* p, void* st
   if (p->dscores == nullptr || p->table_rows <= 0)
     return fail(FDB_ERR_INVALID_ARGUMENT, "fdb_attn_bwd_bucket_sums: dscores and the bucket table are required");
   if (p->groups == 0 || p->rows == 0 || p->seqlen == 0) return FDB_OK;
+  // the limit that the checks below enforce, asked for once: calls of other sizes on other host threads launch the same kernels
+  constexpr size_t kSumsSmem = 200 * 1024;
+  static std::atomic<uint64_t> c2p_done{0}, p2c_done{0};
   if (p->c2p_sums != nullptr) {
     if (p->table_rows > 8192) return fail(FDB_ERR_LIMIT, "fdb_attn_bwd_bucket_sums: position tables of more than 8192 rows");
     const size_t smem_c = sizeof(float) * kCWarps * (size_t)p->table_rows + sizeof(int16_t) * (size_t)p->lut_len;
-    if (smem_c > 200 * 1024) return fail(FDB_ERR_LIMIT, "fdb_attn_bwd_bucket_sums: 32 * table_rows + 2 * lut_len bytes of shared memory exceed 200 KB");
+    if (smem_c > kSumsSmem) return fail(FDB_ERR_LIMIT, "fdb_attn_bwd_bucket_sums: 32 * table_rows + 2 * lut_len bytes of shared memory exceed 200 KB");
     if (smem_c > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(bwd_c2p_sums_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_c);
+      const cudaError_t e = allow_smem(c2p_done, reinterpret_cast<const void*>(bwd_c2p_sums_kernel), (int)kSumsSmem);
       if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "cudaFuncSetAttribute(bwd_c2p_sums_kernel): %s", cudaGetErrorString(e));
     }
     bwd_c2p_sums_kernel<<<dim3((p->rows + kCWarps - 1) / kCWarps, p->groups), kCThreads, smem_c, static_cast<cudaStream_t>(stream)>>>(*p);
@@ -378,10 +382,10 @@ extern "C" FDB_API int fdb_attn_bwd_bucket_sums(const fdb_bwd_block* p, void* st
   }
   if (p->p2c_sums != nullptr) {
     const size_t smem = sizeof(float) * kQKeys * (size_t)(p->table_rows + 2) + sizeof(int16_t) * ((size_t)p->rows + kQKeys);
-    if (smem > 200 * 1024)
+    if (smem > kSumsSmem)
       return fail(FDB_ERR_LIMIT, "fdb_attn_bwd_bucket_sums: 64 * (table_rows + 2) + 2 * (rows + 16) bytes of shared memory exceed 200 KB");
-    if (smem > 48 * 1024) {  // per device and cheap, so asked for on every such launch
-      const cudaError_t e = cudaFuncSetAttribute(bwd_p2c_sums_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > 48 * 1024) {
+      const cudaError_t e = allow_smem(p2c_done, reinterpret_cast<const void*>(bwd_p2c_sums_kernel), (int)kSumsSmem);
       if (e != cudaSuccess) return fail(FDB_ERR_CUDA, "cudaFuncSetAttribute(bwd_p2c_sums_kernel): %s", cudaGetErrorString(e));
     }
     bwd_p2c_sums_kernel<<<dim3((p->seqlen + kQKeys - 1) / kQKeys, p->groups), kQThreads, smem, static_cast<cudaStream_t>(stream)>>>(*p);

@@ -484,3 +484,50 @@ def test_heads_in_groups_give_the_same_gradients():
         for a, b in zip(got[3:], want[3:]):  # fp32 sums in two orders, then rounded: one bf16 step where they fall on either side
             assert ((a[h:h + 1].float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-4 * b.float().abs().max()).all()
     ops.check_status()
+
+
+def test_bucket_sums_of_several_sizes_on_host_threads_at_once():
+    """Tables of several sizes, a host thread and a stream for each, through the C entry: what one thread's launch needs of the kernel
+    no other thread may take away.  The scores are small whole numbers, so every order of the sums gives the same."""
+    import ctypes as C
+    import threading
+
+    from flashdeberta_b200 import _lib, backward
+
+    lib, S = _lib.load(), 64
+
+    def problem(table_rows):
+        g = torch.Generator().manual_seed(table_rows)
+        ds = torch.randint(-8, 9, (2, S, S), generator=g).float()
+        lut = (torch.arange(2 * S - 1) - (S - 1) + table_rows // 2).to(torch.int16)
+        index = (torch.arange(S)[:, None] - torch.arange(S)[None] + table_rows // 2).expand(2, S, S)
+        want = [torch.zeros(2, S, table_rows).scatter_add_(2, index, ds),
+                torch.zeros(2, S, table_rows).scatter_add_(2, index.transpose(1, 2), ds.transpose(1, 2))]
+        ds, lut = ds.bfloat16().to(DEV), lut.to(DEV)
+        outs = [torch.zeros(2, S, table_rows, device=DEV) for _ in range(2)]
+        p = backward._block_struct(dict(groups=2, heads=1, seqlen=S, row0=0, rows=S, table_rows=table_rows, lut_d_min=1 - S, lut_len=2 * S - 1,
+                                        sm_scale=1.0, seq_lens=None, lut=lut, status=None))
+        p.dscores, p.c2p_sums, p.p2c_sums = ds.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr()
+        return p, outs, want, (ds, lut)
+
+    problems = [problem(t) for t in (3000, 1800, 2400, 1600)]
+    torch.cuda.synchronize()
+    streams, errors, calls = [torch.cuda.Stream() for _ in problems], [], 300
+
+    def run(i):
+        try:
+            torch.cuda.set_device(0)
+            for _ in range(calls):
+                _lib.check(lib.fdb_attn_bwd_bucket_sums(C.byref(problems[i][0]), streams[i].cuda_stream))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(problems))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for _, (c2p, p2c), (want_c, want_p), _ in problems:
+        assert torch.equal(c2p.cpu(), want_c) and torch.equal(p2c.cpu(), calls * want_p)
