@@ -71,9 +71,11 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float lo, floa
 }
 
 // A pair of columns: the sums scaled, bias added, activation.
-template <bool GELU, bool FINE> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
+template <typename OUT, bool GELU> __device__ __forceinline__ uint64_t finish_pair(uint32_t a0, uint32_t a1, uint64_t w_scale, uint64_t x_scale, uint64_t bias) {
   const uint64_t v = fma_f32x2(mul_f32x2(pack_f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1)), w_scale), x_scale, bias);
-  return GELU ? gelu_tail2<FINE>(v) : v;
+  if constexpr (!GELU) return v;
+  else if constexpr (sizeof(OUT) == 4) return gelu_fine2(v);
+  else return gelu_tail2(v);
 }
 
 template <typename T> __device__ __forceinline__ float bias_at(const Int8Args& a, int n) {
@@ -97,8 +99,8 @@ __device__ __forceinline__ void convert_rows(const uint32_t (&acc)[A], uint64_t 
       const int c = p * kPiece + e;
       const float4 ws = *reinterpret_cast<const float4*>(cols + c), b = *reinterpret_cast<const float4*>(cols + COLS + c);
       float v0, v1, v2, v3;
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[AT + c], acc[AT + c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
-      unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[AT + c + 2], acc[AT + c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
+      unpack_f32x2(finish_pair<T, GELU>(acc[AT + c], acc[AT + c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v0, v1);
+      unpack_f32x2(finish_pair<T, GELU>(acc[AT + c + 2], acc[AT + c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v2, v3);
       if constexpr (sizeof(T) == 4) {
         o[0] = __float_as_uint(v0); o[1] = __float_as_uint(v1); o[2] = __float_as_uint(v2); o[3] = __float_as_uint(v3);
       } else {
@@ -121,8 +123,8 @@ __device__ __forceinline__ void store_turned(const Int8Args& a, const uint32_t (
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
     const float4 ws = *reinterpret_cast<const float4*>(cols + c), b = *reinterpret_cast<const float4*>(cols + COLS + c);
-    unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c], acc[c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v[c], v[c + 1]);
-    unpack_f32x2(finish_pair<GELU, sizeof(T) == 4>(acc[c + 2], acc[c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v[c + 2], v[c + 3]);
+    unpack_f32x2(finish_pair<T, GELU>(acc[c], acc[c + 1], pack_f32x2(ws.x, ws.y), sx, pack_f32x2(b.x, b.y)), v[c], v[c + 1]);
+    unpack_f32x2(finish_pair<T, GELU>(acc[c + 2], acc[c + 3], pack_f32x2(ws.z, ws.w), sx, pack_f32x2(b.z, b.w)), v[c + 2], v[c + 3]);
   }
   const int n = n0 + lane, rows = (int)min((int64_t)32, a.rows - row0);
   T* out = static_cast<T*>(a.out) + row0 * a.n + n;

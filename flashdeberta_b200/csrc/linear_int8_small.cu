@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) linear_int8_small_kernel(const __gri
     float b = 0.f;
     if (a.bias != nullptr) b = a.bias_fp32 ? __ldg(static_cast<const float*>(a.bias) + n) : to_float<OUT>(static_cast<const OUT*>(a.bias)[n]);
     float v = fmaf(__int2float_rn(sum) * __ldg(a.w_scale + n), s_scale[r], b), other;
-    if (a.gelu) ptx::unpack_f32x2(gelu_tail2<sizeof(OUT) == 4>(ptx::pack_f32x2(v, v)), v, other);
+    if (a.gelu) ptx::unpack_f32x2(sizeof(OUT) == 4 ? gelu_fine2(ptx::pack_f32x2(v, v)) : gelu_tail2(ptx::pack_f32x2(v, v)), v, other);
     static_cast<OUT*>(a.out)[(int64_t)r * a.n + n] = from_float<OUT>(v);
   }
 }

@@ -242,6 +242,26 @@ def test_gelu_over_its_range():
     _check(out, xq, xs, w, torch.ones(8), None, True)
 
 
+@pytest.mark.parametrize("rows", [1, 40, 3000])
+def test_gelu_in_fp32_holds_what_fp32_holds(rows):
+    """Values that reach the GELU unrounded (as the features' scales, everything else one).  Of q = |v| Phi(-|v|) the steps in fp32 leave
+    5.8 * 2^-24 where reciprocal and exponential are correctly rounded (all of them simulated over 0 < |v| < 13); the approximate ones
+    are documented to 2^-23 and 2^-22 relative, of which the reciprocal's counts at most twice and half a step of either is in the
+    simulation already: 2 and 4 more, 12 in all.  Half a step of the result, and nothing below fp32's smallest normal number."""
+    v = torch.cat([torch.linspace(-20, 20, 8001), -torch.logspace(-30, 1.1, 500), torch.logspace(-30, 30, 499)])
+    x = torch.ones(rows, 16, dtype=torch.int8, device=DEV)
+    w = torch.zeros(9000, 16, dtype=torch.int8, device=DEV)
+    w[:, 3] = 1
+    out = ops.linear_int8(x, w, v.to(DEV), x_scale=torch.ones(rows, device=DEV), gelu=True, out_dtype=torch.float32)
+    assert (out == out[:1]).all()
+    v = v.double()
+    q = 0.5 * v.abs() * torch.special.erfc(v.abs() / 2 ** 0.5)
+    want = v.clamp(min=0) - q
+    allowed = 12 * 2.0 ** -24 * q + 2.0 ** -24 * want.abs() + torch.finfo(torch.float32).tiny
+    worst = ((out[0].double().cpu() - want).abs() / allowed).max().item()
+    assert worst <= 1.0, f"{worst:.3g} times what is allowed"
+
+
 @pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) + 8, (1 << 32) + 8])
 def test_rows_that_are_too_long_are_refused(cols):
     """Before anything is read or copied, in the last case before 8 columns are left of them in 32 bits."""
