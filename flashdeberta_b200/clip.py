@@ -66,6 +66,7 @@ class _Listed:
             raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
         if len(cards) > 1:
             raise ValueError(f"{what} takes tensors of one device, got {sorted(cards)}")
+        ops.refuse_tangents(what, tensors)
         self.tensors, n = tensors, len(tensors)
         try:
             self.kind = np.fromiter(map(TYPES.__getitem__, map(_dtype, tensors)), np.int64, n)

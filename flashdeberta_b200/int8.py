@@ -69,6 +69,7 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"quantize_int8 takes rows of 1 to {MAX_COLS} elements")
     if ops.intercepted(x):
         raise RuntimeError("quantize_int8 goes by the memory of plain tensors: call it outside tracing, or linear_int8, which rounds within")
+    ops.refuse_tangents("quantize_int8", (x,))
     cols = x.shape[-1]
     x = x if x.is_contiguous() else x.contiguous()
     q = torch.empty(*x.shape[:-1], _pitch(cols), dtype=torch.int8, device=x.device)[..., :cols]
@@ -144,6 +145,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
     if ops.wants_grad(x, weight_scale, bias, x_scale):
         raise RuntimeError("the 8-bit linear layer is forward-only; call under torch.no_grad() or detach the inputs")
+    ops.refuse_tangents("the 8-bit linear layer", (x, weight_scale, bias, x_scale))
     if weight.dtype != torch.int8 or weight.dim() != 2 or weight_scale.dtype != torch.float32 or weight_scale.shape != weight.shape[:1]:
         raise ValueError("weight must be int8 (out_features, in_features) with float32 weight_scale (out_features,)")
     if x.dim() < 1 or x.shape[-1] != weight.shape[1]:

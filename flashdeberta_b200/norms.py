@@ -190,6 +190,7 @@ def _setup(ctx, inputs, output):
 
 def _op_backward(ctx, dnormed, dstream, _):
     *tensors, stats = ctx.saved_tensors
+    ops.refuse_tangents("the backward of residual_norm", (dnormed, dstream))
     x = tensors[0]
     dnormed, dstream = (torch.zeros_like(x) if g is None else g for g in (dnormed, dstream))
     grads = residual_norm_bwd_op(dnormed, dstream, *tensors, stats, *ctx.norm_args)
@@ -216,6 +217,7 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dnormed, dstream):
         if ops.intercepted(dnormed, dstream) or any(g is not None and ops.batched(g) for g in (dnormed, dstream)):
             return _op_backward(ctx, dnormed, dstream, None)
+        ops.refuse_tangents("the backward of residual_norm", (dnormed, dstream))
         grads = _backward(dnormed, dstream, *ctx.saved_tensors, *ctx.norm_args, ctx.needs_input_grad)
         return (*grads, None, None, None)
 
@@ -231,10 +233,12 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: tor
     is.  ``gate`` broadcasts to x: (hidden,) a gate per channel, (batch, 1, hidden) one per sequence, x's shape one per element; None is
     a gate of one.  ``residual`` may be None.  Rows are bfloat16, float16 or float32; the norms' parameters are of that type or all
     float32, the gate of either.  Statistics and sums are float32, every result is rounded once (``normed`` is made of the stream
-    before it is rounded).  Gradients of every input, in the inputs' types; no second derivative."""
+    before it is rounded).  Gradients of every input, in the inputs' types; no second derivative, and none in
+    forward mode."""
     gate = _gate_of(x, residual, weight, bias, post_weight, post_bias, gate, rms)
     tensors = (x, residual, weight, bias, post_weight, post_bias, gate)
     eps, rms, residual_scale = float(eps), bool(rms), float(residual_scale)
+    ops.refuse_tangents("residual_norm", tensors)
     if ops.intercepted(*tensors):
         return residual_norm_op(*tensors, eps, rms, residual_scale)[:2]
     if torch.is_grad_enabled():

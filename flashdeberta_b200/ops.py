@@ -16,6 +16,7 @@ import math
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.nn.modules import module as _nn_module
 
 from . import _lib, bucket
@@ -132,6 +133,15 @@ def intercepted(*tensors) -> bool:
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 #: whether a tensor is a gradient of ``torch.autograd.grad(..., is_grads_batched=True)``
 batched = torch._C._functorch.is_legacy_batchedtensor
+
+
+def refuse_tangents(what: str, tensors) -> None:
+    """Raises where one of the tensors carries a forward-mode derivative (``torch.autograd.forward_ad``, ``torch.func.jvp``): calls that
+    go by addresses would lose it without a word, and no operator here computes one."""
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: call it on the primal values")
 
 
 def capturing(t: torch.Tensor) -> bool:

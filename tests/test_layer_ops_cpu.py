@@ -212,6 +212,21 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    x = torch.ones(3)
+    ops.refuse_tangents("it", (x, None))
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones(3))
+        ops.refuse_tangents("it", (x, None))
+        for bad in ((dual,), (None, x, dual)):
+            with pytest.raises(RuntimeError, match="it has no forward-mode"):
+                ops.refuse_tangents("it", bad)
+    ops.refuse_tangents("it", (dual,))  # (the tangent ended with its level)
+    with pytest.raises(RuntimeError, match="no forward-mode"):
+        torch.func.jvp(lambda v: ops.refuse_tangents("it", (v,)) or v, (x,), (x,))
+
+
 def test_empty_lists_of_gradients():
     assert ops.grad_norm([]).item() == 0.0 and ops.clip_grads_([], 1.0).item() == 0.0
     assert ops.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0).item() == 0.0  # no gradient there

@@ -152,3 +152,27 @@ def test_backward_of_several_widths_on_host_threads_at_once(dtype, gate):
     assert not errors, errors
     for _, outs, want, _ in problems:
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Rather than lost: results of tensors with a tangent would have none."""
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.randn(4, 64, device=DEV), torch.ones(64, device=DEV)
+    q, s = ops.quantize_int8(torch.randn(48, 64, device=DEV))
+    want = ops.residual_norm(x, x, w)
+    one = torch.ones_like(x)
+    with fwd.dual_level():
+        dual, scale = fwd.make_dual(x, one), fwd.make_dual(s, torch.ones_like(s))
+        for bad in (lambda: ops.residual_norm(dual, x, w), lambda: ops.residual_norm(x, dual, w), lambda: ops.residual_norm(x, x, fwd.make_dual(w, w)),
+                    lambda: ops.quantize_int8(dual), lambda: ops.linear_int8(dual, q, s), lambda: ops.linear_int8(x, q, scale),
+                    lambda: ops.grad_norm([x, dual]), lambda: ops.clip_grads_([dual], 1.0), lambda: ops.clip_grads_([x], 1.0, out=[dual])):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                bad()
+        got = ops.residual_norm(x, x, w)  # (nothing here has a tangent)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert ops.linear_int8(x, q, s).shape == (4, 48) and abs(ops.grad_norm([x]).item() - x.norm().item()) < 1e-4
+        leaf = x.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.autograd.grad(ops.residual_norm(leaf, x, w)[0], leaf, fwd.make_dual(one, one))
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda v: ops.residual_norm(v, x, w), (x,), (one,))
