@@ -46,6 +46,74 @@ def _apart(writes, reads=()) -> bool:
     return True
 
 
+def _layout(t: torch.Tensor):
+    """(first byte, bytes of a run without gaps, [(bytes between, count)] of what the runs are repeated over)."""
+    run, outer = t.element_size(), []
+    for stride, size in sorted((s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride == run and not outer:
+            run *= size
+        else:
+            outer.append((stride, size))
+    return t.data_ptr(), run, outer
+
+
+def _starts(at, run, outer) -> np.ndarray:
+    """Where the runs begin, in order."""
+    starts = np.array([at], np.int64)
+    for stride, size in outer:
+        starts = (starts[:, None] + stride * np.arange(size, dtype=np.int64)).ravel()
+    return np.sort(starts)
+
+
+def _folded(at, run, outer) -> bool:
+    """Whether two elements of a tensor lie in the same place."""
+    span = run
+    for stride, size in outer:
+        if stride < span:  # (an expanded dimension, or windows that slide)
+            return bool((np.diff(_starts(at, run, outer)) < run).any())
+        span += stride * (size - 1)
+    return False
+
+
+def _apart_modulo(layouts) -> bool:
+    """Whether the runs keep apart modulo what all strides are multiples of: slices of one matrix's columns do.  (They may be
+    apart without that.)"""
+    period = math.gcd(*(stride for _, _, outer in layouts for stride, _ in outer))
+    if period == 0:
+        return False
+    runs = sorted((at % period, run) for at, run, _ in layouts)
+    return all(a + n <= b for (a, n), (b, _) in zip(runs, runs[1:] + [(runs[0][0] + period, 0)]))
+
+
+def _cross(a, b) -> bool:
+    """Whether two tensors have an element in the same place."""
+    if _apart_modulo((a, b)):
+        return False
+    (sa, ra), (sb, rb) = (_starts(*a), a[1]), (_starts(*b), b[1])
+    near = np.searchsorted(sa, sb + rb) - 1  # the last run that begins before each of b's ends
+    return bool(((near >= 0) & (sa[near] + ra > sb)).any())
+
+
+def _collide(writes, reads) -> bool:
+    """Whether an element that is written is also another one that is written, or one that is read."""
+    placed = [(_layout(t), True) for t in writes] + [(_layout(t), False) for t in reads]
+    if any(writes and _folded(*layout) for layout, writes in placed):
+        return True
+    placed = sorted(((at, at + run + sum(s * (n - 1) for s, n in outer), (at, run, outer), w) for (at, run, outer), w in placed), key=lambda p: p[:2])
+    group, end = [], 0
+    for p in placed + [(math.inf, math.inf, None, False)]:
+        if p[0] >= end:  # nothing so far reaches further: a group of tensors in one another's way
+            if any(g[3] for g in group) and len(group) > 1 and not _apart_modulo([g[2] for g in group]):
+                for i, a in enumerate(group):
+                    for b in group[i + 1:]:
+                        if (a[3] or b[3]) and b[0] < a[1] and _cross(a[2], b[2]):
+                            return True
+            group = []
+        group.append(p)
+        end = max(end, p[1])
+    return False
+
+
 _at, _count, _whole, _card = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
 _dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 _PLAIN = {torch.Tensor, torch.nn.Parameter}
@@ -137,8 +205,9 @@ def grad_norm(grads: Tensors, norm_type: float = 2.0) -> torch.Tensor:
 def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))``, norm as in ``grad_norm``, in place, or into ``out`` (tensors of the same
     shapes, of any of the three types: an optimizer's float32 buffers beside bfloat16 gradients), and returns the norm before.  Nothing
-    is read back to the host.  Where the factor is one, tensors scaled in place are not written.  The tensors that are written must not
-    overlap one another or, but for a tensor that is its own output, those that are read."""
+    is read back to the host.  Where the factor is one, tensors scaled in place are not written (but for those with gaps in memory,
+    which go through a copy).  The tensors that are written must not overlap one another or, but for a tensor that is its own
+    output, those that are read."""
     norm_type, grads = _norm_type(norm_type), _Listed(grads, "clip_grads_")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -158,16 +227,17 @@ def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out:
 @torch.no_grad()
 def _clip_any(grads, outs, max_norm, norm_type):
     """The kernel goes through memory: a tensor that is no run of it, or is ordered unlike its output, is taken through a copy."""
+    pairs = [(g, o) for g, o in zip(grads, outs) if g.numel() > 0]
+    if any(g.data_ptr() == o.data_ptr() and g.dtype != o.dtype for g, o in pairs):
+        raise ValueError("a gradient cannot be scaled in place into another type")
+    if _collide([o for _, o in pairs], [g for g, o in pairs if g.data_ptr() != o.data_ptr()]):
+        raise ValueError("the tensors that are written overlap one another or a gradient that is read")
     reads, writes, back = [], [], []
-    for g, o in zip(grads, outs):
-        if g.numel() == 0:
-            continue
+    for g, o in pairs:
         if (g.is_contiguous() and o.is_contiguous()) or (_dense(g) and _dense(o) and g.stride() == o.stride()):
             reads.append(g)
             writes.append(o)
             continue
-        if g.data_ptr() == o.data_ptr() and g.dtype != o.dtype:
-            raise ValueError("a gradient cannot be scaled in place into another type")
         reads.append(g.contiguous())
         writes.append(o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device))
         if writes[-1] is not o:

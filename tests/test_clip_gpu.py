@@ -200,6 +200,29 @@ def test_refusals():
     assert abs(ops.grad_norm([a, a]).item() - math.sqrt(200)) < 1e-4  # (read twice, counted twice)
 
 
+def test_strided_tensors_that_overlap_are_refused():
+    """As tensors without gaps are, and before anything is scaled."""
+    m, other = torch.ones(30, 90, device=DEV), torch.full((30, 7), 3.0, device=DEV)
+    out = torch.zeros(30, 90, device=DEV)
+    t = m[:, 3:80]
+    for bad in (lambda: ops.clip_grads_([t, t], 1.0), lambda: ops.clip_grads_([other, m[:, :10], m[:, 9:20]], 1.0), lambda: ops.clip_grads_([t, m], 1.0),
+                lambda: ops.clip_grads_([other, other.clone()], 1.0, out=[out[:, :7], out[:, 5:12]]), lambda: ops.clip_grads_([m[:, ::2], m[:, ::3]], 1.0),
+                lambda: ops.clip_grads_([m[:, :7], other], 1.0, out=[out[:, :7], m[:, 6:13]]), lambda: ops.clip_grads_([m[:1].expand(5, 90)], 1.0),
+                lambda: ops.clip_grads_([m[:, :7].contiguous()], 1.0, out=[out[:1, :7].expand(30, 7)]),
+                lambda: ops.clip_grads_([m.t()[:10], m.t()[9:]], 1.0)):
+        with pytest.raises(ValueError, match="overlap"):
+            bad()
+    assert (m == 1).all() and (other == 3).all() and (out == 0).all()
+    norm = ops.clip_grads_([m[:, :40], m[:, 40:41], m[:, 41:]], 1.0)  # slices beside one another
+    assert abs(norm.item() - 2700 ** 0.5) < 1e-4 and (m == m[0, 0]).all() and abs(m[0, 0].item() - 2700 ** -0.5) < 1e-6
+    m.fill_(1.0)
+    assert abs(ops.clip_grads_([m[:, ::2], m[:, 1::2]], 1.0).item() - 2700 ** 0.5) < 1e-4 and (m == m[0, 0]).all()
+    square = torch.arange(64.0, device=DEV).view(8, 8)  # its own output in another order
+    want = square.t() / square.norm()
+    ops.clip_grads_([square[:, :]], 1.0, out=[square.t()])
+    torch.testing.assert_close(square, want, rtol=1e-5, atol=0)
+
+
 def test_streams_and_captures():
     ts = _tensors([(500, 600), 333, (64, 64)], 8)
     kept = [t.clone() for t in ts]

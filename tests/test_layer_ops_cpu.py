@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from flashdeberta_b200 import _lib, ops
-from flashdeberta_b200.clip import _apart, _dense
+from flashdeberta_b200.clip import _apart, _collide, _dense
 from flashdeberta_b200.int8 import _rows, int8_rows
 from flashdeberta_b200.norms import _gate_rows
 from tests.test_abi_cpu import _refused, test_other_struct_layouts_match_the_header as _layout
@@ -201,6 +201,43 @@ def test_tensors_that_fill_their_memory():
     t = torch.zeros(3, 4, 5)
     assert _dense(t) and _dense(t.permute(2, 0, 1)) and _dense(t[1:2]) and _dense(t[:, :1].contiguous().transpose(0, 1)) and _dense(torch.zeros(()))
     assert not _dense(t[:, 1:]) and not _dense(t[..., ::2]) and not _dense(torch.zeros(1, 4).expand(3, 4))
+
+
+def test_elements_in_one_place():
+    m = torch.zeros(12, 35)
+    apart = [[m[:, :10], m[:, 10:20], m[:, 20:]], [m[:, ::2], m[:, 1::2]], [m[::2], m[1::2]], [m[::3, 1::2], m[1::3], m[2::3, ::7], m[::3, ::2]],
+             [m[:6], m[6:, :4], m[6:, 4:]], [m.t()[:7], m[:, 7:].t()], [m.view(-1)[::6], m.view(-1)[1::6], m.view(-1)[2::3]], [m[:, 34], m[:, 0]],
+             [m.view(3, 4, 35)[:, 1:3, 5], m.view(3, 4, 35)[:, 1:3, 6:9], m.view(3, 4, 35)[:, ::3]], [m.bfloat16(), m[:, 1:]], []]
+    for ts in apart:
+        assert not _collide(ts, []) and not _collide(ts[:1], ts[1:]) and not _collide([], ts + ts)
+    together = [[m[:, 1:], m[:, 1:]], [m[:, :10], m[:, 9:20]], [m[:, ::2], m[:, ::3]], [m[:6, 1:], m[5:, ::2]], [m, m[3, 5:6]], [m[::2, :4], m.t()[3]],
+                [m.view(-1)[::6], m.view(-1)[::4]], [m[:, 1:], m.view(torch.bfloat16)[7:9, 4:5]]]
+    for a, b in together:
+        assert _collide([a, b], []) and _collide([b], [a]) and _collide([a], [b]) and _collide([m.clone()[:, 2:], b, a], []) and not _collide([], [a, b])
+    for t in (m[:1].expand(4, 35), m.view(-1).as_strided((5, 4), (3, 1)), m[:, :1].expand(12, 3)):
+        assert _collide([t], []) and not _collide([], [t]) and not _collide([m.clone()], [t])
+    for t in (m.as_strided((5, 4), (2, 3)), m.as_strided((3, 2), (2, 3))):  # 2 i + 3 j: twice six, or never twice
+        places = {2 * i + 3 * j for i in range(t.shape[0]) for j in range(t.shape[1])}
+        assert _collide([t], []) == (len(places) < t.numel())
+    assert _collide([m.as_strided((5, 4), (2, 3))], []) and not _collide([m.as_strided((3, 2), (2, 3))], [])
+
+
+def test_elements_in_one_place_against_a_list_of_them():
+    gen = torch.Generator().manual_seed(0)
+    pick = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=gen))
+    base, seen = torch.zeros(400), set()
+    for _ in range(400):
+        views = []
+        for _ in range(pick(1, 4)):
+            shape = [pick(1, 5) for _ in range(pick(1, 4))]
+            views.append(base.as_strided(shape, [pick(0 if pick(0, 6) == 0 else 1, 24) for _ in shape], pick(0, 60)))
+        places = [torch.arange(400).as_strided(v.shape, v.stride(), v.storage_offset()).flatten().tolist() for v in views]
+        cut = pick(1, len(views) + 1)
+        written = sum(places[:cut], [])
+        want = len(set(written)) < len(written) or bool(set(written) & set(sum(places[cut:], [])))
+        assert _collide(views[:cut], views[cut:]) == want, [(v.shape, v.stride(), v.storage_offset()) for v in views]
+        seen.add(want)
+    assert seen == {True, False}
 
 
 # ---- the Python layer ----------------------------------------------------------------------------------------------------
