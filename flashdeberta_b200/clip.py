@@ -1,4 +1,4 @@
-"""The global norm of a model's gradients, and clipping by it: two launches however many tensors there are.
+"""The global norm of a model's gradients, and clipping by it: two launches for every thousand tensors.
 
 The reference leaves this step of training to torch (its models are trained by transformers' Trainer over
 src/flashdeberta/model.py:394-920), which launches over lists of tensors per type and keeps the norms of the single tensors.
@@ -19,6 +19,7 @@ from .norms import TYPES
 
 Tensors = Union[torch.Tensor, Iterable[torch.Tensor]]
 _NORMS = {1.0: 1, 2.0: 2, math.inf: 0}
+_TABLE = 1000  # tensors that a launch takes
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -180,7 +181,8 @@ def _run(grads: _Listed, outs: Optional[_Listed], max_norm: float, norm_type: fl
         _lib.check(lib.fdb_clip_grads(C.byref(p), ops.raw_stream(device)))
     if outs is not None:  # the write is seen by whoever compares versions (autograd, the caches of this package)
         torch.autograd.graph.increment_version(outs.tensors)
-    ops._launches += 2
+    tables = -(-len(at) // _TABLE)
+    ops._launches += tables + (tables if outs is not None else 1)
     return norm
 
 

@@ -1,5 +1,5 @@
-// Norm over many tensors taken as one vector, and the tensors scaled to a bound on it (fdb_clip_grads): two launches however many
-// tensors there are.
+// Norm over many tensors taken as one vector, and the tensors scaled to a bound on it (fdb_clip_grads): two launches for every thousand
+// tensors (the norm alone: one, and one more for all).
 //
 // norm_kernel: the tensors are cut into chunks of 16384 elements, a CTA takes one run of chunks; squares (or magnitudes) are summed in
 // fp32 over the 32 elements that a thread has in registers, those sums in fp64.  A sum of 32 that has left fp32's comfortable range

@@ -132,6 +132,17 @@ def test_many_tensors(count):
     _check([flat], [kept], 1.0 / (want + 1e-6))
 
 
+@pytest.mark.parametrize("count,tables", [(1, 1), (1000, 1), (1001, 2), (2300, 3)])
+def test_launches_are_counted(count, tables):
+    """A launch takes a thousand tensors: that many for the norm, as many again to scale or one to join the norm."""
+    ts = list(torch.ones(count * 3, device=DEV).split(3))
+    before = ops.launch_count()
+    ops.grad_norm(ts)
+    assert ops.launch_count() - before == tables + 1
+    ops.clip_grads_(ts, 1.0)
+    assert ops.launch_count() - before == 3 * tables + 1
+
+
 def test_tensors_that_start_anywhere():
     base = torch.randn(50000, device=DEV, generator=torch.Generator(DEV).manual_seed(6))
     for dtype in TYPES:
