@@ -149,7 +149,9 @@ def _backward(dnormed, dstream, x, residual, weight, bias, post_weight, post_bia
         need = lib.fdb_residual_norm_bwd_workspace_bytes(head + _BWD_TAIL.pack(*addresses, 0, 0))
     ws = x.new_empty(need, dtype=torch.uint8)
     ops.call_on(device, lib.fdb_residual_norm_bwd, head + _BWD_TAIL.pack(*addresses, ws.data_ptr(), need))
-    ops._launches += 1 + int(any(g is not None for g in grads[2:]))
+    # (the gradient of a gate per element is no sum over rows)
+    summed = any(g is not None for g in grads[2:6]) or (grads[6] is not None and (grads[6].numel() < x.numel() or x.numel() == x.shape[-1]))
+    ops._launches += 1 + int(summed)
     return grads
 
 

@@ -342,6 +342,21 @@ def test_refusals():
             bad()
 
 
+@pytest.mark.parametrize("gate,wanted,launches", [
+    (None, ("x",), 1), (None, ("x", "bias"), 2), ((64,), ("gate",), 2), ((2, 1, 64), ("x", "gate"), 2), ((2, 3, 64), ("x", "gate"), 1),
+    ((2, 3, 64), ("gate", "post_weight"), 2), ((2, 1, 64), ("residual",), 1)])
+def test_launches_are_counted(gate, wanted, launches):
+    """One for the rows, one more where a gradient is a sum over them."""
+    t, grads = _inputs((2, 3, 64), torch.float32, False, True, gate, 21)
+    for k in wanted:
+        t[k].requires_grad_()
+    before = ops.launch_count()
+    out = _call(t)
+    assert ops.launch_count() - before == 1
+    torch.autograd.grad(out, [t[k] for k in wanted], grads)
+    assert ops.launch_count() - before == 1 + launches
+
+
 def test_in_a_layer_beside_add_layernorm():
     """The tail of this package's own output blocks: the same result as ops.add_layernorm up to the sum that it rounds first."""
     t, _ = _inputs((64, 768), torch.bfloat16, False, False, None, 18)
