@@ -1,4 +1,5 @@
-// The 8-bit linear layer for a few tokens (fdb_linear_int8 with up to 32 rows): one launch, the rounding of the tokens included.
+// The 8-bit linear layer for a few tokens (fdb_linear_int8 with up to 32 rows, of integers up to 8): one launch, the rounding of the tokens
+// included.
 //
 // What there is to do is to read the weight once and to wait for little else, so this kernel is built for latency: no tensor memory to
 // allocate, no copies to set up, the weight goes straight into the registers of warp-level matrix instructions (mma.sync, 16 features
@@ -216,7 +217,8 @@ int launch(const SmallArgs& a, size_t smem, cudaStream_t s) {
 
 template <typename X, typename OUT>
 int launch_tokens(const SmallArgs& a, int tg, size_t smem, cudaStream_t s) {
-  return tg == 1 ? launch<X, OUT, 1>(a, smem, s) : (tg == 2 ? launch<X, OUT, 2>(a, smem, s) : launch<X, OUT, 4>(a, smem, s));
+  if constexpr (sizeof(X) == 1) return launch<X, OUT, 1>(a, smem, s);  // (int8_is_small: one round)
+  else return tg == 1 ? launch<X, OUT, 1>(a, smem, s) : (tg == 2 ? launch<X, OUT, 2>(a, smem, s) : launch<X, OUT, 4>(a, smem, s));
 }
 template <typename X>
 int launch_type(const SmallArgs& a, int out_dtype, int tg, size_t smem, cudaStream_t s) {
