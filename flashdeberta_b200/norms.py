@@ -84,7 +84,8 @@ def _gate_of(x, residual, weight, bias, post_weight, post_bias, gate, rms):
         raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms)
     if gate.shape != vector and (gate.dim() == 0 or _gate_rows(gate, shape) is None):  # shared in some other way: one per element then
         try:
-            return gate.expand(shape)
+            # (its gradient is summed where it is shared: of numbers that are not rounded before)
+            return (gate.float() if gate.requires_grad and torch.is_grad_enabled() else gate).expand(shape)
         except RuntimeError:
             raise _refusal(x, residual, weight, bias, post_weight, post_bias, gate, rms) from None
     return gate

@@ -184,6 +184,14 @@ def test_gate_that_broadcasts_in_another_way():
         _compare(t, grads)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 9, 136), (4, 9, 1), (9, 1), (4, 1, 1), (1,)])
+def test_gradient_of_a_shared_gate_is_rounded_once(dtype, shape):
+    """The sum over what shares a number of the gate, of parts that have not been rounded to the gate's type."""
+    t, grads = _inputs((4, 9, 136), dtype, False, True, shape, 23)
+    _compare(t, grads)
+
+
 def test_one_gradient_and_only_what_is_asked_for():
     t, grads = _inputs((2, 17, 320), torch.float32, False, True, (320,), 8)
     want, bound = _want(t, (grads[0], torch.zeros_like(grads[1])), 1e-5, False, 1.0)
