@@ -195,7 +195,7 @@ def _norm_type(norm_type: float) -> float:
 
 def grad_norm(grads: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm (1, 2 or inf) over all elements of the tensors taken as one vector: a float32 scalar on their device, zero where there
-    are none.  Tensors are bfloat16, float16 or float32 in any mixture, of one device."""
+    are none.  Tensors are bfloat16, float16 or float32 in any mixture, of one device.  As torch's own, it records no gradient."""
     norm_type, grads = _norm_type(norm_type), _Listed(grads, "grad_norm")
     if not grads.tensors:
         return torch.tensor(0.0)
@@ -254,7 +254,8 @@ def _clip_any(grads, outs, max_norm, norm_type):
 
 def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_`` over this package's kernels: the gradients of the parameters that have one are clipped in
-    place to ``max_norm``; returns their norm before.  ``error_if_nonfinite`` reads the norm back to the host first (and raises before
+    place to ``max_norm``; returns their norm before.  Narrower than torch's: plain bfloat16, float16 or float32 tensors of one device,
+    and norms 1, 2 and inf; anything else raises.  ``error_if_nonfinite`` reads the norm back to the host first (and raises before
     anything is scaled); without it nothing is read back."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads = [p.grad for p in parameters if p.grad is not None]

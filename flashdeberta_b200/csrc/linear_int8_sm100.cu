@@ -9,8 +9,8 @@
 //           store.  Scales and biases of the next tile are fetched while one is worked on.
 // Bound by the tensor cores at the power limit where K is long, by the epilogue where it is short (4800 clocks a 256 x 256 tile, with the
 // GELU 8700, against 680 per 128 of K).  Measured: 16384 x 4096 -> 4096 167 us = 3.30 POP/s (twice the measured bf16 rate is 3.31);
-// 16384 x 4096 -> 1024 49 us = 2.81; 16384 x 1024 -> 4096 54 us = 2.55, with the GELU 66 us = 2.09; 16384 x 256 -> 4096 32 us, 134 MB
-// written.  On the way (16384 x 1024 -> 4096 with GELU, the product alone): eight epilogue warps that store from registers 137 us;
+// 16384 x 4096 -> 1024 49 us = 2.81; 16384 x 1024 -> 4096 54 us = 2.55, with the GELU 66 us = 2.09 (fp32 results 72 and 92 us); 16384 x 256 -> 4096 32 us,
+// 134 MB written.  On the way (16384 x 1024 -> 4096 with GELU, the product alone): eight epilogue warps that store from registers 137 us;
 // sixteen 90; TMA stores 84; scales a tile ahead 73; tensor memory handed over without a cluster-wide release 66.
 // Every wait is bounded; on a timeout the CTA raises FDB_DEV_TIMEOUT in the status word, frees its tensor memory and returns.
 // No TMA multicast.

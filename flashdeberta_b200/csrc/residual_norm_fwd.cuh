@@ -20,10 +20,14 @@ using ptx::mul_f32x2;
 // (and a channel's gate) are converted to fp32 once, into shared memory, and the next rows are on their way while one is worked on.
 constexpr int kNormFwdWarpElems = 1024;
 constexpr int kNormFwdThreads = 512;  // of a CTA of longer rows, one per SM (at most 128 registers a thread)
-// Whether 16-bit rows of one warp are on their way in shared memory, two ahead, instead of one ahead in registers.  16 M elements, registers
-// against shared memory, both LayerNorms with a gate per sequence, then one LayerNorm: 256 columns 37 and 31 us, 24 and 21; 512 30 and 27, 23
-// and 20; 768 28 and 27, 22 and 21 (with a
-// gate per channel 24 and 26); 1024 29 and 28, 21 and 21.5 (with a gate per element 24 and 25.5).
+// Whether 16-bit rows of one warp are on their way in shared memory, two ahead, instead of one ahead in registers.  16 M elements in bf16,
+// registers against shared memory, without a gate, one per channel, per sequence, per element:
+//    256 columns, LayerNorms on both sides  34.9 35.5 39.2 41.0 and 29.3 30.8 33.7 36.5    one LayerNorm  26.7 27.4 31.5 33.9 and 26.6 26.7 27.1 31.0 us
+//    512                                    29.1 30.8 33.0 35.0     27.4 29.5 30.8 32.8                   26.5 26.8 28.0 32.3     25.9 26.4 25.8 30.5
+//    768                                    27.0 27.1 30.9 34.0     26.9 28.9 31.1 34.4                   25.9 26.5 27.4 31.0     26.4 26.7 27.0 31.0
+//   1024                                    30.7 31.9 32.7 36.9     27.6 30.0 32.1 34.0                   25.8 26.6 26.3 30.9     25.7 26.4 27.3 31.0
+// RMS norms gain at 256 and 512 (both sides 30.8 and 26.8, 27.2 and 25.6) and are even at 768 and 1024.  Only both LayerNorms at 768 with a gate
+// per channel lose (27.1 and 28.9); the gate is no part of the rule, which would take another set of kernels for that one form.
 constexpr int kNormFwdRows = 2;
 template <typename T> __host__ __device__ constexpr bool norm_fwd_ring(bool rms, bool post, bool wide, int v, bool one) {
   return sizeof(T) == 2 && wide && one && (v < 4 || (post && !rms));

@@ -60,7 +60,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows as 8-bit integers with a scale each: ``scale = amax / 127``, ``q = round(x * (127 / amax))``, ties to even, in float32.  x:
     (..., cols) bfloat16, float16 or float32; returns int8 of x's shape (rows start on 16 bytes) and float32 of shape ``x.shape[:-1]``.
     The same call scales the tokens of an activation and the output channels of a weight.  Rows of zeros (or below 2^-100) have scale
-    zero; rows with an infinity or NaN have integers zero and a scale that makes NaN of whatever is multiplied by it."""
+    zero; rows with an infinity or NaN have integers zero and a scale that makes NaN of whatever is multiplied by it.
+    No gradient is recorded; rows have at most 2^30 elements."""
     if not x.is_cuda:
         raise RuntimeError("flashdeberta_b200 runs on CUDA devices only; there is no CPU path")
     if x.dtype not in TYPES:

@@ -262,6 +262,18 @@ def test_gelu_in_fp32_holds_what_fp32_holds(rows):
     assert worst <= 1.0, f"{worst:.3g} times what is allowed"
 
 
+@pytest.mark.parametrize("rows", [2, 60])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gelu_of_what_is_not_finite_and_of_the_largest(rows, dtype):
+    v = torch.tensor([float("inf"), -float("inf"), float("nan"), 3e38, -3e38, 0.0, -0.0, 1e-45]).to(DEV)
+    x = torch.ones(rows, 16, dtype=torch.int8, device=DEV)
+    w = torch.zeros(8, 16, dtype=torch.int8, device=DEV)
+    w[:, 3] = 1
+    out = ops.linear_int8(x, w, v, x_scale=torch.ones(rows, device=DEV), gelu=True, out_dtype=dtype)
+    assert (out[:, 0] == float("inf")).all() and (out[:, 1] == 0).all() and torch.isnan(out[:, 2]).all()
+    assert (out[:, 3] == v[3].to(dtype)).all() and (out[:, 4:7] == 0).all() and (out[:, 7].abs() <= 1e-45).all()
+
+
 @pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) + 8, (1 << 32) + 8])
 def test_rows_that_are_too_long_are_refused(cols):
     """Before anything is read or copied, in the last case before 8 columns are left of them in 32 bits."""
