@@ -95,12 +95,16 @@ def _cross(a, b) -> bool:
     return bool(((near >= 0) & (sa[near] + ra > sb)).any())
 
 
+def _end(at, run, outer) -> int:
+    return at + run + sum(stride * (size - 1) for stride, size in outer)
+
+
 def _collide(writes, reads) -> bool:
     """Whether an element that is written is also another one that is written, or one that is read."""
     placed = [(_layout(t), True) for t in writes] + [(_layout(t), False) for t in reads]
     if any(writes and _folded(*layout) for layout, writes in placed):
         return True
-    placed = sorted(((at, at + run + sum(s * (n - 1) for s, n in outer), (at, run, outer), w) for (at, run, outer), w in placed), key=lambda p: p[:2])
+    placed = sorted(((layout[0], _end(*layout), layout, w) for layout, w in placed), key=lambda p: p[:2])
     group, end = [], 0
     for p in placed + [(math.inf, math.inf, None, False)]:
         if p[0] >= end:  # nothing so far reaches further: a group of tensors in one another's way
@@ -223,19 +227,48 @@ def clip_grads_(grads: Tensors, max_norm: float, *, norm_type: float = 2.0, out:
         raise ValueError(f"out is on {outs.tensors[0].device}, the gradients on {grads.tensors[0].device}")
     if grads.whole() and (out is None or outs.whole()):
         return _run(grads, outs, max_norm, norm_type)
-    return _clip_any(grads.tensors, outs.tensors, max_norm, norm_type)
+    return _clip_any(grads, outs, max_norm, norm_type)
+
+
+def _check_any(grads: _Listed, outs: _Listed) -> None:
+    """What ``_run`` checks of tensors without gaps, of tensors in any layout."""
+    same, live = grads.at == outs.at, grads.count > 0
+    if (same & live & (grads.kind != outs.kind)).any():
+        raise ValueError("a gradient cannot be scaled in place into another type")
+    writes, reads = np.flatnonzero(live), np.flatnonzero(live & ~same)
+
+    gaps = []  # layouts of the tensors that are written and not contiguous
+
+    def ends(listed):
+        to = listed.at + listed.count * _BYTES[listed.kind]
+        for i in np.flatnonzero(~np.fromiter(map(_whole, listed.tensors), bool, len(to)) & live):
+            layout = _layout(listed.tensors[i])
+            to[i] = _end(*layout)
+            if listed is outs:
+                gaps.append(layout)
+        return to
+
+    starts, to = outs.at[writes], ends(outs)[writes]
+    if len(reads):
+        starts, to = np.concatenate((starts, grads.at[reads])), np.concatenate((to, ends(grads)[reads]))
+    order = np.argsort(starts)
+    if (np.maximum.accumulate(to[order])[:-1] > starts[order][1:]).any():  # one reaches into another: they may still pass by one another
+        bad = _collide([outs.tensors[i] for i in writes], [grads.tensors[i] for i in reads])
+    else:
+        bad = any(_folded(*layout) for layout in gaps)
+    if bad:
+        raise ValueError("the tensors that are written overlap one another or a gradient that is read")
 
 
 @torch.no_grad()
-def _clip_any(grads, outs, max_norm, norm_type):
+def _clip_any(grads: _Listed, outs: _Listed, max_norm, norm_type):
     """The kernel goes through memory: a tensor that is no run of it, or is ordered unlike its output, is taken through a copy."""
-    pairs = [(g, o) for g, o in zip(grads, outs) if g.numel() > 0]
-    if any(g.data_ptr() == o.data_ptr() and g.dtype != o.dtype for g, o in pairs):
-        raise ValueError("a gradient cannot be scaled in place into another type")
-    if _collide([o for _, o in pairs], [g for g, o in pairs if g.data_ptr() != o.data_ptr()]):
-        raise ValueError("the tensors that are written overlap one another or a gradient that is read")
+    _check_any(grads, outs)
+    grads, outs = grads.tensors, outs.tensors
     reads, writes, back = [], [], []
-    for g, o in pairs:
+    for g, o in zip(grads, outs):
+        if g.numel() == 0:
+            continue
         if (g.is_contiguous() and o.is_contiguous()) or (_dense(g) and _dense(o) and g.stride() == o.stride()):
             reads.append(g)
             writes.append(o)
@@ -246,7 +279,8 @@ def _clip_any(grads, outs, max_norm, norm_type):
             back.append((o, writes[-1]))
     if not reads:
         return grads[0].new_zeros((), dtype=torch.float32)
-    norm = _run(_Listed(reads, "clip_grads_"), _Listed(writes, "clip_grads_"), max_norm, norm_type)
+    into = _Listed(writes, "clip_grads_")
+    norm = _run(into if all(map(operator.is_, reads, writes)) else _Listed(reads, "clip_grads_"), into, max_norm, norm_type)
     for o, scaled in back:
         o.copy_(scaled)
     return norm
