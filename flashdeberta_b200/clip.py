@@ -62,6 +62,8 @@ def _starts(at, run, outer) -> np.ndarray:
     """Where the runs begin, in order."""
     starts = np.array([at], np.int64)
     for stride, size in outer:
+        if stride == 0:  # (the same places again)
+            continue
         starts = (starts[:, None] + stride * np.arange(size, dtype=np.int64)).ravel()
     return np.sort(starts)
 
@@ -70,7 +72,9 @@ def _folded(at, run, outer) -> bool:
     """Whether two elements of a tensor lie in the same place."""
     span = run
     for stride, size in outer:
-        if stride < span:  # (an expanded dimension, or windows that slide)
+        if stride == 0:  # (an expanded dimension)
+            return True
+        if stride < span:  # windows that slide, or rows that pass through one another
             return bool((np.diff(_starts(at, run, outer)) < run).any())
         span += stride * (size - 1)
     return False

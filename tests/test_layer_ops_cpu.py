@@ -222,6 +222,12 @@ def test_elements_in_one_place():
     assert _collide([m.as_strided((5, 4), (2, 3))], []) and not _collide([m.as_strided((3, 2), (2, 3))], [])
 
 
+def test_elements_that_stand_for_many_are_not_counted_out():
+    m = torch.zeros(40)
+    many = m[3:4].expand(10 ** 6, 10 ** 6)
+    assert _collide([many], []) and _collide([m[::3]], [many]) and not _collide([m[::2]], [many])
+
+
 def test_elements_in_one_place_against_a_list_of_them():
     gen = torch.Generator().manual_seed(0)
     pick = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=gen))
