@@ -176,3 +176,34 @@ def test_forward_mode_derivatives_are_refused():
             torch.autograd.grad(ops.residual_norm(leaf, x, w)[0], leaf, fwd.make_dual(one, one))
     with pytest.raises(RuntimeError, match="no forward-mode derivative"):
         torch.func.jvp(lambda v: ops.residual_norm(v, x, w), (x,), (one,))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements through each operator: the last rows as they come out alone."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB of device memory")
+    h, rows = 1000, 2200003
+    gen = torch.Generator(DEV).manual_seed(0)
+    rand = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    x, r, dn, w, b = rand(rows, h).requires_grad_(), rand(rows, h), rand(rows, h), rand(h), rand(h)
+    last = slice(rows - 777, rows)
+    normed, stream = ops.residual_norm(x, r, w, b, post_weight=w, post_bias=b)
+    dx, = torch.autograd.grad(normed, x, dn)
+    x = x.detach()
+    few = x[last].clone().requires_grad_()
+    n, s = ops.residual_norm(few, r[last].clone(), w, b, post_weight=w, post_bias=b)
+    assert torch.equal(normed[last], n) and torch.equal(stream[last], s) and torch.equal(dx[last], torch.autograd.grad(n, few, dn[last].clone())[0])
+    few = few.detach()
+    del normed, stream, dx, dn, r
+    for n, dtype in ((1024, torch.bfloat16), (1001, torch.float32)):
+        wq, ws = ops.quantize_int8(torch.randn(n, h, device=DEV))
+        assert torch.equal(ops.linear_int8(x, wq, ws, out_dtype=dtype)[last], ops.linear_int8(few, wq, ws, out_dtype=dtype))
+    assert all(torch.equal(a[last], c) for a, c in zip(ops.quantize_int8(x), ops.quantize_int8(few)))
+    want = sum(c.double().square().sum() for c in x.split(100000)).sqrt().item()
+    out = torch.zeros_like(x)
+    assert abs(ops.clip_grads_([x.view(-1)[1:]], 1.0, out=[out.view(-1)[1:]]).item() - want) <= 2.0 ** -17 * want
+    # (a factor of 1 / want up to 2^-18, and a rounding to bf16)
+    assert ((out[last].double() * want - few.double()).abs() <= (2.0 ** -8 + 2.0 ** -17) * few.double().abs()).all()
+    ops.check_status()
+    del x, out
+    torch.cuda.empty_cache()
